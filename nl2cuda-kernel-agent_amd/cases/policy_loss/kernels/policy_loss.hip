@@ -1,0 +1,253 @@
+// Clipped policy loss with a KL term, from logits, for MI355X (gfx950).  C-ABI
+// in include/policy_loss.h, row kernels in csrc/token_rows.h.
+//
+// Three launches: the sum of the weights (left out where the caller gives the
+// denominator), the rows, the sum of their terms.
+
+#include "policy_loss.h"
+#include "token_rows.h"
+
+namespace {
+
+using nl2k::rows::Shape;
+
+constexpr int kSumBlocks = 64;  // most partial sums of the weights: one a lane
+
+// Weight of a row: 0 where its label is ignored, else its mask.
+struct Weights {
+  const void* mask;
+  int kind;
+  __device__ __forceinline__ float at(uint32_t r, int64_t lab, int64_t ignore) const {
+    if (lab == ignore) return 0.f;
+    if (kind == 0) return 1.f;
+    if (kind == 1) return static_cast<const unsigned char*>(mask)[r] ? 1.f : 0.f;
+    return static_cast<const float*>(mask)[r];
+  }
+};
+
+__device__ __forceinline__ double block_sum(double v, double* red) {
+  v = nl2k::wave_sum(v);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) red[wave] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[i];
+  return s;
+}
+
+__global__ __launch_bounds__(1024) void weight_sum_kernel(const int64_t* __restrict__ labels,
+                                                          Weights w, uint32_t rows, int64_t ignore,
+                                                          double* __restrict__ partial) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (uint32_t r = blockIdx.x * 1024 + threadIdx.x; r < rows; r += gridDim.x * 1024)
+    s += w.at(r, labels[r], ignore);
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// 1 / D, or 0 where the weights sum to 0; the same in every lane of a wave.
+__device__ __forceinline__ float inv_denominator(float denom, const double* __restrict__ partial,
+                                                 int blocks) {
+  if (denom > 0.f) return 1.f / denom;
+  const int lane = threadIdx.x & 63;
+  const double d = nl2k::wave_sum(lane < blocks ? partial[lane] : 0.0);
+  return d != 0.0 ? (float)(1.0 / d) : 0.f;
+}
+
+__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ terms, uint32_t rows,
+                                                    float denom,
+                                                    const double* __restrict__ partial, int blocks,
+                                                    float* __restrict__ loss) {
+  __shared__ double red[16];
+  const float inv = inv_denominator(denom, partial, blocks);
+  double s = 0.0;
+  for (uint32_t r = threadIdx.x; r < rows; r += 1024) s += terms[r];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) loss[0] = (float)(s * inv);
+}
+
+struct PolicyOp {
+  const float* __restrict__ old_logp;
+  const float* __restrict__ adv;
+  int64_t adv_bs, adv_ss;
+  const float* __restrict__ ref;
+  Weights w;
+  float lo, hi, kl_coef, denom;
+  const double* __restrict__ partial;
+  int blocks;
+  float* __restrict__ terms;
+  float* __restrict__ logp;
+  float* __restrict__ coef;
+
+  __device__ bool counts(const Shape& sh, uint32_t r, int64_t lab) const {
+    return w.at(r, lab, sh.ignore) != 0.f;
+  }
+  __device__ void skip(uint32_t r, bool lead) const {
+    if (!lead) return;
+    terms[r] = 0.f;
+    logp[r] = 0.f;
+    if (coef) coef[r] = 0.f;
+  }
+  __device__ float finish(const Shape& sh, uint32_t r, float lp, bool lead) const {
+    const uint32_t b = sh.S == sh.rows ? 0u : r / sh.S;
+    const float a = adv[(int64_t)b * adv_bs + (int64_t)(r - b * sh.S) * adv_ss];
+    const float weight = w.kind == 2 ? static_cast<const float*>(w.mask)[r] : 1.f;
+    const float ratio = expf(lp - old_logp[r]);
+    // selects that let a NaN through, as the products do
+    const float cut = ratio < lo ? lo : ratio > hi ? hi : ratio;
+    const float free_term = ratio * a, cut_term = cut * a;
+    const bool held = a >= 0.f ? ratio > hi : ratio < lo;  // the clamp holds the minimum
+    float term = held ? -cut_term : -free_term;
+    float g = held ? 0.f : -free_term;
+    if (ref) {
+      const float d = ref[r] - lp;
+      const float e = expm1f(d);
+      term += kl_coef * (e - d);
+      g -= kl_coef * e;
+    }
+    if (lead) {
+      terms[r] = weight * term;
+      logp[r] = lp;
+    }
+    g *= weight * inv_denominator(denom, partial, blocks);
+    if (lead && coef) coef[r] = g;
+    return g;
+  }
+};
+
+int sum_blocks(int64_t rows) {
+  return (int)std::min<int64_t>(kSumBlocks, nl2k::ceil_div(rows, (int64_t)4096));
+}
+
+size_t workspace_bytes_of(int64_t rows) { return kSumBlocks * 8 + (size_t)(rows + 1) / 2 * 8; }
+
+struct Call {
+  Shape sh;
+  PolicyOp op;
+};
+
+// Checks what both forwards take and fills in the op.
+int make_call(const char* what, const void* logits, int dtype, const int64_t* labels,
+              const float* old_logp, const float* adv, int64_t adv_bs, int64_t adv_ss,
+              const float* ref, const void* mask, int mask_kind, float* loss, float* logp,
+              int64_t B, int64_t S, int64_t V, int64_t bs, int64_t rs, int64_t ignore,
+              float temperature, float clip_low, float clip_high, float kl_coef, float denom,
+              void* ws, size_t ws_bytes, Call* c) {
+  int st = nl2k::rows::make_shape(B, S, V, bs, rs, ignore, temperature, dtype, &c->sh);
+  if (st) return st;
+  if (!loss) return nl2k::fail(NL2K_ERR_NULL, "%s: loss is required", what);
+  if (mask_kind < 0 || mask_kind > 2)
+    return nl2k::fail(NL2K_ERR_VALUE, "%s: mask_kind must be 0, 1 or 2, got %d", what, mask_kind);
+  if (!(clip_low >= 0.f) || !(clip_low <= 1.f) || !(clip_high >= 0.f) || !(clip_high < INFINITY))
+    return nl2k::fail(NL2K_ERR_VALUE,
+                      "%s: clip_low must be in [0, 1] and clip_high at least 0, got %g and %g",
+                      what, (double)clip_low, (double)clip_high);
+  if (!(kl_coef >= 0.f) || !(kl_coef < INFINITY))
+    return nl2k::fail(NL2K_ERR_VALUE, "%s: kl_coef must be finite and at least 0, got %g", what,
+                      (double)kl_coef);
+  if (!(denom >= 0.f) || !(denom < INFINITY))
+    return nl2k::fail(NL2K_ERR_VALUE, "%s: denom must be finite and positive, or 0 for the sum of "
+                      "the weights, got %g", what, (double)denom);
+  if (kl_coef > 0.f && !ref && c->sh.rows)
+    return nl2k::fail(NL2K_ERR_NULL, "%s: kl_coef %g needs ref_logp", what, (double)kl_coef);
+  if (c->sh.rows && (!logits || !labels || !old_logp || !adv || !logp || (mask_kind && !mask)))
+    return nl2k::fail(NL2K_ERR_NULL, "%s: a required pointer is NULL", what);
+  if (ws_bytes < workspace_bytes_of(c->sh.rows) || !ws)
+    return nl2k::fail(NL2K_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs %zu", what, ws_bytes,
+                      workspace_bytes_of(c->sh.rows));
+  if ((st = nl2k::rows::check_align(ws, 0, "workspace", 8))) return st;
+  if ((st = nl2k::rows::check_align(logits, dtype, "logits"))) return st;
+  double* partial = static_cast<double*>(ws);
+  c->op = PolicyOp{old_logp, adv, adv_bs, adv_ss, kl_coef > 0.f ? ref : nullptr,
+                   Weights{mask, mask_kind}, 1.f - clip_low, 1.f + clip_high, kl_coef, denom,
+                   partial, sum_blocks(c->sh.rows), reinterpret_cast<float*>(partial + kSumBlocks),
+                   logp, nullptr};
+  return NL2K_SUCCESS;
+}
+
+void sum_weights(const int64_t* labels, const Call& c, hipStream_t stream) {
+  if (c.op.denom > 0.f || c.op.blocks == 0) return;
+  hipLaunchKernelGGL(weight_sum_kernel, dim3(c.op.blocks), dim3(1024), 0, stream, labels, c.op.w,
+                     c.sh.rows, c.sh.ignore, const_cast<double*>(c.op.partial));
+}
+
+int sum_loss(const Call& c, float* loss, hipStream_t stream) {
+  hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, stream, c.op.terms, c.sh.rows,
+                     c.op.denom, c.op.partial, c.op.blocks, loss);
+  return nl2k::check_launch("loss_kernel");
+}
+
+}  // namespace
+
+extern "C" size_t policy_loss_workspace_bytes(int64_t B, int64_t S) {
+  if (B < 0 || S < 0 || (S && B > ((int64_t)1 << 28) / S)) return 0;
+  return workspace_bytes_of(B * S);
+}
+
+extern "C" int policy_loss_forward(const void* logits, int dtype, const int64_t* labels,
+                                   const float* old_logp, const float* advantages, int64_t adv_bs,
+                                   int64_t adv_ss, const float* ref_logp, const void* mask,
+                                   int mask_kind, float* loss, float* logp, float* stats,
+                                   float* coef, int64_t B, int64_t S, int64_t V,
+                                   int64_t batch_stride, int64_t row_stride, int64_t ignore_index,
+                                   float temperature, float clip_low, float clip_high,
+                                   float kl_coef, float denom, void* workspace,
+                                   size_t workspace_bytes, hipStream_t stream) {
+  Call c;
+  int st = make_call("policy_loss_forward", logits, dtype, labels, old_logp, advantages, adv_bs,
+                     adv_ss, ref_logp, mask, mask_kind, loss, logp, B, S, V, batch_stride,
+                     row_stride, ignore_index, temperature, clip_low, clip_high, kl_coef, denom,
+                     workspace, workspace_bytes, &c);
+  if (st) return st;
+  if ((stats == nullptr) != (coef == nullptr))
+    return nl2k::fail(NL2K_ERR_NULL, "policy_loss_forward: stats and coef come together");
+  if ((st = nl2k::rows::check_align(stats, 0, "stats", 8))) return st;
+  c.op.coef = coef;
+  if (c.sh.rows) {
+    sum_weights(labels, c, stream);
+    st = nl2k::rows::launch_forward(logits, dtype, labels, reinterpret_cast<nl2k::f32x2*>(stats),
+                                    c.sh, c.op, stream);
+    if (st) return st;
+  }
+  return sum_loss(c, loss, stream);
+}
+
+extern "C" int policy_loss_backward(const void* logits, int dtype, const int64_t* labels,
+                                    const float* stats, const float* coef, const float* gout,
+                                    void* dlogits, int64_t B, int64_t S, int64_t V,
+                                    int64_t batch_stride, int64_t row_stride,
+                                    int64_t ignore_index, float temperature, hipStream_t stream) {
+  return nl2k::rows::backward("policy_loss_backward", logits, dtype, labels, stats, coef, gout,
+                              dlogits, B, S, V, batch_stride, row_stride, ignore_index,
+                              temperature, stream);
+}
+
+extern "C" int policy_loss_and_grad(const void* logits, int dtype, const int64_t* labels,
+                                    const float* old_logp, const float* advantages, int64_t adv_bs,
+                                    int64_t adv_ss, const float* ref_logp, const void* mask,
+                                    int mask_kind, float* loss, float* logp, void* dlogits,
+                                    int64_t B, int64_t S, int64_t V, int64_t batch_stride,
+                                    int64_t row_stride, int64_t ignore_index, float temperature,
+                                    float clip_low, float clip_high, float kl_coef, float denom,
+                                    void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Call c;
+  int st = make_call("policy_loss_and_grad", logits, dtype, labels, old_logp, advantages, adv_bs,
+                     adv_ss, ref_logp, mask, mask_kind, loss, logp, B, S, V, batch_stride,
+                     row_stride, ignore_index, temperature, clip_low, clip_high, kl_coef, denom,
+                     workspace, workspace_bytes, &c);
+  if (st) return st;
+  if (c.sh.rows) {
+    if (!dlogits)
+      return nl2k::fail(NL2K_ERR_NULL, "policy_loss_and_grad: dlogits is required");
+    if ((st = nl2k::rows::check_align(dlogits, dtype, "dlogits"))) return st;
+    if (dlogits == logits && (row_stride != V || (B > 1 && batch_stride != S * V)))
+      return nl2k::fail(NL2K_ERR_SHAPE, "policy_loss_and_grad: in place needs dense logits");
+    sum_weights(labels, c, stream);
+    st = nl2k::rows::launch_fused(logits, dtype, labels, dlogits, c.sh, c.op, stream);
+    if (st) return st;
+  }
+  return sum_loss(c, loss, stream);
+}
+
+extern "C" const char* policy_loss_last_error(void) { return nl2k::error_slot().text; }

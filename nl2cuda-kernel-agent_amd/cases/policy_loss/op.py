@@ -1,0 +1,217 @@
+"""Clipped policy loss with a KL term: autograd wrapper over the HIP library
+(kernels/policy_loss.hip).
+
+``policy_loss`` is the differentiable loss: its forward reads the logits once,
+its backward once more.  ``policy_loss_and_grad`` gives the loss and its
+gradient with the logits read once, and in their place if asked: hand the
+gradient on with ``logits.backward(dlogits)``.  There is no CPU path: without a
+GPU the library refuses to load.
+"""
+
+import functools
+import os
+
+import torch
+
+from framework import capi, token_rows
+from framework.loader import load_kernel
+
+KERNEL_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kernels")
+LIB_NAME = "policy_loss_hip"
+SOURCES = ["policy_loss.hip"]
+
+
+def bind_library(lib):
+    V, I64, I, F, S = capi.c_void_p, capi.c_int64, capi.c_int, capi.c_float, capi.c_size_t
+    rows = [I64, I64, I64, I64, I64, I64, F]
+    given = [V, I, V, V, V, I64, I64, V, V, I]
+    scalars = [F, F, F, F, V, S, V]
+    capi.bind(lib, "policy_loss_workspace_bytes", [I64, I64], S)
+    capi.bind(lib, "policy_loss_forward", given + [V, V, V, V] + rows + scalars)
+    capi.bind(lib, "policy_loss_backward", [V, I, V, V, V, V, V] + rows + [V])
+    capi.bind(lib, "policy_loss_and_grad", given + [V, V, V] + rows + scalars)
+    capi.bind_last_error(lib, "policy_loss_last_error")
+    return lib
+
+
+@functools.lru_cache(maxsize=1)
+def _lib():
+    return bind_library(load_kernel(LIB_NAME, SOURCES, base_dir=KERNEL_DIR))
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B, S):
+    return _lib().policy_loss_workspace_bytes(B, S)
+
+
+def _given(labels, old_logp, advantages, ref_logp, mask):
+    """What comes with the logits, as the C entries take it: (tensors to keep
+    until the call, arguments)."""
+    shape = labels.shape
+    labels = labels.contiguous()
+    old = token_rows.per_token(old_logp, "old_logp", shape)
+    ref = None if ref_logp is None else token_rows.per_token(ref_logp, "ref_logp", shape)
+    capi.require(advantages.dtype == torch.float32, "advantages must be float32")
+    adv = advantages
+    if adv.shape != shape:
+        try:  # one a sequence: [B] or [B, 1]
+            adv = (adv.unsqueeze(-1) if adv.dim() == 1 and len(shape) == 2 and
+                   adv.size(0) == shape[0] else adv).expand(shape)
+        except RuntimeError:
+            raise RuntimeError(f"advantages must broadcast to the labels' shape {tuple(shape)}, "
+                               f"got {tuple(advantages.shape)}") from None
+    if len(shape) == 2:
+        adv_bs, adv_ss = adv.stride()
+    elif len(shape) == 1:
+        adv_bs, adv_ss = 0, adv.stride(0)
+    else:
+        adv = adv.contiguous()
+        adv_bs, adv_ss = 0, 1
+    kind = 0
+    if mask is not None:
+        capi.require(mask.dtype in (torch.bool, torch.uint8, torch.float32),
+                     "mask must be bool, uint8 or float32")
+        kind = 2 if mask.dtype == torch.float32 else 1
+        try:
+            mask = mask.expand(shape).contiguous()
+        except RuntimeError:
+            raise RuntimeError(f"mask must broadcast to the labels' shape {tuple(shape)}, "
+                               f"got {tuple(mask.shape)}") from None
+    args = (labels.data_ptr(), old.data_ptr(), adv.data_ptr(), adv_bs, adv_ss,
+            0 if ref is None else ref.data_ptr(), 0 if mask is None else mask.data_ptr(), kind)
+    return (labels, old, adv, ref, mask), args
+
+
+def _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom):
+    token_rows.check(logits, labels, ("old_logp", old_logp), ("advantages", advantages),
+                     ("ref_logp", ref_logp), ("mask", mask))
+    capi.require(kl_coef == 0.0 or ref_logp is not None, "kl_coef needs ref_logp")
+    capi.require(denom is None or denom > 0, "denom must be positive")
+
+
+def loss_forward(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *, clip_low=0.2,
+                 clip_high=0.2, kl_coef=0.0, temperature=1.0, denom=None, ignore_index=-100,
+                 keep_stats=False):
+    """(loss, logp, stats, coef); stats and coef are for ``loss_backward``
+    (None unless ``keep_stats``)."""
+    _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
+    lib = _lib()
+    x, B, S, V, bs, rs = token_rows.layout(logits)
+    keep, given = _given(labels, old_logp, advantages, ref_logp, mask)
+    ws_bytes = _workspace_bytes(B, S)
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=logits.device)
+    loss, logp = ws.new_empty(()), ws.new_empty(labels.shape)
+    stats = coef = None
+    if keep_stats:
+        stats, coef = ws.new_empty(labels.shape + (2,)), ws.new_empty(labels.shape)
+    st = capi.launch(lib.policy_loss_forward, logits.get_device(), x.data_ptr(),
+                     token_rows.DTYPES[x.dtype], *given, loss.data_ptr(), logp.data_ptr(),
+                     stats.data_ptr() if keep_stats else 0, coef.data_ptr() if keep_stats else 0,
+                     B, S, V, bs, rs, ignore_index, temperature, clip_low, clip_high, kl_coef,
+                     0.0 if denom is None else denom, ws.data_ptr(), ws_bytes)
+    if st:
+        capi.check(st, lib.policy_loss_last_error, "policy_loss")
+    del keep
+    return loss, logp, stats, coef
+
+
+def loss_backward(logits, labels, stats, coef, gout, temperature=1.0, ignore_index=-100):
+    """dlogits of the loss, times the one-element tensor gout."""
+    token_rows.check(logits, labels, ("stats", stats), ("coef", coef), ("gout", gout))
+    capi.require(gout.dtype == torch.float32 and gout.numel() == 1,
+                 "gout must be a one-element float32 GPU tensor")
+    lib = _lib()
+    x, B, S, V, bs, rs = token_rows.layout(logits)
+    labels = labels.contiguous()
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    st = capi.launch(lib.policy_loss_backward, logits.get_device(), x.data_ptr(),
+                     token_rows.DTYPES[x.dtype], labels.data_ptr(), stats.data_ptr(),
+                     coef.data_ptr(), gout.data_ptr(), dlogits.data_ptr(), B, S, V, bs, rs,
+                     ignore_index, temperature)
+    if st:
+        capi.check(st, lib.policy_loss_last_error, "policy_loss backward")
+    return dlogits
+
+
+class PolicyLossFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, old_logp, advantages, ref_logp, mask, opts):
+        loss, logp, stats, coef = loss_forward(logits, labels, old_logp, advantages, ref_logp,
+                                               mask, keep_stats=True, **opts)
+        ctx.save_for_backward(logits, labels, stats, coef)
+        ctx.scalars = opts["temperature"], opts["ignore_index"]
+        ctx.mark_non_differentiable(logp)
+        ctx.set_materialize_grads(False)
+        return loss, logp
+
+    @staticmethod
+    def backward(ctx, gout, _):
+        if gout is None:
+            return (None,) * 7
+        logits, labels, stats, coef = ctx.saved_tensors
+        return (loss_backward(logits, labels, stats, coef, gout, *ctx.scalars),) + (None,) * 6
+
+
+def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *, clip_low=0.2,
+                clip_high=0.2, kl_coef=0.0, temperature=1.0, denom=None, ignore_index=-100):
+    """(loss, logp): the clipped policy loss, differentiable in the logits, and
+    the tokens' log-probabilities (not differentiable).
+
+    logits [..., V]; labels, old_logp, ref_logp of their leading shape;
+    advantages too, or one a sequence ([B] or [B, 1]); mask bool or float32
+    weights.  A token counts unless its label is ``ignore_index`` or its weight
+    0; what it and its other inputs hold then is not looked at.  The weighted
+    terms are divided by ``denom`` (> 0), or by the sum of the weights.
+    """
+    opts = dict(clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, temperature=temperature,
+                denom=denom, ignore_index=ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return PolicyLossFunction.apply(logits, labels, old_logp, advantages, ref_logp, mask, opts)
+    return loss_forward(logits, labels, old_logp, advantages, ref_logp, mask, **opts)[:2]
+
+
+def policy_loss_and_grad(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *,
+                         clip_low=0.2, clip_high=0.2, kl_coef=0.0, temperature=1.0, denom=None,
+                         ignore_index=-100, inplace=False):
+    """(loss, logp, dlogits) of ``policy_loss`` in one pass over the logits,
+    outside autograd.  ``inplace`` writes dlogits over the logits, which must
+    be dense then."""
+    _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
+    lib = _lib()
+    logits = logits.detach()
+    if inplace:
+        capi.require(logits.is_contiguous(), "inplace needs contiguous logits")
+    x, B, S, V, bs, rs = token_rows.layout(logits)
+    keep, given = _given(labels, old_logp, advantages, ref_logp, mask)
+    ws_bytes = _workspace_bytes(B, S)
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=logits.device)
+    loss, logp = ws.new_empty(()), ws.new_empty(labels.shape)
+    dlogits = logits if inplace else torch.empty(logits.shape, dtype=logits.dtype,
+                                                 device=logits.device)
+    st = capi.launch(lib.policy_loss_and_grad, logits.get_device(), x.data_ptr(),
+                     token_rows.DTYPES[x.dtype], *given, loss.data_ptr(), logp.data_ptr(),
+                     dlogits.data_ptr(), B, S, V, bs, rs, ignore_index, temperature, clip_low,
+                     clip_high, kl_coef, 0.0 if denom is None else denom, ws.data_ptr(), ws_bytes)
+    if st:
+        capi.check(st, lib.policy_loss_last_error, "policy_loss_and_grad")
+    del keep
+    return loss, logp, dlogits
+
+
+def _options(params):
+    names = ("clip_low", "clip_high", "kl_coef", "temperature", "denom", "ignore_index")
+    return {k: params[k] for k in names if k in params}
+
+
+def candidate(inputs, params):
+    """Framework candidate contract: inputs={"logits","labels","old_logp",
+    "advantages","ref_logp","mask"} -> scalar loss."""
+    return policy_loss(inputs["logits"], inputs["labels"], inputs["old_logp"],
+                       inputs["advantages"], inputs.get("ref_logp"), inputs.get("mask"),
+                       **_options(params))[0]
+
+
+def forward_only(inputs, params):
+    """Forward without autograd."""
+    with torch.no_grad():
+        return candidate(inputs, params)

@@ -36,6 +36,6 @@ PROTOCOL = Protocol()
 def dtype_of(name):
     """Map a dtype name to a torch dtype (reference: protocol.py:33-36)."""
     import torch
-    return {"float32": torch.float32, "float64": torch.float64,
+    return {"float32": torch.float32, "float64": torch.float64, "bfloat16": torch.bfloat16,
             "float16": torch.float16, "int32": torch.int32,
             "int64": torch.int64}[name]
