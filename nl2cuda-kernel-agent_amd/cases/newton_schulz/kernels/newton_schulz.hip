@@ -380,6 +380,9 @@ struct Scales {
 };
 
 int make_scales(int steps, float a, float b, float c, Scales* s) {
+  if (!(std::fabs(a) < 1e3f && std::fabs(b) < 1e3f && std::fabs(c) < 1e3f))
+    return nl2k::fail(NL2K_ERR_VALUE, "coefficients must be finite and below 1000, got (%g, %g, %g)",
+                      (double)a, (double)b, (double)c);
   double top = 1.0, top_x = 1.0, top_b = 0.0;
   for (int i = 0; i < steps; ++i) {
     double next = 0.0;
