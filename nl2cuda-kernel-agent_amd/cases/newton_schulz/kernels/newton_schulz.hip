@@ -29,45 +29,118 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half_t;
 
 constexpr int kBatch = 32;        // matrices of one launch: their pointers are kernel arguments
-constexpr int kPartials = 256;    // most workgroups that sum a matrix's squares
-constexpr int kStep = 64;         // float16 of a row a tile step takes: 128 bytes
+constexpr int kPartials = 1024;   // most workgroups that sum a matrix's squares
+constexpr int kStep = 64;         // float16 of a row that a stage takes: 128 bytes
 constexpr size_t kMaxBatchBytes = (size_t)4 << 30;
 
 // ------------------------------------------------------------------ elements
-__device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {
-  if (dtype == 0) return static_cast<const float*>(p)[i];
-  const unsigned short h = static_cast<const unsigned short*>(p)[i];
-  if (dtype == 1) return __builtin_bit_cast(float, (uint32_t)h << 16);
-  return (float)__builtin_bit_cast(half_t, h);
+// Eight elements of a user's matrix at any alignment of its own type; of the
+// last ones of a row `count` < 8.
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float widen(unsigned short h, int dtype) {
+  return dtype == 1 ? __builtin_bit_cast(float, (uint32_t)h << 16)
+                    : (float)__builtin_bit_cast(half_t, h);
 }
 
-__device__ __forceinline__ void store_elem(void* p, int64_t i, int dtype, float v) {
-  if (dtype == 0)
-    static_cast<float*>(p)[i] = v;
-  else if (dtype == 1)
-    static_cast<unsigned short*>(p)[i] = __builtin_bit_cast(unsigned short, (__bf16)v);
-  else
-    static_cast<half_t*>(p)[i] = (half_t)v;
+__device__ __forceinline__ unsigned short narrow(float v, int dtype) {
+  return dtype == 1 ? __builtin_bit_cast(unsigned short, (__bf16)v)
+                    : __builtin_bit_cast(unsigned short, (half_t)v);
 }
 
-// Where element t of an operand row lies, in float16 (the second half 32 on).
+__device__ __forceinline__ void load8(const void* p, int64_t at, int dtype, int count,
+                                      float (&v)[8]) {
+  if (dtype == 0) {
+    const float* q = static_cast<const float*>(p) + at;
+    if (count >= 8) {
+      const f32x4 a = *reinterpret_cast<const f32x4_u*>(q);
+      const f32x4 b = *reinterpret_cast<const f32x4_u*>(q + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < count ? q[e] : 0.f;
+    }
+  } else {
+    const unsigned short* q = static_cast<const unsigned short*>(p) + at;
+    u16x8 h;
+    if (count >= 8) {
+      h = __builtin_bit_cast(u16x8, (u32x4)*reinterpret_cast<const u32x4_u*>(q));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = e < count ? q[e] : (unsigned short)0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = widen(h[e], dtype);
+  }
+}
+
+__device__ __forceinline__ void store8(void* p, int64_t at, int dtype, int count,
+                                       const float (&v)[8]) {
+  if (dtype == 0) {
+    float* q = static_cast<float*>(p) + at;
+    if (count >= 8) {
+      *reinterpret_cast<f32x4_u*>(q) = f32x4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4_u*>(q + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) q[e] = v[e];
+    }
+  } else {
+    unsigned short* q = static_cast<unsigned short*>(p) + at;
+    u16x8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = narrow(v[e], dtype);
+    if (count >= 8) {
+      *reinterpret_cast<u32x4_u*>(q) = __builtin_bit_cast(u32x4, h);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) q[e] = h[e];
+    }
+  }
+}
+
+// Eight elements t .. t + 7 of an operand row, t a multiple of 8: in full
+// precision the second halves lie 32 on.
+template <int PL>
+struct Halves {
+  f16x8 h[PL];
+};
+
 template <int PL>
 __device__ __forceinline__ int64_t at(int t) {
   return PL == 1 ? t : (int64_t)(t >> 5) * 64 + (t & 31);
 }
 
 template <int PL>
-__device__ __forceinline__ void put(half_t* row, int t, float v) {
-  const half_t hi = (half_t)v;
-  half_t* p = row + at<PL>(t);
-  p[0] = hi;
-  if (PL == 2) p[32] = (half_t)(v - (float)hi);
+__device__ __forceinline__ Halves<PL> get8(const half_t* row, int t) {
+  Halves<PL> r;
+#pragma unroll
+  for (int p = 0; p < PL; ++p)
+    r.h[p] = *reinterpret_cast<const f16x8*>(row + at<PL>(t) + 32 * p);
+  return r;
 }
 
 template <int PL>
-__device__ __forceinline__ float get(const half_t* row, int t) {
-  const half_t* p = row + at<PL>(t);
-  return PL == 2 ? (float)p[0] + (float)p[32] : (float)p[0];
+__device__ __forceinline__ float value(const Halves<PL>& r, int e) {
+  return PL == 2 ? (float)r.h[0][e] + (float)r.h[PL - 1][e] : (float)r.h[0][e];
+}
+
+template <int PL>
+__device__ __forceinline__ void put8(half_t* row, int t, const float (&v)[8]) {
+  f16x8 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    hi[e] = (half_t)v[e];
+    lo[e] = (half_t)(v[e] - (float)hi[e]);
+  }
+  half_t* p = row + at<PL>(t);
+  *reinterpret_cast<f16x8*>(p) = hi;
+  if (PL == 2) *reinterpret_cast<f16x8*>(p + 32) = lo;
 }
 
 // ------------------------------------------------------------------ prologue
@@ -81,30 +154,44 @@ struct Source {
   int m, n;
 };
 
-// U's element from G and the momentum after its update.
-__device__ __forceinline__ float update_of(const Source& s, float g, float mom) {
-  return s.nesterov ? fmaf(s.mu, mom, g) : mom;
+// U from G and the momentum after its update.
+__device__ __forceinline__ void update_of(const Source& s, float (&g)[8], const float (&mom)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] = s.nesterov ? fmaf(s.mu, mom[e], g[e]) : mom[e];
 }
 
-// Momentum and the sum of U's squares: a partial sum in 64 bits a workgroup.
+// Momentum and the sum of U's squares, a partial sum in 64 bits a workgroup:
+// the squares of 32-bit numbers leave 32 bits on either side.
 __global__ __launch_bounds__(256) void square_kernel(Source s, double* __restrict__ partial) {
   __shared__ double red[4];
   const int b = blockIdx.y;
   const void* g = s.g[b];
   void* mom = s.mom[b];
+  const int groups = (s.n + 7) / 8;  // of eight elements a row
+  const int64_t total = (int64_t)groups * s.m;
   double sum = 0.0;
-  for (int i = blockIdx.x; i < s.m; i += gridDim.x)
-    for (int j = threadIdx.x; j < s.n; j += 256) {
-      float u = load_elem(g, i * s.g_stride + j, s.g_dtype);
-      if (mom) {
-        const int64_t at_m = i * s.m_stride + j;
-        const float x = fmaf(s.mu, load_elem(mom, at_m, s.m_dtype), u);
-        store_elem(mom, at_m, s.m_dtype, x);
-        // the momentum as it is kept, so that U is what a reader of it would form
-        u = update_of(s, u, load_elem(mom, at_m, s.m_dtype));
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total;
+       x += (int64_t)gridDim.x * 256) {
+    const int i = total < (int64_t)1 << 31 ? (uint32_t)x / (uint32_t)groups : (int)(x / groups);
+    const int j = (int)(x - (int64_t)i * groups) * 8;
+    float u[8];
+    load8(g, i * s.g_stride + j, s.g_dtype, s.n - j, u);
+    if (mom) {
+      const int64_t at_m = i * s.m_stride + j;
+      float v[8];
+      load8(mom, at_m, s.m_dtype, s.n - j, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = fmaf(s.mu, v[e], u[e]);
+        // as it is kept, so that U is what a reader of the momentum would form
+        if (s.m_dtype != 0) v[e] = widen(narrow(v[e], s.m_dtype), s.m_dtype);
       }
-      sum += (double)u * u;
+      store8(mom, at_m, s.m_dtype, s.n - j, v);
+      update_of(s, u, v);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += (double)u[e] * u[e];
+  }
   sum = nl2k::wave_sum(sum);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -121,37 +208,55 @@ __global__ __launch_bounds__(256) void scale_kernel(Source s, const double* __re
                                                     int rows_len, int64_t rows_batch,
                                                     half_t* __restrict__ cols, int cols_pitch,
                                                     int cols_len, int64_t cols_batch) {
-  __shared__ float tile[64][65];
+  __shared__ float tile[64][68];
   __shared__ double red[4];
   const int b = blockIdx.z;
-  double q = (int)threadIdx.x < blocks ? partial[(int64_t)b * kPartials + threadIdx.x] : 0.0;
-  q = nl2k::wave_sum(q);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = q;
+  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
+  float u[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int i = i0 + (threadIdx.x >> 3) + 32 * q, j = j0 + (threadIdx.x & 7) * 8;
+    const int count = i < s.m ? s.n - j : 0;
+    if (count > 0) {
+      load8(s.g[b], i * s.g_stride + j, s.g_dtype, count, u[q]);
+      if (s.mom[b]) {
+        float v[8];
+        load8(s.mom[b], i * s.m_stride + j, s.m_dtype, count, v);
+        update_of(s, u[q], v);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[q][e] = e < count ? u[q][e] : 0.f;
+  }
+  double part = 0.0;
+  for (int x = threadIdx.x; x < blocks; x += 256) part += partial[(int64_t)b * kPartials + x];
+  part = nl2k::wave_sum(part);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = part;
   __syncthreads();
-  const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
-  const double f = norm + (double)eps;
+  const double f = sqrt((red[0] + red[1]) + (red[2] + red[3])) + (double)eps;
   // 0 / 0 is an update of zeros; sx / f may pass 32 bits where the elements are small
   const double scale = f > 0.0 ? sx / f : (f == 0.0 ? 0.0 : NAN);
-  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-  const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int r = r0; r < 64; r += 4) {
-    const int i = i0 + r, j = j0 + c;
-    float u = 0.f;
-    if (i < s.m && j < s.n) {
-      u = load_elem(s.g[b], i * s.g_stride + j, s.g_dtype);
-      if (s.mom[b]) u = update_of(s, u, load_elem(s.mom[b], i * s.m_stride + j, s.m_dtype));
-      u = (float)(u * scale);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int r = (threadIdx.x >> 3) + 32 * q, c = (threadIdx.x & 7) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u[q][e] = (float)(u[q][e] * scale);
+      tile[r][c + e] = u[q][e];
     }
-    tile[r][c] = u;
     // rows: [m, n] padded along n to rows_len, cols: [n, m] along m to cols_len
-    if (i < s.m && j < rows_len) put<PL>(rows + b * rows_batch + (int64_t)i * rows_pitch, j, u);
+    if (i0 + r < s.m && j0 + c < rows_len)
+      put8<PL>(rows + b * rows_batch + (int64_t)(i0 + r) * rows_pitch, j0 + c, u[q]);
   }
   __syncthreads();
-#pragma unroll 4
-  for (int r = r0; r < 64; r += 4) {
-    const int j = j0 + r, i = i0 + c;
-    if (j < s.n && i < cols_len) put<PL>(cols + b * cols_batch + (int64_t)j * cols_pitch, i, tile[c][r]);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int c = (threadIdx.x >> 3) + 32 * q, r = (threadIdx.x & 7) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[r + e][c];
+    if (j0 + c < s.n && i0 + r < cols_len)
+      put8<PL>(cols + b * cols_batch + (int64_t)(j0 + c) * cols_pitch, i0 + r, v);
   }
 }
 
@@ -163,14 +268,16 @@ struct Operands {
   int p_rows, q_rows;
   int p_pitch, q_pitch;      // float16 a row
   int64_t p_batch, q_batch;  // float16 a matrix
-  int steps;                 // tile steps along a row
+  int row_bytes;             // of a row, padded
+  int steps;                 // stages that those are
+  int tiles_p, tiles_q;      // tiles of a matrix
+  int tiles;                 // all of them
 };
 
-__device__ __forceinline__ void load_lds16(const half_t* g, char* l) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) void*)g,
-      (__attribute__((address_space(3))) void*)l, 16, 0, 0);
-}
+// What becomes of the sums.  row8 is given eight of a row, turns them into the
+// result and stores it; col8 is given eight of the result down a column, where
+// a transpose is stored too.  `Pre` is what row8 reads from memory, fetched
+// ahead of the sums.
 
 // A symmetric result [n, n], both triangles from the tiles on and below the
 // diagonal: v = alpha acc + beta D.
@@ -182,13 +289,21 @@ struct SymmetricStore {
   int n, pitch, cols;  // cols: n padded to a tile step
   int64_t batch;
   float alpha, beta;
-  __device__ __forceinline__ void operator()(int b, int i, int j, float acc, bool diagonal) const {
-    float v = alpha * acc;
-    const bool in = i < n && j < n;
-    if (in && d) v = fmaf(beta, get<PL>(d + b * batch + (int64_t)i * pitch, j), v);
-    if (!in) v = 0.f;
-    if (i < n && j < cols) put<PL>(c + b * batch + (int64_t)i * pitch, j, v);
-    if (!diagonal && j < n && i < cols) put<PL>(c + b * batch + (int64_t)j * pitch, i, v);
+  using Pre = Halves<PL>;
+  __device__ __forceinline__ Pre fetch(int b, int i, int j) const {
+    Pre r{};
+    if (d && i < n && j < cols) r = get8<PL>(d + b * batch + (int64_t)i * pitch, j);
+    return r;
+  }
+  __device__ __forceinline__ void row8(int b, int i, int j, float (&v)[8], const Pre& pre) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = i < n && j + e < n ? fmaf(beta, value<PL>(pre, e), alpha * v[e]) : 0.f;
+    if (i < n && j < cols) put8<PL>(c + b * batch + (int64_t)i * pitch, j, v);
+  }
+  __device__ __forceinline__ bool columns(bool diagonal) const { return !diagonal; }
+  __device__ __forceinline__ void col8(int b, int i, int j, const float (&v)[8]) const {
+    if (j < n && i < cols) put8<PL>(c + b * batch + (int64_t)j * pitch, i, v);
   }
 };
 
@@ -201,12 +316,21 @@ struct StepStore {
   int k, l, x_pitch, t_pitch, x_cols, t_cols;
   int64_t x_batch, t_batch;
   float alpha, beta;
-  __device__ __forceinline__ void operator()(int b, int i, int j, float acc, bool) const {
-    const bool in = i < k && j < l;
-    half_t* row = x + b * x_batch + (int64_t)i * x_pitch;
-    const float v = in ? fmaf(beta, get<PL>(row, j), alpha * acc) : 0.f;
-    if (i < k && j < x_cols) put<PL>(row, j, v);
-    if (j < l && i < t_cols) put<PL>(xt + b * t_batch + (int64_t)j * t_pitch, i, v);
+  using Pre = Halves<PL>;
+  __device__ __forceinline__ Pre fetch(int b, int i, int j) const {
+    Pre r{};
+    if (i < k && j < x_cols) r = get8<PL>(x + b * x_batch + (int64_t)i * x_pitch, j);
+    return r;
+  }
+  __device__ __forceinline__ void row8(int b, int i, int j, float (&v)[8], const Pre& pre) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = i < k && j + e < l ? fmaf(beta, value<PL>(pre, e), alpha * v[e]) : 0.f;
+    if (i < k && j < x_cols) put8<PL>(x + b * x_batch + (int64_t)i * x_pitch, j, v);
+  }
+  __device__ __forceinline__ bool columns(bool) const { return true; }
+  __device__ __forceinline__ void col8(int b, int i, int j, const float (&v)[8]) const {
+    if (j < l && i < t_cols) put8<PL>(xt + b * t_batch + (int64_t)j * t_pitch, i, v);
   }
 };
 
@@ -218,119 +342,336 @@ struct LastStore {
   const half_t* x;
   int dtype, tall, update;
   int64_t stride;
-  int k, l, x_pitch;
+  int k, l, x_pitch, x_cols;
   int64_t x_batch;
   float alpha, beta, keep, rate;
-  __device__ __forceinline__ void operator()(int b, int i, int j, float acc, bool) const {
-    if (i >= k || j >= l) return;
-    const float v =
-        fmaf(beta, get<PL>(x + b * x_batch + (int64_t)i * x_pitch, j), alpha * acc);
-    const int64_t o = tall ? j * stride + i : i * stride + j;
-    store_elem(out[b], o, dtype,
-               update ? fmaf(-rate, v, keep * load_elem(out[b], o, dtype)) : v);
+  using Pre = Halves<PL>;
+  __device__ __forceinline__ Pre fetch(int b, int i, int j) const {
+    Pre r{};
+    if (i < k && j < x_cols) r = get8<PL>(x + b * x_batch + (int64_t)i * x_pitch, j);
+    return r;
+  }
+  __device__ __forceinline__ void emit(int b, int r, int c, int count, const float (&v)[8]) const {
+    if (count <= 0) return;
+    const int64_t o = r * stride + c;
+    float w[8];
+    if (update) load8(out[b], o, dtype, count, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = update ? fmaf(-rate, v[e], keep * w[e]) : v[e];
+    store8(out[b], o, dtype, count, w);
+  }
+  __device__ __forceinline__ void row8(int b, int i, int j, float (&v)[8], const Pre& pre) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fmaf(beta, value<PL>(pre, e), alpha * v[e]);
+    if (!tall) emit(b, i, j, i < k ? l - j : 0, v);
+  }
+  __device__ __forceinline__ bool columns(bool) const { return tall; }
+  __device__ __forceinline__ void col8(int b, int i, int j, const float (&v)[8]) const {
+    emit(b, j, i, j < l ? k - i : 0, v);
   }
 };
 
-// T x T tiles, four waves of T/2 x T/2, two stages of a tile step in LDS.
-template <int T, int PL, class Store>
-__global__ __launch_bounds__(256) void product_kernel(Operands o, Store store) {
-  constexpr int kRowBytes = kStep * 2;
+// 16 bytes a lane from global memory straight to LDS: lane n's land at lds + 16 n.
+// The count of outstanding loads is waited for by hand (wait_tile): the
+// compiler, which does not know which part of LDS a load writes, would have
+// every read of LDS wait for all of them.
+__device__ __forceinline__ void load_lds16(const half_t* base, uint32_t off, uint32_t lds) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);  // the same in all lanes
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(hi << 32 | lo)
+               : "memory");
+}
+
+// Waits until at most N of this wave's loads are outstanding.
+template <int N>
+__device__ __forceinline__ void wait_tile() {
+  static_assert(N < 64, "the counter has six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0xf70);
+}
+
+// Waits until none of its LDS reads are.
+__device__ __forceinline__ void wait_reads() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+
+// The barrier alone: what it waits for, wait_tile has waited for.  The compiler may move no
+// access across it.
+__device__ __forceinline__ void workgroup_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Between what the lanes of a wave write to its part of LDS and read there: LDS keeps a wave's
+// accesses in order, so the compiler has to keep them too.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// T x T tiles of WM x WN waves, kB x kB matrix products, S stages of 128 bytes a row in LDS.
+template <int T, int WM, int WN, int S, int kB, int PL, class Store>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store store) {
+  constexpr int kWaves = WM * WN;
+  constexpr int kRowBytes = 128;
   constexpr int kStage = 2 * T * kRowBytes;
-  constexpr int kLoads = T / 32;   // 16-byte loads a thread and operand
-  constexpr int W = T / 2 / 16;    // 16 x 16 blocks a wave, each way
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  constexpr int kGroup = 1024 / kRowBytes;           // rows of a wave's load
+  constexpr int kLoads = 2 * T / kGroup / kWaves;    // loads a wave and stage
+  constexpr int BM = T / WM / kB, BN = T / WN / kB;  // kB x kB blocks of a wave
+  constexpr int kK = kB / 16;                        // products of 32 float16 along the rows
+  constexpr int kCols = BN * kB;
+  constexpr int kRegs = kB * kB / 64;
+  typedef float acc_t __attribute__((ext_vector_type(kRegs)));
+  constexpr int kPitch = kCols + 4;       // floats a row where the sums pass through LDS
+  constexpr int kPass = 32 * kPitch * 4;  // bytes a wave needs there: 32 rows at a time
+  constexpr int kLds = S * kStage > kWaves * kPass ? S * kStage : kWaves * kPass;
+  static_assert(T % (kGroup * kWaves) == 0 && BM * kB % 32 == 0 && 32 * kCols / 8 % 64 == 0,
+                "tile shape");
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // Workgroups go round the eight XCDs in turn; each XCD is given tiles that lie next to each
+  // other, so that its L2 holds the rows they share.
+  int x = blockIdx.x;
+  {
+    const int per = o.tiles >> 3, more = o.tiles & 7, xcd = x & 7;
+    x = xcd * per + min(xcd, more) + (x >> 3);
+  }
+  const int one = Store::kSymmetric ? o.tiles_p * (o.tiles_p + 1) / 2 : o.tiles_p * o.tiles_q;
+  const int b = x / one;
+  x -= b * one;
   int ti, tj;
   if (Store::kSymmetric) {
-    const int x = blockIdx.x;
     ti = (int)((sqrtf(8.f * x + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > x) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= x) ++ti;
     tj = x - ti * (ti + 1) / 2;
   } else {
-    ti = blockIdx.x;
-    tj = blockIdx.y;
+    // down four tiles, then across
+    const int band = x / (4 * o.tiles_q), first = band * 4;
+    const int high = min(4, o.tiles_p - first);
+    x -= first * o.tiles_q;
+    tj = x / high;
+    ti = first + x - tj * high;
   }
-  const int b = blockIdx.z;
   const int i0 = ti * T, j0 = tj * T;
 
-  // a wave's load fills eight rows of 128 bytes; the 16-byte pieces of a row are permuted by
-  // its number so that the reads below meet no bank twice
-  const int sub = lane >> 3, piece = (lane & 7) ^ sub;
-  const half_t* src[2 * kLoads];
+  // A wave's load fills 1024 bytes, rows one after the other.  The 16-byte pieces of a row are
+  // permuted by its number so that the rows that a wave reads a piece of at a time lie in
+  // different banks.  Rows past the operand's last are copies of it, whose sums are not stored.
+  auto permuted = [](int piece, int row) {
+    return piece ^ ((kB == 16 ? row : row >> 1) & 7);
+  };
+  const half_t* pbase = o.p + b * o.p_batch + (int64_t)i0 * o.p_pitch;
+  const half_t* qbase = o.q + b * o.q_batch + (int64_t)j0 * o.q_pitch;
+  uint32_t off[kLoads];
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) {
-    const int row = (q * 4 + wave) * 8 + sub;
-    src[q] = o.p + b * o.p_batch + (int64_t)min(i0 + row, o.p_rows - 1) * o.p_pitch + piece * 8;
-    src[kLoads + q] =
-        o.q + b * o.q_batch + (int64_t)min(j0 + row, o.q_rows - 1) * o.q_pitch + piece * 8;
+    const bool second = q >= kLoads / 2;  // P's rows, then Q's
+    const int row = (q % (kLoads / 2) * kWaves + wave) * kGroup + lane / (64 / kGroup);
+    const int last = (second ? o.q_rows - j0 : o.p_rows - i0) - 1;
+    const int pitch = second ? o.q_pitch : o.p_pitch;
+    off[q] = (uint32_t)min(row, last) * (uint32_t)(pitch * 2) +
+             permuted(lane % (64 / kGroup), row) * 16;
   }
-  auto load = [&](int step, int stage) {
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  uint32_t to = lds0 + wave * 1024;  // where the next stage's loads go
+  auto load_some = [&](int from, int upto) {
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
-      char* at_row = lds + stage * kStage + (q * 4 + wave) * 1024;
-      load_lds16(src[q] + (int64_t)step * kStep, at_row);
-      load_lds16(src[kLoads + q] + (int64_t)step * kStep, at_row + T * kRowBytes);
-    }
+    for (int q = 0; q < kLoads; ++q)
+      if (q >= from && q < upto)
+        load_lds16(q < kLoads / 2 ? pbase : qbase, off[q],
+                   __builtin_amdgcn_readfirstlane(to + q * kWaves * 1024));
+  };
+  auto load_next = [&]() {
+    pbase += kRowBytes / 2;
+    qbase += kRowBytes / 2;
+    to += kStage;
+    if (to >= lds0 + S * kStage) to -= S * kStage;
   };
 
-  f32x4 acc[W][W];
+  acc_t acc[BM][BN];
 #pragma unroll
-  for (int x = 0; x < W; ++x)
+  for (int m = 0; m < BM; ++m)
 #pragma unroll
-    for (int y = 0; y < W; ++y) acc[x][y] = nl2k::zero4();
+    for (int n = 0; n < BN; ++n)
+#pragma unroll
+      for (int e = 0; e < kRegs; ++e) acc[m][n][e] = 0.f;
 
-  const int wi = (wave >> 1) * (T / 2), wj = (wave & 1) * (T / 2);
-  const int frag_row = lane & 15;
-  int frag[2];
+  const int wi = (wave / WN) * (T / WM), wj = (wave % WN) * (T / WN);
+  constexpr int kHalves = 2;  // 32 float16 of a row each
+  const char* frag[kHalves * kK];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    frag[h] = frag_row * kRowBytes + (((h * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
-
-  load(0, 0);
-  for (int s = 0; s < o.steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile is in LDS,
-    __syncthreads();                     // then all of it is, and the other stage is free
-    const char* pa = lds + (s & 1) * kStage + wi * kRowBytes;
-    const char* qa = lds + (s & 1) * kStage + (T + wj) * kRowBytes;
-    f16x8 fp[2][W], fq[2][W];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int x = 0; x < W; ++x) {
-        fp[h][x] = *reinterpret_cast<const f16x8*>(pa + x * 16 * kRowBytes + frag[h]);
-        fq[h][x] = *reinterpret_cast<const f16x8*>(qa + x * 16 * kRowBytes + frag[h]);
-      }
-    if (s + 1 < o.steps) load(s + 1, (s + 1) & 1);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int x = 0; x < W; ++x)
-#pragma unroll
-        for (int y = 0; y < W; ++y) {
-          if (PL == 1) {
-            acc[x][y] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[h][x], fq[h][y], acc[x][y], 0, 0, 0);
-          } else if (h == 0) {
-            acc[x][y] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][x], fq[0][y], acc[x][y], 0, 0, 0);
-          } else {
-            acc[x][y] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][x], fq[1][y], acc[x][y], 0, 0, 0);
-            acc[x][y] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[1][x], fq[0][y], acc[x][y], 0, 0, 0);
-          }
-        }
+  for (int h = 0; h < kHalves * kK; ++h) {
+    const int row = lane & (kB - 1);
+    frag[h] = lds + row * kRowBytes + permuted(h * (4 / kK) + lane / kB, row) * 16;
   }
+  auto read = [&](int stage, int h, int row, f16x8& f) {
+    f = *reinterpret_cast<const f16x8*>(frag[h] + stage * kStage + row * kRowBytes);
+  };
+  // A run of products (fp, fq), row by row of blocks; between them, what is needed later is
+  // fetched a little at a time, so that the wave does not stand behind its own requests: the
+  // reads of half h of a stage to (np, nq), and loads from .. upto of a stage in the making.
+  auto run = [&](const f16x8(&fp)[BM * kK], const f16x8(&fq)[BN * kK], bool reads, int stage, int h,
+                 f16x8(&np)[BM * kK], f16x8(&nq)[BN * kK], bool loads, int from, int upto) {
 #pragma unroll
-  for (int x = 0; x < W; ++x)
+    for (int m = 0; m < BM; ++m) {
+      if (reads) {
+        constexpr int R = (BM + BN) * kK;
 #pragma unroll
-    for (int y = 0; y < W; ++y)
+        for (int r = m * R / BM; r < (m + 1) * R / BM; ++r) {
+          if (r < BN * kK)
+            read(stage, h * kK + r % kK, T + wj + r / kK * kB, nq[r < BN * kK ? r : 0]);
+          else
+            read(stage, h * kK + r % kK, wi + (r / kK - BN) * kB, np[r < BN * kK ? 0 : r - BN * kK]);
+        }
+      }
+      if (loads) load_some(from + m * (upto - from) / BM, from + (m + 1) * (upto - from) / BM);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        store(b, i0 + wi + x * 16 + (lane >> 4) * 4 + r, j0 + wj + y * 16 + frag_row,
-              acc[x][y][r], Store::kSymmetric && ti == tj);
+      for (int x = 0; x < kK; ++x)
+#pragma unroll
+        for (int n = 0; n < BN; ++n) {
+          if constexpr (kB == 16)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[m], fq[n], acc[m][n], 0, 0, 0);
+          else
+            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[m * kK + x], fq[n * kK + x],
+                                                               acc[m][n], 0, 0, 0);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Stage s is in LDS once at most the loads of the S - 2 after it are outstanding.  This wave's
+  // reads are done, and after the barrier all waves': the stage read last may be refilled.
+  auto arrive = [&](int s) {
+    __builtin_amdgcn_sched_barrier(0);
+    wait_reads();
+    if (s + S - 1 <= o.steps)
+      wait_tile<(S - 2) * kLoads>();
+    else
+      wait_tile<0>();
+    workgroup_barrier();
+  };
+  // The last reads, of a stage past the last, are of no use and do no harm.
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < o.steps) {
+      load_some(0, kLoads);
+      load_next();
+    }
+  f16x8 p0[BM * kK], q0[BN * kK], p1[BM * kK], q1[BN * kK], q2[BN * kK];
+  arrive(0);
+  bool more = S - 1 < o.steps;  // whether there is a stage to load during this step
+  int stage = 0;
+#pragma unroll
+  for (int m = 0; m < BM * kK; ++m) read(0, m % kK, wi + m / kK * kB, p0[m]);
+#pragma unroll
+  for (int n = 0; n < BN * kK; ++n) read(0, n % kK, T + wj + n / kK * kB, q0[n]);
+  // Loads are issued between the products of a step's runs; with two stages, which leave them
+  // one step to arrive in, all at once.
+  constexpr int kRuns = PL == 2 ? 3 : kHalves;
+  constexpr int kPart = S == 2 ? kLoads : kLoads / kRuns;
+  auto begin = [&]() {
+    if (S == 2 && more) load_some(0, kLoads);
+  };
+  auto next_stage = [&](int s) {
+    if (more) load_next();
+    arrive(s + 1);
+    more = s + S < o.steps;
+    stage = stage + 1 == S ? 0 : stage + 1;
+    begin();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto part = [&](int r) { return S == 2 ? 0 : r == kRuns ? kLoads : r * kPart; };
+  begin();
+  if constexpr (PL == 1) {
+    if (S > 2 && more) load_some(0, part(1));
+    for (int s = 0; s < o.steps; ++s) {
+      wait_reads();
+      run(p0, q0, true, stage, kHalves - 1, p1, q1, more, part(1), part(2));
+      next_stage(s);
+      run(p1, q1, true, stage, 0, p0, q0, more, part(0), part(1));
+    }
+  } else {
+    if (S > 2 && more) load_some(0, part(1));
+    // q: the first halves of Q of this step, nq those of the next
+    auto step = [&](int s, const f16x8(&q)[BN * kK], f16x8(&nq)[BN * kK]) {
+      wait_reads();
+      run(p0, q, true, stage, kHalves - 1, p1, q1, more, part(1), part(2));
+      wait_reads();
+      run(p0, q1, false, 0, 0, p1, q1, more, part(2), part(3));
+      next_stage(s);
+      run(p1, q, true, stage, 0, p0, nq, more, part(0), part(1));
+    };
+    for (int s = 0; s < o.steps; s += 2) {
+      step(s, q0, q2);
+      if (s + 1 < o.steps) step(s + 1, q2, q0);
+    }
+  }
+  wait_reads();
+  __builtin_amdgcn_sched_barrier(0);
+
+  // The sums pass through the wave's own part of LDS, 32 rows at a time, so that rows and
+  // columns of the result leave in 16-byte pieces.
+  float* pass = reinterpret_cast<float*>(lds + wave * kPass);
+  const bool columns = store.columns(Store::kSymmetric && ti == tj);
+  constexpr int kUnits = 32 * kCols / 8 / 64;
+  constexpr int kPasses = BM * kB / 32;
+  typename Store::Pre pre[kPasses][kUnits];
+#pragma unroll
+  for (int m = 0; m < kPasses; ++m)
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at_u = u * 64 + lane;
+      pre[m][u] = store.fetch(b, i0 + wi + m * 32 + at_u / (kCols / 8),
+                              j0 + wj + at_u % (kCols / 8) * 8);
+    }
+#pragma unroll
+  for (int m = 0; m < kPasses; ++m) {
+    const int i = i0 + wi + m * 32, j = j0 + wj;
+#pragma unroll
+    for (int n = 0; n < BN; ++n) {
+      if constexpr (kB == 16) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          pass[(r / 4 * 16 + (lane >> 4) * 4 + r % 4) * kPitch + n * 16 + (lane & 15)] =
+              acc[m * 2 + r / 4][n][r % 4];
+      } else {
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r)
+          pass[(r / 4 * 8 + (lane >> 5) * 4 + r % 4) * kPitch + n * 32 + (lane & 31)] =
+              acc[m][n][r];
+      }
+    }
+    wave_order();
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int at_u = u * 64 + lane, r = at_u / (kCols / 8), c = at_u % (kCols / 8) * 8;
+      float* q = pass + r * kPitch + c;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      store.row8(b, i + r, j + c, v, pre[m][u]);
+      if (columns) {
+        *reinterpret_cast<f32x4*>(q) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(q + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      }
+    }
+    wave_order();
+    if (columns) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int at_u = u * 64 + lane, c = at_u >> 2, r = (at_u & 3) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = pass[(r + e) * kPitch + c];
+        store.col8(b, i + r, j + c, v);
+      }
+      wave_order();
+    }
+  }
 }
 
 // ----------------------------------------------------------------- host side
@@ -357,7 +698,7 @@ int make_plan(int64_t m, int64_t n, int64_t count, int precision, Plan* p) {
                       (long long)m, (long long)n);
   p->k = std::min(m, n);
   p->l = std::max(m, n);
-  const int unit = kStep / precision;  // elements of a tile step
+  const int unit = kStep / precision;  // elements of a stage
   p->kcols = (int)(nl2k::ceil_div(p->k, (int64_t)unit) * unit);
   p->lcols = (int)(nl2k::ceil_div(p->l, (int64_t)unit) * unit);
   p->kp = p->kcols * precision;
@@ -410,20 +751,72 @@ int make_scales(int steps, float a, float b, float c, Scales* s) {
   return NL2K_SUCCESS;
 }
 
+template <int T, int WM, int WN, int S, int kB, int PL, class Store>
+int launch_tiles(Operands o, const Store& store, int nb, hipStream_t stream) {
+  o.steps = o.row_bytes / 128;
+  o.tiles_p = (int)nl2k::ceil_div(o.p_rows, T);
+  o.tiles_q = (int)nl2k::ceil_div(o.q_rows, T);
+  const int64_t tiles = (int64_t)nb * (Store::kSymmetric ? (int64_t)o.tiles_p * (o.tiles_p + 1) / 2
+                                                         : (int64_t)o.tiles_p * o.tiles_q);
+  if (tiles > nl2k::max_blocks(64 * WM * WN) || tiles > INT32_MAX)
+    return nl2k::fail(NL2K_ERR_OVERFLOW, "product of %lld tiles is more than a launch has",
+                      (long long)tiles);
+  o.tiles = (int)tiles;
+  hipLaunchKernelGGL((product_kernel<T, WM, WN, S, kB, PL, Store>), dim3((unsigned)tiles),
+                     dim3(64 * WM * WN), 0, stream, o, store);
+  return nl2k::check_launch("product_kernel");
+}
+
+// Tile shapes and what they were measured to take, in us: a product's fixed part, a stage of a
+// tile alone on its CU, and a stage where all CUs hold `per_cu` of them.  Between those lies a
+// round that is part full; full rounds of large tiles draw the chip's power limit.  More stages
+// in LDS changed nothing (64 x 64: 3, 5 or 9), nor did 64 bytes a row in place of 128.
+struct Shape {
+  int tile, per_cu;
+  double fixed, alone, full;
+};
+constexpr int kShapes = 4;
+constexpr Shape kHalfShapes[kShapes] = {
+    {256, 1, 9.0, 1.13, 1.80}, {192, 1, 8.0, 0.76, 1.31}, {128, 2, 7.0, 0.55, 1.18},
+    {64, 3, 4.0, 0.29, 0.64}};
+constexpr Shape kFullShapes[kShapes] = {  // in full precision 256 x 256 does not fit the registers
+    {0, 0, 0.0, 0.0, 0.0}, {192, 1, 8.0, 0.91, 1.69}, {128, 2, 7.0, 0.63, 1.53},
+    {64, 3, 4.0, 0.31, 0.77}};
+
+// Tiles of a product of matrices p x q; on and below the diagonal where it is symmetric.
+double tiles_of(int64_t p, int64_t q, int tile, bool symmetric, int nb) {
+  const double tp = (double)nl2k::ceil_div(p, (int64_t)tile);
+  const double tq = (double)nl2k::ceil_div(q, (int64_t)tile);
+  return nb * (symmetric ? tp * (tp + 1) / 2 : tp * tq);
+}
+
+// The shape whose rounds over 256 CUs take least.
+int choose(const Shape (&shapes)[kShapes], const Operands& o, bool symmetric, int nb) {
+  int best = -1;
+  double least = 0.0;
+  for (int c = 0; c < kShapes; ++c) {
+    const Shape& s = shapes[c];
+    if (s.tile == 0) continue;
+    const double rounds = tiles_of(o.p_rows, o.q_rows, s.tile, symmetric, nb) / (256 * s.per_cu);
+    const double rest = rounds - std::floor(rounds);
+    const double stage = std::floor(rounds) * s.full +
+                         (rest > 0.0 ? s.alone + (s.full - s.alone) * rest : 0.0);
+    const double time = s.fixed + stage * (o.row_bytes / 128);
+    if (best < 0 || time < least) best = c, least = time;
+  }
+  return best;
+}
+
 template <int PL, class Store>
 int launch_product(const Operands& o, const Store& store, int nb, hipStream_t stream) {
-  auto go = [&](auto tag) {
-    constexpr int T = decltype(tag)::value;
-    const int64_t ti = nl2k::ceil_div(o.p_rows, T), tj = nl2k::ceil_div(o.q_rows, T);
-    const dim3 grid = Store::kSymmetric ? dim3((unsigned)(ti * (ti + 1) / 2), 1, nb)
-                                        : dim3((unsigned)ti, (unsigned)tj, nb);
-    hipLaunchKernelGGL((product_kernel<T, PL, Store>), grid, dim3(256), 0, stream, o, store);
-    return nl2k::check_launch("product_kernel");
-  };
-  const int64_t big = nl2k::ceil_div(o.p_rows, 128) * nl2k::ceil_div(o.q_rows, 128) * nb /
-                      (Store::kSymmetric ? 2 : 1);
-  if (big >= 256) return go(std::integral_constant<int, 128>{});
-  return go(std::integral_constant<int, 64>{});
+  switch (choose(PL == 1 ? kHalfShapes : kFullShapes, o, Store::kSymmetric, nb)) {
+    case 0:
+      if constexpr (PL == 1) return launch_tiles<256, 2, 4, 2, 16, PL>(o, store, nb, stream);
+      break;
+    case 1: return launch_tiles<192, 2, 4, 3, 16, PL>(o, store, nb, stream);
+    case 2: return launch_tiles<128, 2, 2, 2, 32, PL>(o, store, nb, stream);
+  }
+  return launch_tiles<64, 2, 2, 3, 16, PL>(o, store, nb, stream);
 }
 
 struct Job {
@@ -446,7 +839,8 @@ int run_batch(const Job& job, const Plan& p, const Scales& sc, int first, int nb
   half_t* ga = xt2 + (int64_t)p.per * p.xt;
   half_t* gb = ga + (int64_t)p.per * p.a;
   const bool tall = job.src.m > job.src.n;
-  const int blocks = (int)std::min<int64_t>(job.src.m, kPartials);
+  const int blocks = (int)std::min<int64_t>(
+      nl2k::ceil_div((int64_t)job.src.m * nl2k::ceil_div(job.src.n, 8), 256), kPartials);
   hipLaunchKernelGGL(square_kernel, dim3(blocks, nb), dim3(256), 0, stream, job.src, partial);
   int st = nl2k::check_launch("square_kernel");
   if (st) return st;
@@ -460,23 +854,23 @@ int run_batch(const Job& job, const Plan& p, const Scales& sc, int first, int nb
 
   const int k = (int)p.k, l = (int)p.l;
   for (int i = 0; i < job.steps; ++i) {
-    const Operands xx{x, x, k, k, p.lp, p.lp, p.x, p.x, p.lp / kStep};
+    const Operands xx{x, x, k, k, p.lp, p.lp, p.x, p.x, p.lp * 2};
     st = launch_product<PL>(
         xx, SymmetricStore<PL>{ga, nullptr, k, p.kp, p.kcols, p.a, sc.a / (sc.x * sc.x), 0.f}, nb,
         stream);
     if (st) return st;
-    const Operands aa{ga, ga, k, k, p.kp, p.kp, p.a, p.a, p.kp / kStep};
+    const Operands aa{ga, ga, k, k, p.kp, p.kp, p.a, p.a, p.kp * 2};
     st = launch_product<PL>(
         aa, SymmetricStore<PL>{gb, ga, k, p.kp, p.kcols, p.a, job.c * sc.b / (sc.a * sc.a),
                                job.b * sc.b / sc.a}, nb, stream);
     if (st) return st;
-    const Operands bx{gb, xt, k, l, p.kp, p.kp, p.a, p.xt, p.kp / kStep};
+    const Operands bx{gb, xt, k, l, p.kp, p.kp, p.a, p.xt, p.kp * 2};
     if (i + 1 < job.steps) {
       st = launch_product<PL>(
           bx, StepStore<PL>{x, xt2, k, l, p.lp, p.kp, p.lcols, p.kcols, p.x, p.xt, 1.f / sc.b,
                             job.a}, nb, stream);
     } else {
-      LastStore<PL> last{{}, x, job.out_dtype, tall, job.update, job.out_stride, k, l, p.lp, p.x,
+      LastStore<PL> last{{}, x, job.out_dtype, tall, job.update, job.out_stride, k, l, p.lp, p.lcols, p.x,
                          1.f / (sc.b * sc.x), job.a / sc.x, job.keep, job.rate};
       for (int q = 0; q < nb; ++q) last.out[q] = job.out[first + q];
       st = launch_product<PL>(bx, last, nb, stream);
