@@ -104,6 +104,18 @@ __device__ __forceinline__ void store8(void* p, int64_t at, int dtype, int count
   }
 }
 
+__device__ __forceinline__ float load1(const void* p, int64_t at, int dtype) {
+  return dtype == 0 ? static_cast<const float*>(p)[at]
+                    : widen(static_cast<const unsigned short*>(p)[at], dtype);
+}
+
+__device__ __forceinline__ void store1(void* p, int64_t at, int dtype, float v) {
+  if (dtype == 0)
+    static_cast<float*>(p)[at] = v;
+  else
+    static_cast<unsigned short*>(p)[at] = narrow(v, dtype);
+}
+
 // Eight elements t .. t + 7 of an operand row, t a multiple of 8: in full
 // precision the second halves lie 32 on.
 template <int PL>
@@ -674,6 +686,245 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   }
 }
 
+// ------------------------------------------------------------ a short side
+// Where k is at most 64 the products of a step are too small for the chip, and their launches
+// are most of the time.  There the steps go over the Gram matrix alone: with P = a + b A + c A A,
+// X becomes P X, so A becomes P A P and, of all steps, O = P_last .. P_1 X_0 = Q X_0.  Three
+// launches: G = U U' (||U||_F^2 is its trace), Q in one workgroup's LDS, Q U.  A rounding of A in
+// the directions that X_0 hardly has grows by a^2 a step, where the products of X keep A = X X'
+// whole; so all of this is in 64 bits, and a^(2 steps) is bounded (kGramGrowth).  Against the
+// tiles, us: 32 x 200 fp32 74 -> 28, 64 x 2000 96 -> 48.
+constexpr int kGram = 64;
+constexpr double kGramGrowth = 1e9;  // times 2^-53: 1e-7 of a step's polynomial
+constexpr int kGramBlocks = 32;      // most workgroups that sum a Gram matrix
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// U's columns j0 .. j0 + 63 (rows, where U is tall) into LDS, zeros past its edges.  The momentum
+// is updated on the way if `first` is set.
+// Row r, column c at tile[r][c], or tile[c][r].
+template <int KP, bool kByColumn, class Tile>
+__device__ __forceinline__ void load_block(const Source& s, int b, int j0, bool first,
+                                           Tile& tile) {
+  const bool tall = s.m > s.n;
+  const int k = tall ? s.n : s.m, l = tall ? s.m : s.n;
+  const void* g = s.g[b];
+  void* mom = s.mom[b];
+#pragma unroll
+  for (int q = 0; q < KP * 64 / 256; ++q) {
+    const int x = q * 256 + threadIdx.x;
+    const int r = tall ? x % KP : x / 64, c = tall ? x / KP : x % 64;
+    const int j = j0 + c;
+    float u = 0.f;
+    if (r < k && j < l) {
+      const int row = tall ? j : r, col = tall ? r : j;
+      u = load1(g, row * s.g_stride + col, s.g_dtype);
+      if (mom) {
+        const int64_t at_m = row * s.m_stride + col;
+        float v = load1(mom, at_m, s.m_dtype);
+        if (first) {
+          v = fmaf(s.mu, v, u);
+          if (s.m_dtype != 0) v = widen(narrow(v, s.m_dtype), s.m_dtype);
+          store1(mom, at_m, s.m_dtype, v);
+        }
+        u = s.nesterov ? fmaf(s.mu, v, u) : v;
+      }
+    }
+    tile[kByColumn ? c : r][kByColumn ? r : c] = u;
+  }
+}
+
+// A 16 x 16 block of lhs rhs' in 64 bits, sums over `len` columns: lane n reads row n % 16 of both
+// and gets rows n / 16 + 4 r of column n % 16 in element r.
+template <int len, class L, class R>
+__device__ __forceinline__ f64x4 block64(const L* lhs, int lhs_pitch, const R* rhs, int rhs_pitch,
+                                         f64x4 acc) {
+  const int lane = threadIdx.x & 63;
+  const L* p = lhs + (lane & 15) * lhs_pitch + (lane >> 4);
+  const R* q = rhs + (lane & 15) * rhs_pitch + (lane >> 4);
+#pragma unroll
+  for (int t = 0; t < len; t += 4)
+    acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)p[t], (double)q[t], acc, 0, 0, 0);
+  return acc;
+}
+
+// Block x on or below the diagonal, row by row of blocks.
+__device__ __forceinline__ void below(int x, int& ti, int& tj) {
+  ti = 0;
+  while ((ti + 1) * (ti + 2) / 2 <= x) ++ti;
+  tj = x - ti * (ti + 1) / 2;
+}
+
+template <int KP>
+__global__ __launch_bounds__(256) void gram_kernel(Source s, double* __restrict__ partial) {
+  __shared__ float tile[KP][65];
+  constexpr int kBlocks = KP / 16 * (KP / 16 + 1) / 2, kEach = (kBlocks + 3) / 4;
+  const int l = max(s.m, s.n);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  f64x4 acc[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) acc[e] = f64x4{0.0, 0.0, 0.0, 0.0};
+  for (int j0 = blockIdx.x * 64; j0 < l; j0 += gridDim.x * 64) {
+    __syncthreads();
+    load_block<KP, false>(s, blockIdx.y, j0, true, tile);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      int ti, tj;
+      below(min(wave + 4 * e, kBlocks - 1), ti, tj);
+      acc[e] = block64<64>(&tile[ti * 16][0], 65, &tile[tj * 16][0], 65, acc[e]);
+    }
+  }
+  double* out = partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * KP * KP;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    int ti, tj;
+    below(min(wave + 4 * e, kBlocks - 1), ti, tj);
+    if (wave + 4 * e < kBlocks) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = ti * 16 + (lane >> 4) + 4 * r, j = tj * 16 + (lane & 15);
+        if (i >= j) {
+          out[i * KP + j] = acc[e][r];
+          out[j * KP + i] = acc[e][r];
+        }
+      }
+    }
+  }
+}
+
+// Q / (||U||_F + eps) of one matrix.  The operands are symmetric and commute; a wave takes a
+// 16 x 16 block on or below the diagonal of each product and writes it to both sides.
+template <int KP>
+__global__ __launch_bounds__(64 * (KP / 16) * (KP / 16)) void polynomial_kernel(
+    const double* __restrict__ partial, int blocks, double* __restrict__ out, int steps, double a,
+    double b, double c, double eps) {
+  constexpr int R = KP / 16, kThreads = 64 * R * R, kPitch = KP + 1;
+  __shared__ double A[KP * kPitch], P[KP * kPitch], Q[KP * kPitch];
+  __shared__ double trace;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int ti, tj;
+  below(wave, ti, tj);
+  const bool active = ti < R;
+  {
+    const int x = 4 * threadIdx.x;  // KP * KP elements, four a thread
+    const f64x4* g = reinterpret_cast<const f64x4*>(partial + (int64_t)blockIdx.x * blocks * KP *
+                                                                  KP + x);
+    f64x4 v{0.0, 0.0, 0.0, 0.0};
+#pragma unroll 8
+    for (int i = 0; i < blocks; ++i) v += g[(int64_t)i * (KP * KP / 4)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) A[x / KP * kPitch + x % KP + e] = v[e];
+  }
+  static_assert(4 * kThreads == KP * KP, "four elements a thread");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double v = 0.0;
+    for (int i = 0; i < KP; ++i) v += A[i * kPitch + i];
+    trace = v;
+  }
+  __syncthreads();
+  const double f = sqrt(trace) + eps;
+  const double inv = f > 0.0 ? 1.0 / f : (f == 0.0 ? 0.0 : NAN);
+  for (int x = threadIdx.x; x < KP * KP; x += kThreads) {
+    const int at = x / KP * kPitch + x % KP;
+    A[at] *= inv * inv;
+    Q[at] = x / KP == x % KP ? 1.0 : 0.0;
+  }
+  __syncthreads();
+  auto product = [&](const double* p, const double* q) {
+    const f64x4 zero{0.0, 0.0, 0.0, 0.0};
+    return active ? block64<KP>(p + ti * 16 * kPitch, kPitch, q + tj * 16 * kPitch, kPitch, zero)
+                  : zero;
+  };
+  auto put = [&](double* to, const f64x4& v) {
+    if (active) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = ti * 16 + (lane >> 4) + 4 * r, j = tj * 16 + (lane & 15);
+        if (i >= j) {
+          to[i * kPitch + j] = v[r];
+          to[j * kPitch + i] = v[r];
+        }
+      }
+    }
+    __syncthreads();
+  };
+  for (int s = 0; s < steps; ++s) {
+    f64x4 v = product(A, A);
+    if (active) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = ti * 16 + (lane >> 4) + 4 * r, j = tj * 16 + (lane & 15);
+        v[r] = c * v[r] + b * A[i * kPitch + j] + (i == j ? a : 0.0);
+      }
+    }
+    put(P, v);
+    if (s == 0) {
+      for (int x = threadIdx.x; x < KP * kPitch; x += kThreads) Q[x] = P[x];
+      __syncthreads();
+    } else {
+      v = product(P, Q);
+      __syncthreads();
+      put(Q, v);
+    }
+    if (s + 1 == steps) break;
+    v = product(P, A);
+    __syncthreads();
+    put(A, v);
+    v = product(A, P);
+    __syncthreads();
+    put(A, v);
+  }
+  double* o = out + (int64_t)blockIdx.x * KP * KP;
+  for (int x = threadIdx.x; x < KP * KP; x += kThreads)
+    o[x] = Q[x / KP * kPitch + x % KP] * inv;
+}
+
+// O = Q U for 64 columns of U (rows, where it is tall), or the weights that it updates.
+struct ApplyStore {
+  void* out[kBatch];
+  int dtype, update;
+  int64_t stride;
+  float keep, rate;
+};
+
+template <int KP>
+__global__ __launch_bounds__(256) void apply_kernel(Source s, const double* __restrict__ poly,
+                                                    ApplyStore store) {
+  __shared__ float tile[64][KP + 1];  // U's columns as rows
+  __shared__ double q[KP * (KP + 1)];
+  const bool tall = s.m > s.n;
+  const int k = min(s.m, s.n), l = max(s.m, s.n), b = blockIdx.y, j0 = blockIdx.x * 64;
+  load_block<KP, true>(s, b, j0, false, tile);
+  for (int x = threadIdx.x; x < KP * KP; x += 256)
+    q[x / KP * (KP + 1) + x % KP] = poly[(int64_t)b * KP * KP + x];
+  __syncthreads();  // the result may lie where U did
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int x = 0; x < KP / 16; ++x) {
+    // Q is symmetric: either factor may give the rows.  Neighbouring lanes take neighbouring
+    // elements of the result's rows.
+    const f64x4 zero{0.0, 0.0, 0.0, 0.0};
+    const double* qr = q + x * 16 * (KP + 1);
+    const float* ur = &tile[wave * 16][0];
+    const f64x4 acc = tall ? block64<KP>(ur, KP + 1, qr, KP + 1, zero)
+                           : block64<KP>(qr, KP + 1, ur, KP + 1, zero);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = (lane >> 4) + 4 * r, col = lane & 15;
+      const int i = x * 16 + (tall ? col : row), j = j0 + wave * 16 + (tall ? row : col);
+      if (i < k && j < l) {
+        const int64_t o = tall ? j * store.stride + i : i * store.stride + j;
+        float v = (float)acc[r];
+        if (store.update)
+          v = fmaf(-store.rate, v, store.keep * load1(store.out[b], o, store.dtype));
+        store1(store.out[b], o, store.dtype, v);
+      }
+    }
+  }
+}
+
 // ----------------------------------------------------------------- host side
 struct Plan {
   int64_t k, l;
@@ -682,6 +933,8 @@ struct Plan {
   int64_t x, xt, a;           // float16 of X, X' and A (or B) a matrix
   size_t partials;            // bytes
   int per;                    // matrices a launch
+  int gram;                   // k padded to 16, 32 or 64 where it is that short, else 0
+  int gram_blocks;
   size_t bytes;
 };
 
@@ -711,6 +964,13 @@ int make_plan(int64_t m, int64_t n, int64_t count, int precision, Plan* p) {
       1, std::min<int64_t>({count, kBatch, (int64_t)(kMaxBatchBytes / std::max<size_t>(one, 1))}));
   p->partials = (size_t)p->per * kPartials * sizeof(double);
   p->bytes = p->partials + p->per * one;
+  p->gram = p->k > kGram ? 0 : p->k > 32 ? 64 : p->k > 16 ? 32 : 16;
+  p->gram_blocks = (int)std::min<int64_t>(nl2k::ceil_div(std::max<int64_t>(p->l, 1), 64),
+                                          kGramBlocks);
+  if (p->gram) {  // the steps may ask for either way
+    const size_t square = (size_t)p->gram * p->gram * sizeof(double);
+    p->bytes = std::max(p->bytes, p->per * square * (p->gram_blocks + 1));
+  }
   return NL2K_SUCCESS;
 }
 
@@ -881,6 +1141,26 @@ int run_batch(const Job& job, const Plan& p, const Scales& sc, int first, int nb
   return nl2k::succeed();
 }
 
+template <int KP>
+int run_gram(const Job& job, const Plan& p, int first, int nb, void* workspace,
+             hipStream_t stream) {
+  double* partial = static_cast<double*>(workspace);
+  double* poly = partial + (int64_t)p.per * p.gram_blocks * KP * KP;
+  hipLaunchKernelGGL((gram_kernel<KP>), dim3(p.gram_blocks, nb), dim3(256), 0, stream, job.src,
+                     partial);
+  int st = nl2k::check_launch("gram_kernel");
+  if (st) return st;
+  hipLaunchKernelGGL((polynomial_kernel<KP>), dim3(nb), dim3(64 * (KP / 16) * (KP / 16)), 0,
+                     stream, partial, p.gram_blocks, poly, job.steps, (double)job.a,
+                     (double)job.b, (double)job.c, (double)job.eps);
+  if ((st = nl2k::check_launch("polynomial_kernel"))) return st;
+  ApplyStore store{{}, job.out_dtype, job.update, job.out_stride, job.keep, job.rate};
+  for (int q = 0; q < nb; ++q) store.out[q] = job.out[first + q];
+  hipLaunchKernelGGL((apply_kernel<KP>), dim3((unsigned)nl2k::ceil_div(p.l, (int64_t)64), nb),
+                     dim3(256), 0, stream, job.src, poly, store);
+  return nl2k::check_launch("apply_kernel");
+}
+
 int check_scalars(const char* what, int steps, float eps) {
   if (steps < 1 || steps > 64)
     return nl2k::fail(NL2K_ERR_VALUE, "%s: steps must be from 1 to 64, got %d", what, steps);
@@ -931,8 +1211,15 @@ int run_all(const char* what, Job& job, const void* const* grads, void* const* m
       job.src.g[q] = grads[first + q];
       job.src.mom[q] = momenta ? momenta[first + q] : nullptr;
     }
-    st = precision == 1 ? run_batch<1>(job, p, sc, (int)first, nb, workspace, stream)
-                        : run_batch<2>(job, p, sc, (int)first, nb, workspace, stream);
+    const double growth = std::pow(std::max(1.0, std::fabs((double)job.a)), 2.0 * job.steps);
+    if (p.gram && growth <= kGramGrowth)
+      st = p.gram == 16   ? run_gram<16>(job, p, (int)first, nb, workspace, stream)
+           : p.gram == 32 ? run_gram<32>(job, p, (int)first, nb, workspace, stream)
+                          : run_gram<64>(job, p, (int)first, nb, workspace, stream);
+    else
+      st = precision == 1 ? run_batch<1>(job, p, sc, (int)first, nb, workspace, stream)
+                        
+                          : run_batch<2>(job, p, sc, (int)first, nb, workspace, stream);
     if (st) return st;
   }
   return nl2k::succeed();

@@ -590,7 +590,7 @@ inline int launch_forward(const void* logits, int dtype, const int64_t* labels, 
     else if (sh.rows >= 1024 || n <= 1024)
       launch_forward_at<T, 256, 4>(logits, labels, stats, sh, op, s);
     else
-      launch_forward_at<T, 1024, 4>(logits, labels, stats, sh, op, s);
+      launch_forward_at<T, 512, 4>(logits, labels, stats, sh, op, s);
     return check_launch("forward_kernel");
   });
 }
