@@ -296,6 +296,7 @@ struct Operands {
 template <int PL>
 struct SymmetricStore {
   static constexpr bool kSymmetric = true;
+  static constexpr bool kSplit = false;
   half_t* c;
   const half_t* d;
   int n, pitch, cols;  // cols: n padded to a tile step
@@ -319,10 +320,75 @@ struct SymmetricStore {
   }
 };
 
+// One part of the sums of a symmetric product, along its rows: 64 x 64 tiles of
+// float32, one after the other, for sum_kernel to add.
+constexpr int kSplitTile = 64 * 64;
+constexpr int kSplitTiles = 512;  // most of them, all parts together
+struct SplitStore {
+  static constexpr bool kSymmetric = true;
+  static constexpr bool kSplit = true;
+  float* parts;
+  int nb, per;  // matrices; stages of a part
+  int tiles;    // of a matrix
+  struct Pre {};
+  __device__ __forceinline__ Pre fetch(int, int, int) const { return Pre{}; }
+  __device__ __forceinline__ void row8(int b, int i, int j, float (&v)[8], const Pre&) const {
+    const int ti = i >> 6, tj = j >> 6;
+    float* q = parts + ((int64_t)b * tiles + ti * (ti + 1) / 2 + tj) * kSplitTile +
+               (i & 63) * 64 + (j & 63);
+    *reinterpret_cast<f32x4*>(q) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(q + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+  __device__ __forceinline__ bool columns(bool) const { return false; }
+  __device__ __forceinline__ void col8(int, int, int, const float (&)[8]) const {}
+};
+
+// The parts of a symmetric product, added in their order and stored.
+template <int PL>
+__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ parts, int count,
+                                                  SymmetricStore<PL> store) {
+  __shared__ float tile[64][68];
+  const int tiles = gridDim.x, nb = gridDim.y, b = blockIdx.y;
+  int ti = 0;
+  while ((ti + 1) * (ti + 2) / 2 <= (int)blockIdx.x) ++ti;
+  const int tj = blockIdx.x - ti * (ti + 1) / 2;
+  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+  f32x4 sum[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sum[q] = nl2k::zero4();
+#pragma unroll 4
+  for (int s = 0; s < count; ++s) {
+    const float* p =
+        parts + (((int64_t)s * nb + b) * tiles + blockIdx.x) * kSplitTile + r * 64 + c;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] += nl2k::load4(p + 4 * q);
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const f32x4 lo = sum[2 * h], hi = sum[2 * h + 1];
+    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    const int i = ti * 64 + r, j = tj * 64 + c + 8 * h;
+    store.row8(b, i, j, v, store.fetch(b, i, j));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[r][c + 8 * h + e] = v[e];
+  }
+  __syncthreads();
+  if (!store.columns(ti == tj)) return;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int col = threadIdx.x >> 2, row = ((threadIdx.x & 3) * 2 + h) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[row + e][col];
+    store.col8(b, ti * 64 + row, tj * 64 + col, v);
+  }
+}
+
 // X = alpha acc + beta X, as [k, l] in place and as [l, k].
 template <int PL>
 struct StepStore {
   static constexpr bool kSymmetric = false;
+  static constexpr bool kSplit = false;
   half_t* x;
   half_t* xt;
   int k, l, x_pitch, t_pitch, x_cols, t_cols;
@@ -350,6 +416,7 @@ struct StepStore {
 template <int PL>
 struct LastStore {
   static constexpr bool kSymmetric = false;
+  static constexpr bool kSplit = false;
   void* out[kBatch];
   const half_t* x;
   int dtype, tall, update;
@@ -453,8 +520,16 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
     x = xcd * per + min(xcd, more) + (x >> 3);
   }
   const int one = Store::kSymmetric ? o.tiles_p * (o.tiles_p + 1) / 2 : o.tiles_p * o.tiles_q;
-  const int b = x / one;
+  const int b = x / one;  // matrix, or matrix of a part of the sums
   x -= b * one;
+  int matrix = b, steps = o.steps;
+  int64_t skip = 0;
+  if constexpr (Store::kSplit) {
+    const int part = b / store.nb, from = part * store.per;
+    matrix = b - part * store.nb;
+    steps = min(store.per, o.steps - from);
+    skip = (int64_t)from * 64;
+  }
   int ti, tj;
   if (Store::kSymmetric) {
     ti = (int)((sqrtf(8.f * x + 1.f) - 1.f) * 0.5f);
@@ -477,8 +552,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   auto permuted = [](int piece, int row) {
     return piece ^ ((kB == 16 ? row : row >> 1) & 7);
   };
-  const half_t* pbase = o.p + b * o.p_batch + (int64_t)i0 * o.p_pitch;
-  const half_t* qbase = o.q + b * o.q_batch + (int64_t)j0 * o.q_pitch;
+  const half_t* pbase = o.p + matrix * o.p_batch + skip + (int64_t)i0 * o.p_pitch;
+  const half_t* qbase = o.q + matrix * o.q_batch + skip + (int64_t)j0 * o.q_pitch;
   uint32_t off[kLoads];
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) {
@@ -561,7 +636,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   auto arrive = [&](int s) {
     __builtin_amdgcn_sched_barrier(0);
     wait_reads();
-    if (s + S - 1 <= o.steps)
+    if (s + S - 1 <= steps)
       wait_tile<(S - 2) * kLoads>();
     else
       wait_tile<0>();
@@ -570,13 +645,13 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   // The last reads, of a stage past the last, are of no use and do no harm.
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
-    if (s < o.steps) {
+    if (s < steps) {
       load_some(0, kLoads);
       load_next();
     }
   f16x8 p0[BM * kK], q0[BN * kK], p1[BM * kK], q1[BN * kK], q2[BN * kK];
   arrive(0);
-  bool more = S - 1 < o.steps;  // whether there is a stage to load during this step
+  bool more = S - 1 < steps;  // whether there is a stage to load during this step
   int stage = 0;
 #pragma unroll
   for (int m = 0; m < BM * kK; ++m) read(0, m % kK, wi + m / kK * kB, p0[m]);
@@ -592,7 +667,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   auto next_stage = [&](int s) {
     if (more) load_next();
     arrive(s + 1);
-    more = s + S < o.steps;
+    more = s + S < steps;
     stage = stage + 1 == S ? 0 : stage + 1;
     begin();
     __builtin_amdgcn_sched_barrier(0);
@@ -601,7 +676,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   begin();
   if constexpr (PL == 1) {
     if (S > 2 && more) load_some(0, part(1));
-    for (int s = 0; s < o.steps; ++s) {
+    for (int s = 0; s < steps; ++s) {
       wait_reads();
       run(p0, q0, true, stage, kHalves - 1, p1, q1, more, part(1), part(2));
       next_stage(s);
@@ -618,9 +693,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
       next_stage(s);
       run(p1, q, true, stage, 0, p0, nq, more, part(0), part(1));
     };
-    for (int s = 0; s < o.steps; s += 2) {
+    for (int s = 0; s < steps; s += 2) {
       step(s, q0, q2);
-      if (s + 1 < o.steps) step(s + 1, q2, q0);
+      if (s + 1 < steps) step(s + 1, q2, q0);
     }
   }
   wait_reads();
@@ -935,6 +1010,7 @@ struct Plan {
   int per;                    // matrices a launch
   int gram;                   // k padded to 16, 32 or 64 where it is that short, else 0
   int gram_blocks;
+  bool split;                 // whether X X' may be summed in parts
   size_t bytes;
 };
 
@@ -964,6 +1040,9 @@ int make_plan(int64_t m, int64_t n, int64_t count, int precision, Plan* p) {
       1, std::min<int64_t>({count, kBatch, (int64_t)(kMaxBatchBytes / std::max<size_t>(one, 1))}));
   p->partials = (size_t)p->per * kPartials * sizeof(double);
   p->bytes = p->partials + p->per * one;
+  const int64_t t = nl2k::ceil_div(p->k, (int64_t)64);
+  p->split = t * (t + 1) <= kSplitTiles && p->lp >= 8 * kStep;  // two parts of four stages
+  if (p->split) p->bytes += (size_t)kSplitTiles * kSplitTile * sizeof(float);
   p->gram = p->k > kGram ? 0 : p->k > 32 ? 64 : p->k > 16 ? 32 : 16;
   p->gram_blocks = (int)std::min<int64_t>(nl2k::ceil_div(std::max<int64_t>(p->l, 1), 64),
                                           kGramBlocks);
@@ -1050,26 +1129,30 @@ double tiles_of(int64_t p, int64_t q, int tile, bool symmetric, int nb) {
   return nb * (symmetric ? tp * (tp + 1) / 2 : tp * tq);
 }
 
-// The shape whose rounds over 256 CUs take least.
-int choose(const Shape (&shapes)[kShapes], const Operands& o, bool symmetric, int nb) {
+// Time of a stage in `rounds` of a shape over 256 CUs.
+double stage_time(const Shape& s, double tiles) {
+  const double rounds = tiles / (256 * s.per_cu), rest = rounds - std::floor(rounds);
+  return std::floor(rounds) * s.full + (rest > 0.0 ? s.alone + (s.full - s.alone) * rest : 0.0);
+}
+
+// The shape that takes least, and its time.
+int choose(const Shape (&shapes)[kShapes], const Operands& o, bool symmetric, int nb,
+           double* time) {
   int best = -1;
-  double least = 0.0;
   for (int c = 0; c < kShapes; ++c) {
     const Shape& s = shapes[c];
     if (s.tile == 0) continue;
-    const double rounds = tiles_of(o.p_rows, o.q_rows, s.tile, symmetric, nb) / (256 * s.per_cu);
-    const double rest = rounds - std::floor(rounds);
-    const double stage = std::floor(rounds) * s.full +
-                         (rest > 0.0 ? s.alone + (s.full - s.alone) * rest : 0.0);
-    const double time = s.fixed + stage * (o.row_bytes / 128);
-    if (best < 0 || time < least) best = c, least = time;
+    const double t = s.fixed + stage_time(s, tiles_of(o.p_rows, o.q_rows, s.tile, symmetric, nb)) *
+                                   (o.row_bytes / 128);
+    if (best < 0 || t < *time) best = c, *time = t;
   }
   return best;
 }
 
 template <int PL, class Store>
 int launch_product(const Operands& o, const Store& store, int nb, hipStream_t stream) {
-  switch (choose(PL == 1 ? kHalfShapes : kFullShapes, o, Store::kSymmetric, nb)) {
+  double time;
+  switch (choose(PL == 1 ? kHalfShapes : kFullShapes, o, Store::kSymmetric, nb, &time)) {
     case 0:
       if constexpr (PL == 1) return launch_tiles<256, 2, 4, 2, 16, PL>(o, store, nb, stream);
       break;
@@ -1077,6 +1160,41 @@ int launch_product(const Operands& o, const Store& store, int nb, hipStream_t st
     case 2: return launch_tiles<128, 2, 2, 2, 32, PL>(o, store, nb, stream);
   }
   return launch_tiles<64, 2, 2, 3, 16, PL>(o, store, nb, stream);
+}
+
+// A symmetric product of few tiles and long rows: cut along the rows into parts whose sums a
+// second launch adds, where that takes less.
+constexpr double kSplitTime = 6.0;  // the second launch
+
+int splits_of(const Shape (&shapes)[kShapes], const Operands& o, int nb) {
+  double least;
+  choose(shapes, o, true, nb, &least);
+  const Shape& s = shapes[kShapes - 1];
+  const int steps = o.row_bytes / 128;
+  const double tiles = tiles_of(o.p_rows, o.q_rows, 64, true, nb);
+  int best = 1;
+  for (int parts = 2; parts <= 16 && parts * tiles <= kSplitTiles && 4 * parts <= steps;
+       parts *= 2) {
+    const double t =
+        s.fixed + stage_time(s, tiles * parts) * nl2k::ceil_div(steps, parts) + kSplitTime;
+    if (t < least) best = parts, least = t;
+  }
+  return best;
+}
+
+template <int PL>
+int launch_gram(const Operands& o, const SymmetricStore<PL>& store, int nb, float* parts,
+                hipStream_t stream) {
+  const int splits = parts ? splits_of(PL == 1 ? kHalfShapes : kFullShapes, o, nb) : 1;
+  if (splits == 1) return launch_product<PL>(o, store, nb, stream);
+  const int t = (int)nl2k::ceil_div(o.p_rows, 64), tiles = t * (t + 1) / 2;
+  const int per = (int)nl2k::ceil_div(o.row_bytes / 128, splits);
+  const int count = (int)nl2k::ceil_div(o.row_bytes / 128, per);  // none of them empty
+  const int st = launch_tiles<64, 2, 2, 3, 16, PL>(o, SplitStore{parts, nb, per, tiles},
+                                                   nb * count, stream);
+  if (st) return st;
+  hipLaunchKernelGGL((sum_kernel<PL>), dim3(tiles, nb), dim3(256), 0, stream, parts, count, store);
+  return nl2k::check_launch("sum_kernel");
 }
 
 struct Job {
@@ -1098,6 +1216,7 @@ int run_batch(const Job& job, const Plan& p, const Scales& sc, int first, int nb
   half_t* xt2 = xt + (int64_t)p.per * p.xt;
   half_t* ga = xt2 + (int64_t)p.per * p.xt;
   half_t* gb = ga + (int64_t)p.per * p.a;
+  float* parts = reinterpret_cast<float*>(gb + (int64_t)p.per * p.a);
   const bool tall = job.src.m > job.src.n;
   const int blocks = (int)std::min<int64_t>(
       nl2k::ceil_div((int64_t)job.src.m * nl2k::ceil_div(job.src.n, 8), 256), kPartials);
@@ -1115,9 +1234,9 @@ int run_batch(const Job& job, const Plan& p, const Scales& sc, int first, int nb
   const int k = (int)p.k, l = (int)p.l;
   for (int i = 0; i < job.steps; ++i) {
     const Operands xx{x, x, k, k, p.lp, p.lp, p.x, p.x, p.lp * 2};
-    st = launch_product<PL>(
+    st = launch_gram<PL>(
         xx, SymmetricStore<PL>{ga, nullptr, k, p.kp, p.kcols, p.a, sc.a / (sc.x * sc.x), 0.f}, nb,
-        stream);
+        p.split ? parts : nullptr, stream);
     if (st) return st;
     const Operands aa{ga, ga, k, k, p.kp, p.kp, p.a, p.a, p.kp * 2};
     st = launch_product<PL>(
