@@ -55,11 +55,10 @@ def _given(labels, old_logp, advantages, ref_logp, mask):
     adv = advantages
     if adv.shape != shape:
         try:  # one a sequence: [B] or [B, 1]
-            adv = (adv.unsqueeze(-1) if adv.dim() == 1 and len(shape) == 2 and
-                   adv.size(0) == shape[0] else adv).expand(shape)
+            adv = (adv.unsqueeze(-1) if adv.dim() == 1 and len(shape) == 2 else adv).expand(shape)
         except RuntimeError:
-            raise RuntimeError(f"advantages must broadcast to the labels' shape {tuple(shape)}, "
-                               f"got {tuple(advantages.shape)}") from None
+            raise RuntimeError("advantages must be one a sequence or broadcast to the labels' "
+                               f"shape {tuple(shape)}, got {tuple(advantages.shape)}") from None
     if len(shape) == 2:
         adv_bs, adv_ss = adv.stride()
     elif len(shape) == 1:
@@ -89,45 +88,39 @@ def _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
     capi.require(denom is None or denom > 0, "denom must be positive")
 
 
-def loss_forward(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *, clip_low=0.2,
-                 clip_high=0.2, kl_coef=0.0, temperature=1.0, denom=None, ignore_index=-100,
-                 keep_stats=False):
-    """(loss, logp, stats, coef); stats and coef are for ``loss_backward``
-    (None unless ``keep_stats``)."""
-    _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
+def _forward(logits, labels, old_logp, advantages, ref_logp, mask, opts, keep):
+    """(loss, logp, logits and labels as they were read, rows, kept): kept
+    [3, tokens] holds the rows' statistics and coefficients for ``_backward``
+    (None unless ``keep``)."""
+    _check(logits, labels, old_logp, advantages, ref_logp, mask, opts["kl_coef"], opts["denom"])
     lib = _lib()
     x, B, S, V, bs, rs = token_rows.layout(logits)
-    keep, given = _given(labels, old_logp, advantages, ref_logp, mask)
+    held, given = _given(labels, old_logp, advantages, ref_logp, mask)
+    rows = (B, S, V, bs, rs, opts["ignore_index"], opts["temperature"])
+    n = labels.numel()
     ws_bytes = _workspace_bytes(B, S)
-    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=logits.device)
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
     loss, logp = ws.new_empty(()), ws.new_empty(labels.shape)
-    stats = coef = None
-    if keep_stats:
-        stats, coef = ws.new_empty(labels.shape + (2,)), ws.new_empty(labels.shape)
-    st = capi.launch(lib.policy_loss_forward, logits.get_device(), x.data_ptr(),
-                     token_rows.DTYPES[x.dtype], *given, loss.data_ptr(), logp.data_ptr(),
-                     stats.data_ptr() if keep_stats else 0, coef.data_ptr() if keep_stats else 0,
-                     B, S, V, bs, rs, ignore_index, temperature, clip_low, clip_high, kl_coef,
-                     0.0 if denom is None else denom, ws.data_ptr(), ws_bytes)
+    kept = ws.new_empty(3 * n) if keep else None
+    at = kept.data_ptr() if keep else 0
+    st = capi.launch(lib.policy_loss_forward, x.get_device(), x.data_ptr(),
+                     token_rows.DTYPES[x.dtype], *given, loss.data_ptr(), logp.data_ptr(), at,
+                     at + 8 * n if at else 0, *rows, opts["clip_low"], opts["clip_high"],
+                     opts["kl_coef"], opts["denom"] or 0.0, ws.data_ptr(), ws_bytes)
     if st:
         capi.check(st, lib.policy_loss_last_error, "policy_loss")
-    del keep
-    return loss, logp, stats, coef
+    return loss, logp, x, held[0], rows, kept
 
 
-def loss_backward(logits, labels, stats, coef, gout, temperature=1.0, ignore_index=-100):
+def _backward(x, labels, kept, gout, rows, shape):
     """dlogits of the loss, times the one-element tensor gout."""
-    token_rows.check(logits, labels, ("stats", stats), ("coef", coef), ("gout", gout))
-    capi.require(gout.dtype == torch.float32 and gout.numel() == 1,
-                 "gout must be a one-element float32 GPU tensor")
     lib = _lib()
-    x, B, S, V, bs, rs = token_rows.layout(logits)
-    labels = labels.contiguous()
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    st = capi.launch(lib.policy_loss_backward, logits.get_device(), x.data_ptr(),
-                     token_rows.DTYPES[x.dtype], labels.data_ptr(), stats.data_ptr(),
-                     coef.data_ptr(), gout.data_ptr(), dlogits.data_ptr(), B, S, V, bs, rs,
-                     ignore_index, temperature)
+    dlogits = torch.empty(shape, dtype=x.dtype, device=x.device)
+    at = kept.data_ptr()
+    st = capi.launch(lib.policy_loss_backward, x.get_device(), x.data_ptr(),
+                     token_rows.DTYPES[x.dtype], labels.data_ptr(), at,
+                     at + 8 * labels.numel() if at else 0, gout.data_ptr(), dlogits.data_ptr(),
+                     *rows)
     if st:
         capi.check(st, lib.policy_loss_last_error, "policy_loss backward")
     return dlogits
@@ -136,10 +129,10 @@ def loss_backward(logits, labels, stats, coef, gout, temperature=1.0, ignore_ind
 class PolicyLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, old_logp, advantages, ref_logp, mask, opts):
-        loss, logp, stats, coef = loss_forward(logits, labels, old_logp, advantages, ref_logp,
-                                               mask, keep_stats=True, **opts)
-        ctx.save_for_backward(logits, labels, stats, coef)
-        ctx.scalars = opts["temperature"], opts["ignore_index"]
+        loss, logp, x, labels, ctx.rows, kept = _forward(logits, labels, old_logp, advantages,
+                                                         ref_logp, mask, opts, True)
+        ctx.shape = logits.shape
+        ctx.save_for_backward(x, labels, kept)
         ctx.mark_non_differentiable(logp)
         ctx.set_materialize_grads(False)
         return loss, logp
@@ -148,8 +141,7 @@ class PolicyLossFunction(torch.autograd.Function):
     def backward(ctx, gout, _):
         if gout is None:
             return (None,) * 7
-        logits, labels, stats, coef = ctx.saved_tensors
-        return (loss_backward(logits, labels, stats, coef, gout, *ctx.scalars),) + (None,) * 6
+        return (_backward(*ctx.saved_tensors, gout, ctx.rows, ctx.shape),) + (None,) * 6
 
 
 def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *, clip_low=0.2,
@@ -167,7 +159,7 @@ def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, 
                 denom=denom, ignore_index=ignore_index)
     if logits.requires_grad and torch.is_grad_enabled():
         return PolicyLossFunction.apply(logits, labels, old_logp, advantages, ref_logp, mask, opts)
-    return loss_forward(logits, labels, old_logp, advantages, ref_logp, mask, **opts)[:2]
+    return _forward(logits, labels, old_logp, advantages, ref_logp, mask, opts, False)[:2]
 
 
 def policy_loss_and_grad(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *,

@@ -41,10 +41,11 @@ def _workspace_bytes(B, S, pairs):
     return _lib().preference_loss_workspace_bytes(B, S, pairs)
 
 
-def loss_forward(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=0.1,
-                 label_smoothing=0.0, average=False, ignore_index=-100, keep_stats=False):
-    """(loss, seq_logp, stats, coef); stats and coef are for ``loss_backward``
-    (None unless ``keep_stats``)."""
+def _forward(logits, labels, ref_seq_logp, opts, keep):
+    """(loss, seq_logp, logits and labels as they were read, rows, kept): kept
+    [3, tokens] holds the rows' statistics and coefficients for ``_backward``
+    (None unless ``keep``)."""
+    cu_seqlens = opts["cu_seqlens"]
     token_rows.check(logits, labels, ("ref_seq_logp", ref_seq_logp), ("cu_seqlens", cu_seqlens))
     lib = _lib()
     if cu_seqlens is None:
@@ -63,38 +64,35 @@ def loss_forward(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=0.1
                      "ref_seq_logp must be float32 [2 N]")
         ref_seq_logp = ref_seq_logp.contiguous()
     x, B, S, V, bs, rs = token_rows.layout(logits)
+    rows = (B, S, V, bs, rs, opts["ignore_index"])
     labels = labels.contiguous()
+    n = labels.numel()
     ws_bytes = _workspace_bytes(B, S, count // 2)
-    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=logits.device)
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
     loss, seq = ws.new_empty(()), ws.new_empty(count)
-    stats = coef = None
-    if keep_stats:
-        stats, coef = ws.new_empty(labels.shape + (2,)), ws.new_empty(labels.shape)
-    st = capi.launch(lib.preference_loss_forward, logits.get_device(), x.data_ptr(),
+    kept = ws.new_empty(3 * n) if keep else None
+    at = kept.data_ptr() if keep else 0
+    st = capi.launch(lib.preference_loss_forward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(),
                      0 if ref_seq_logp is None else ref_seq_logp.data_ptr(),
                      0 if cu_seqlens is None else cu_seqlens.data_ptr(), count // 2,
-                     loss.data_ptr(), seq.data_ptr(), stats.data_ptr() if keep_stats else 0,
-                     coef.data_ptr() if keep_stats else 0, B, S, V, bs, rs, ignore_index, beta,
-                     label_smoothing, 1 if average else 0, ws.data_ptr(), ws_bytes)
+                     loss.data_ptr(), seq.data_ptr(), at, at + 8 * n if at else 0, *rows,
+                     opts["beta"], opts["label_smoothing"], 1 if opts["average"] else 0,
+                     ws.data_ptr(), ws_bytes)
     if st:
         capi.check(st, lib.preference_loss_last_error, "preference_loss")
-    return loss, seq, stats, coef
+    return loss, seq, x, labels, rows, kept
 
 
-def loss_backward(logits, labels, stats, coef, gout=None, ignore_index=-100):
+def _backward(x, labels, kept, gout, rows, shape):
     """dlogits of the loss, times the one-element tensor gout where given."""
-    token_rows.check(logits, labels, ("stats", stats), ("coef", coef), ("gout", gout))
-    capi.require(gout is None or (gout.dtype == torch.float32 and gout.numel() == 1),
-                 "gout must be a one-element float32 GPU tensor")
     lib = _lib()
-    x, B, S, V, bs, rs = token_rows.layout(logits)
-    labels = labels.contiguous()
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    st = capi.launch(lib.preference_loss_backward, logits.get_device(), x.data_ptr(),
-                     token_rows.DTYPES[x.dtype], labels.data_ptr(), stats.data_ptr(),
-                     coef.data_ptr(), 0 if gout is None else gout.data_ptr(), dlogits.data_ptr(),
-                     B, S, V, bs, rs, ignore_index)
+    dlogits = torch.empty(shape, dtype=x.dtype, device=x.device)
+    at = kept.data_ptr()
+    st = capi.launch(lib.preference_loss_backward, x.get_device(), x.data_ptr(),
+                     token_rows.DTYPES[x.dtype], labels.data_ptr(), at,
+                     at + 8 * labels.numel() if at else 0, 0 if gout is None else gout.data_ptr(),
+                     dlogits.data_ptr(), *rows)
     if st:
         capi.check(st, lib.preference_loss_last_error, "preference_loss backward")
     return dlogits
@@ -103,10 +101,9 @@ def loss_backward(logits, labels, stats, coef, gout=None, ignore_index=-100):
 class PreferenceLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref_seq_logp, opts):
-        loss, seq, stats, coef = loss_forward(logits, labels, ref_seq_logp, keep_stats=True,
-                                              **opts)
-        ctx.save_for_backward(logits, labels, stats, coef)
-        ctx.ignore_index = opts["ignore_index"]
+        loss, seq, x, labels, ctx.rows, kept = _forward(logits, labels, ref_seq_logp, opts, True)
+        ctx.shape = logits.shape
+        ctx.save_for_backward(x, labels, kept)
         ctx.mark_non_differentiable(seq)
         ctx.set_materialize_grads(False)
         return loss, seq
@@ -115,8 +112,7 @@ class PreferenceLossFunction(torch.autograd.Function):
     def backward(ctx, gout, _):
         if gout is None:
             return None, None, None, None
-        logits, labels, stats, coef = ctx.saved_tensors
-        return loss_backward(logits, labels, stats, coef, gout, ctx.ignore_index), None, None, None
+        return _backward(*ctx.saved_tensors, gout, ctx.rows, ctx.shape), None, None, None
 
 
 def preference_loss(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=0.1,
@@ -134,18 +130,16 @@ def preference_loss(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=
                 average=average, ignore_index=ignore_index)
     if logits.requires_grad and torch.is_grad_enabled():
         return PreferenceLossFunction.apply(logits, labels, ref_seq_logp, opts)
-    return loss_forward(logits, labels, ref_seq_logp, **opts)[:2]
+    return _forward(logits, labels, ref_seq_logp, opts, False)[:2]
 
 
 def preference_loss_and_grad(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=0.1,
                              label_smoothing=0.0, average=False, ignore_index=-100):
     """(loss, seq_logp, dlogits) of ``preference_loss``, outside autograd."""
-    logits = logits.detach()
-    loss, seq, stats, coef = loss_forward(logits, labels, ref_seq_logp, cu_seqlens=cu_seqlens,
-                                          beta=beta, label_smoothing=label_smoothing,
-                                          average=average, ignore_index=ignore_index,
-                                          keep_stats=True)
-    return loss, seq, loss_backward(logits, labels, stats, coef, None, ignore_index)
+    opts = dict(cu_seqlens=cu_seqlens, beta=beta, label_smoothing=label_smoothing,
+                average=average, ignore_index=ignore_index)
+    loss, seq, x, labels, rows, kept = _forward(logits.detach(), labels, ref_seq_logp, opts, True)
+    return loss, seq, _backward(x, labels, kept, None, rows, logits.shape)
 
 
 def _options(params):

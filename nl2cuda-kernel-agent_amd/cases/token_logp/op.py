@@ -39,15 +39,18 @@ def logp_forward(logits, labels, temperature=1.0, ignore_index=-100, keep_stats=
     """(logp, stats): stats [..., 2] hold each row's maximum and sum of
     exponentials for ``logp_backward`` (None unless ``keep_stats``)."""
     token_rows.check(logits, labels)
-    lib = _lib()
     x, B, S, V, bs, rs = token_rows.layout(logits)
-    labels = labels.contiguous()
-    logp = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
+    return _forward(x, labels.contiguous(), (B, S, V, bs, rs, ignore_index, temperature),
+                    keep_stats)
+
+
+def _forward(x, labels, rows, keep_stats):
+    lib = _lib()
+    logp = torch.empty(labels.shape, dtype=torch.float32, device=x.device)
     stats = logp.new_empty(labels.shape + (2,)) if keep_stats else None
-    st = capi.launch(lib.token_logp_forward, logits.get_device(), x.data_ptr(),
+    st = capi.launch(lib.token_logp_forward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), logp.data_ptr(),
-                     stats.data_ptr() if keep_stats else 0, B, S, V, bs, rs, ignore_index,
-                     temperature)
+                     stats.data_ptr() if keep_stats else 0, *rows)
     if st:
         capi.check(st, lib.token_logp_last_error, "token_logp")
     return logp, stats
@@ -60,14 +63,18 @@ def logp_backward(logits, labels, stats, dlogp, temperature=1.0, ignore_index=-1
                  "dlogp must be float32 of the labels' shape")
     capi.require(stats.dtype == torch.float32 and stats.shape == labels.shape + (2,),
                  "stats must be the forward's")
-    lib = _lib()
     x, B, S, V, bs, rs = token_rows.layout(logits)
-    labels, dlogp, stats = labels.contiguous(), dlogp.contiguous(), stats.contiguous()
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    st = capi.launch(lib.token_logp_backward, logits.get_device(), x.data_ptr(),
+    return _backward(x, labels.contiguous(), stats.contiguous(), dlogp,
+                     (B, S, V, bs, rs, ignore_index, temperature), logits.shape)
+
+
+def _backward(x, labels, stats, dlogp, rows, shape):
+    lib = _lib()
+    dlogp = dlogp.contiguous()
+    dlogits = torch.empty(shape, dtype=x.dtype, device=x.device)
+    st = capi.launch(lib.token_logp_backward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), stats.data_ptr(),
-                     dlogp.data_ptr(), 0, dlogits.data_ptr(), B, S, V, bs, rs, ignore_index,
-                     temperature)
+                     dlogp.data_ptr(), 0, dlogits.data_ptr(), *rows)
     if st:
         capi.check(st, lib.token_logp_last_error, "token_logp backward")
     return dlogits
@@ -76,15 +83,17 @@ def logp_backward(logits, labels, stats, dlogp, temperature=1.0, ignore_index=-1
 class TokenLogpFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, temperature, ignore_index):
-        logp, stats = logp_forward(logits, labels, temperature, ignore_index, keep_stats=True)
-        ctx.save_for_backward(logits, labels, stats)
-        ctx.scalars = temperature, ignore_index
+        token_rows.check(logits, labels)
+        x, B, S, V, bs, rs = token_rows.layout(logits)
+        labels = labels.contiguous()
+        ctx.rows, ctx.shape = (B, S, V, bs, rs, ignore_index, temperature), logits.shape
+        logp, stats = _forward(x, labels, ctx.rows, True)
+        ctx.save_for_backward(x, labels, stats)
         return logp
 
     @staticmethod
     def backward(ctx, dlogp):
-        logits, labels, stats = ctx.saved_tensors
-        return logp_backward(logits, labels, stats, dlogp, *ctx.scalars), None, None, None
+        return _backward(*ctx.saved_tensors, dlogp, ctx.rows, ctx.shape), None, None, None
 
 
 def token_logp(logits, labels, temperature=1.0, ignore_index=-100):

@@ -554,7 +554,7 @@ inline int make_shape(int64_t B, int64_t S, int64_t V, int64_t bs, int64_t rs, i
   if (!(temperature >= 1e-30f) || !(temperature <= 1e30f))
     return fail(NL2K_ERR_VALUE, "temperature must be from 1e-30 to 1e30, got %g",
                 (double)temperature);
-  // rows are counted, and a row's columns addressed, in 32 bits; four times the rows is a grid
+  // rows are counted, and a row's columns addressed, in 32 bits
   if (V > (int64_t)1 << 28 || (S && B > ((int64_t)1 << 28) / S))
     return fail(NL2K_ERR_OVERFLOW, "at most 2^28 tokens and 2^28 columns, got B=%lld S=%lld V=%lld",
                 (long long)B, (long long)S, (long long)V);
@@ -571,12 +571,25 @@ inline int check_align(const void* p, int dtype, const char* what, uintptr_t a =
   return NL2K_SUCCESS;
 }
 
+// Workgroups of a launch over all rows.
+template <int TPR>
+inline int row_grid(const Shape& sh, int64_t segs, unsigned* grid) {
+  const int64_t n = TPR == 64 ? ceil_div(sh.rows, 4) : sh.rows * segs;
+  if (n > max_blocks(block_of<TPR>()))
+    return fail(NL2K_ERR_OVERFLOW, "%u rows of %d columns need more workgroups than a launch has",
+                sh.rows, sh.V);
+  *grid = (unsigned)n;
+  return NL2K_SUCCESS;
+}
+
 template <class T, int TPR, int U, class Op>
-inline void launch_forward_at(const void* logits, const int64_t* labels, f32x2* stats,
-                              const Shape& sh, const Op& op, hipStream_t s) {
-  const unsigned grid = TPR == 64 ? (sh.rows + 3) / 4 : sh.rows;
+inline int launch_forward_at(const void* logits, const int64_t* labels, f32x2* stats,
+                             const Shape& sh, const Op& op, hipStream_t s) {
+  unsigned grid;
+  if (const int st = row_grid<TPR>(sh, 1, &grid)) return st;
   hipLaunchKernelGGL((forward_kernel<T, TPR, U, Op>), dim3(grid), dim3(block_of<TPR>()), 0, s,
                      static_cast<const typename Elem<T>::type*>(logits), labels, stats, sh, op);
+  return check_launch("forward_kernel");
 }
 
 template <class Op>
@@ -585,24 +598,24 @@ inline int launch_forward(const void* logits, int dtype, const int64_t* labels, 
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
     const int n = (sh.V + Elem<T>::E - 1) / Elem<T>::E;
-    if (n <= 512)
-      launch_forward_at<T, 64, 4>(logits, labels, stats, sh, op, s);
-    else if (sh.rows >= 1024 || n <= 1024)
-      launch_forward_at<T, 256, 4>(logits, labels, stats, sh, op, s);
-    else
-      launch_forward_at<T, 512, 4>(logits, labels, stats, sh, op, s);
-    return check_launch("forward_kernel");
+    if (n <= 512) return launch_forward_at<T, 64, 4>(logits, labels, stats, sh, op, s);
+    // few long rows: more lanes for each
+    if (sh.rows >= 1024 || n <= 1024)
+      return launch_forward_at<T, 256, 4>(logits, labels, stats, sh, op, s);
+    return launch_forward_at<T, 512, 4>(logits, labels, stats, sh, op, s);
   });
 }
 
 template <class T, int TPR, int U>
-inline void launch_backward_at(const void* logits, const int64_t* labels, const f32x2* stats,
-                               const float* coef, const float* gout, void* dlogits,
-                               const Shape& sh, uint32_t segs, hipStream_t s) {
-  const unsigned grid = TPR == 64 ? (sh.rows + 3) / 4 : sh.rows * segs;
+inline int launch_backward_at(const void* logits, const int64_t* labels, const f32x2* stats,
+                              const float* coef, const float* gout, void* dlogits, const Shape& sh,
+                              int64_t segs, hipStream_t s) {
+  unsigned grid;
+  if (const int st = row_grid<TPR>(sh, segs, &grid)) return st;
   hipLaunchKernelGGL((backward_kernel<T, TPR, U>), dim3(grid), dim3(block_of<TPR>()), 0, s,
                      static_cast<const typename Elem<T>::type*>(logits), labels, stats, coef, gout,
-                     static_cast<typename Elem<T>::type*>(dlogits), sh, segs);
+                     static_cast<typename Elem<T>::type*>(dlogits), sh, (uint32_t)segs);
+  return check_launch("backward_kernel");
 }
 
 inline int launch_backward(const void* logits, int dtype, const int64_t* labels,
@@ -612,17 +625,10 @@ inline int launch_backward(const void* logits, int dtype, const int64_t* labels,
     using T = decltype(tag);
     const int n = (sh.V + Elem<T>::E - 1) / Elem<T>::E;
     constexpr int U = 4;
-    if (n <= 64 * U) {
-      launch_backward_at<T, 64, U>(logits, labels, stats, coef, gout, dlogits, sh, 1, s);
-    } else {
-      const int64_t segs = ceil_div(n, 256 * U);
-      if (segs * sh.rows > max_blocks(256))
-        return fail(NL2K_ERR_OVERFLOW, "%u rows of %d columns need more workgroups than a launch "
-                    "has", sh.rows, sh.V);
-      launch_backward_at<T, 256, U>(logits, labels, stats, coef, gout, dlogits, sh, (uint32_t)segs,
-                                    s);
-    }
-    return check_launch("backward_kernel");
+    if (n <= 64 * U)
+      return launch_backward_at<T, 64, U>(logits, labels, stats, coef, gout, dlogits, sh, 1, s);
+    return launch_backward_at<T, 256, U>(logits, labels, stats, coef, gout, dlogits, sh,
+                                         ceil_div(n, 256 * U), s);
   });
 }
 
@@ -645,39 +651,38 @@ inline int backward(const char* what, const void* logits, int dtype, const int64
 }
 
 template <class T, int TPR, int K, class Op>
-inline void launch_fused_at(const void* logits, const int64_t* labels, void* dlogits,
-                            const Shape& sh, const Op& op, hipStream_t s) {
-  const unsigned grid = TPR == 64 ? (sh.rows + 3) / 4 : sh.rows;
+inline int launch_fused_at(const void* logits, const int64_t* labels, void* dlogits,
+                           const Shape& sh, const Op& op, hipStream_t s) {
+  unsigned grid;
+  if (const int st = row_grid<TPR>(sh, 1, &grid)) return st;
   hipLaunchKernelGGL((fused_kernel<T, TPR, K, Op>), dim3(grid), dim3(block_of<TPR>()), 0, s,
                      static_cast<const typename Elem<T>::type*>(logits), labels,
                      static_cast<typename Elem<T>::type*>(dlogits), sh, op);
+  return check_launch("fused_kernel");
 }
 
+// The fewest lanes whose registers hold a row, 16 windows each at most.
 template <class Op>
 inline int launch_fused(const void* logits, int dtype, const int64_t* labels, void* dlogits,
                         const Shape& sh, const Op& op, hipStream_t s) {
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
     const int n = (sh.V + Elem<T>::E - 1) / Elem<T>::E;
-    if (sh.V < Elem<T>::E || n > 16384)
-      hipLaunchKernelGGL((fused_long_kernel<T, 1024, 4, Op>), dim3(sh.rows), dim3(1024), 0, s,
+    if (sh.V < Elem<T>::E || n > 16384) {
+      unsigned grid;
+      if (const int st = row_grid<1024>(sh, 1, &grid)) return st;
+      hipLaunchKernelGGL((fused_long_kernel<T, 1024, 4, Op>), dim3(grid), dim3(1024), 0, s,
                          static_cast<const typename Elem<T>::type*>(logits), labels,
                          static_cast<typename Elem<T>::type*>(dlogits), sh, op);
-    else if (n <= 128)
-      launch_fused_at<T, 64, 2>(logits, labels, dlogits, sh, op, s);
-    else if (n <= 512)
-      launch_fused_at<T, 64, 8>(logits, labels, dlogits, sh, op, s);
-    else if (n <= 1024)
-      launch_fused_at<T, 256, 4>(logits, labels, dlogits, sh, op, s);
-    else if (n <= 2048)
-      launch_fused_at<T, 256, 8>(logits, labels, dlogits, sh, op, s);
-    else if (n <= 4096)
-      launch_fused_at<T, 256, 16>(logits, labels, dlogits, sh, op, s);
-    else if (n <= 8192)
-      launch_fused_at<T, 512, 16>(logits, labels, dlogits, sh, op, s);
-    else
-      launch_fused_at<T, 1024, 16>(logits, labels, dlogits, sh, op, s);
-    return check_launch("fused_kernel");
+      return check_launch("fused_long_kernel");
+    }
+    if (n <= 128) return launch_fused_at<T, 64, 2>(logits, labels, dlogits, sh, op, s);
+    if (n <= 512) return launch_fused_at<T, 64, 8>(logits, labels, dlogits, sh, op, s);
+    if (n <= 1024) return launch_fused_at<T, 256, 4>(logits, labels, dlogits, sh, op, s);
+    if (n <= 2048) return launch_fused_at<T, 256, 8>(logits, labels, dlogits, sh, op, s);
+    if (n <= 4096) return launch_fused_at<T, 256, 16>(logits, labels, dlogits, sh, op, s);
+    if (n <= 8192) return launch_fused_at<T, 512, 16>(logits, labels, dlogits, sh, op, s);
+    return launch_fused_at<T, 1024, 16>(logits, labels, dlogits, sh, op, s);
   });
 }
 

@@ -110,7 +110,8 @@ def test_newton_schulz_validation():
     assert lib.newton_schulz_workspace_bytes(1 << 17, 1 << 17, 1, 1) == 0
     need = lib.newton_schulz_workspace_bytes(40, 50, 1, 1)
     assert need > 0
-    assert lib.newton_schulz_workspace_bytes(40, 50, 1, 2) > need
+    assert lib.newton_schulz_workspace_bytes(140, 150, 1, 2) > \
+        lib.newton_schulz_workspace_bytes(140, 150, 1, 1) > need
     one = (ctypes.c_void_p * 1)(1 << 20)
     odd = (ctypes.c_void_p * 1)((1 << 20) + 2)
     null = (ctypes.c_void_p * 1)(None)
