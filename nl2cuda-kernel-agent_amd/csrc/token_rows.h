@@ -221,9 +221,12 @@ __device__ __forceinline__ Stat scan_row(const typename Elem<T>::type* x, int32_
   const int n = (V + E - 1) / E;
   Stat st{-INFINITY, 0.f};
   for (int base = 0; base < n; base += TPR * U) {
+    // a wave of its own row passes over windows that no lane has
+    auto none = [&](int u) { return TPR == 64 && u && base + u * TPR >= n; };
     u32x4 w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (none(u)) break;
       const int i = min(base + lane + u * TPR, n - 1);
       w[u] = *reinterpret_cast<const u32x4_u*>(x + min(i * E, V - E));
     }
@@ -231,6 +234,7 @@ __device__ __forceinline__ Stat scan_row(const typename Elem<T>::type* x, int32_
     float cm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (none(u)) break;
       const int i = base + lane + u * TPR;
       unpack<T>(w[u], v[u]);
       if (base + (u + 1) * TPR >= n) {  // may hold the row's last window, or none
@@ -245,9 +249,11 @@ __device__ __forceinline__ Stat scan_row(const typename Elem<T>::type* x, int32_
     const float b = finite_max(nm);
     float cs = 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      if (none(u)) break;
 #pragma unroll
       for (int e = 0; e < E; ++e) cs += exp2_of((v[u][e] - b) * k);
+    }
     st.s = st.s * exp2_of((st.m - b) * k) + cs;
     st.m = nm;
   }
@@ -368,12 +374,12 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(
   const f32x2 st = stats[r];
   const int V = sh.V, n = (V + E - 1) / E;
   auto* d = dlogits + (int64_t)r * V;
-  const int first = (int)seg * TPR * U + lane;
+  const int base = (int)seg * TPR * U, first = base + lane;
   if (g == 0.f) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = first + u * TPR;
-      if (V >= E) store_window<T>(d, i, n, V, u32x4{0u, 0u, 0u, 0u});
+      if (V >= E && base + u * TPR < n) store_window<T>(d, i, n, V, u32x4{0u, 0u, 0u, 0u});
     }
     if (V < E && lane < V) d[lane] = 0;
     return;
@@ -394,10 +400,11 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = min(first + u * TPR, n - 1);
-    w[u] = *reinterpret_cast<const u32x4_u*>(x + min(i * E, V - E));
+    if (base + u * TPR < n) w[u] = *reinterpret_cast<const u32x4_u*>(x + min(i * E, V - E));
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
+    if (base + u * TPR >= n) break;
     const int i = first + u * TPR;
     const u32x4 y = gradient<T>(w[u], min(i * E, V - E), col, m, k, coef_t, scale);
     store_window<T>(d, i, n, V, y);
@@ -598,7 +605,12 @@ inline int launch_forward(const void* logits, int dtype, const int64_t* labels, 
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
     const int n = (sh.V + Elem<T>::E - 1) / Elem<T>::E;
-    if (n <= 512) return launch_forward_at<T, 64, 4>(logits, labels, stats, sh, op, s);
+    // a wave a row, no more windows at a time than there are: 65536 rows of 512 bfloat16 took
+    // 37 us with four in place of one, whose exponentials were for nothing, against 21
+    if (n <= 64) return launch_forward_at<T, 64, 1>(logits, labels, stats, sh, op, s);
+    if (n <= 128) return launch_forward_at<T, 64, 2>(logits, labels, stats, sh, op, s);
+    if (n <= 256) return launch_forward_at<T, 64, 4>(logits, labels, stats, sh, op, s);
+    if (n <= 512) return launch_forward_at<T, 64, 8>(logits, labels, stats, sh, op, s);
     // few long rows: more lanes for each
     if (sh.rows >= 1024 || n <= 1024)
       return launch_forward_at<T, 256, 4>(logits, labels, stats, sh, op, s);
@@ -624,11 +636,14 @@ inline int launch_backward(const void* logits, int dtype, const int64_t* labels,
   return with_type(dtype, [&](auto tag) {
     using T = decltype(tag);
     const int n = (sh.V + Elem<T>::E - 1) / Elem<T>::E;
-    constexpr int U = 4;
-    if (n <= 64 * U)
-      return launch_backward_at<T, 64, U>(logits, labels, stats, coef, gout, dlogits, sh, 1, s);
-    return launch_backward_at<T, 256, U>(logits, labels, stats, coef, gout, dlogits, sh,
-                                         ceil_div(n, 256 * U), s);
+    if (n <= 128)
+      return launch_backward_at<T, 64, 2>(logits, labels, stats, coef, gout, dlogits, sh, 1, s);
+    if (n <= 256)
+      return launch_backward_at<T, 64, 4>(logits, labels, stats, coef, gout, dlogits, sh, 1, s);
+    if (n <= 512)
+      return launch_backward_at<T, 64, 8>(logits, labels, stats, coef, gout, dlogits, sh, 1, s);
+    return launch_backward_at<T, 256, 4>(logits, labels, stats, coef, gout, dlogits, sh,
+                                         ceil_div(n, 256 * 4), s);
   });
 }
 
