@@ -68,7 +68,8 @@ def _row_stride(t):
 
 def newton_schulz(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, precision=None):
     """Each matrix of G [..., m, n] with its singular values taken to p(p(...)),
-    near 1, after division by its Frobenius norm + eps; of G's type.
+    near 1, after division by its Frobenius norm + eps; of G's type, and without
+    a gradient.
 
     precision: "half" holds the iterates in 11 bits, "full" in 22; None takes
     "full" for float32 and "half" for 16-bit matrices, whose own rounding is

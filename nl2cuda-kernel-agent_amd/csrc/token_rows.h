@@ -469,6 +469,9 @@ __global__ __launch_bounds__(block_of<TPR>()) void fused_kernel(
       for (int e = 0; e < E; ++e) t.s += exp2_of((v[e] - b) * k);
     }
   }
+  // d may be the logits: the label's has to be here, not on its way, before another wave of
+  // this row passes row_stat's barriers and overwrites it
+  asm volatile("" : : "v"(xl));
   const Stat st = row_stat<TPR>(t, k, red);
   const float g = op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau), lead) * sh.inv_tau;
   const float m = finite_max(st.m);
@@ -509,12 +512,13 @@ __global__ __launch_bounds__(block_of<TPR>()) void fused_long_kernel(
   const float k = kLog2e * sh.inv_tau;
   const float xl = load_one<T>(x + max(col, 0));
   const Stat t = V >= E ? scan_row<T, TPR, U>(x, V, k, lane) : scan_short<T, TPR>(x, V, k, lane);
+  // d may be the logits: the label's has to be here, not on its way, before another wave of
+  // this row passes row_stat's barriers and overwrites it
+  asm volatile("" : : "v"(xl));
   const Stat st = row_stat<TPR>(t, k, red);
   const float g = op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau), lead) * sh.inv_tau;
   const float m = finite_max(st.m);
   const float scale = g / st.s;
-  // every thread has its share of xl's row before any of it is overwritten (d may be the
-  // logits): row_stat's barriers, or the one wave's order, stand between
   if (V < E) {
     if (lane < V)
       d[lane] = round_one<T>((lane == col ? g : 0.f) -

@@ -262,6 +262,31 @@ def test_another_stream():
     assert torch.equal(got, want)
 
 
+def test_more_than_2_to_the_31_logits():
+    announce("policy_loss over 2^31 elements")
+    from cases.policy_loss.op import policy_loss, policy_loss_and_grad
+    rows, v = 65536 + 4, 32776
+    assert rows * v > 2 ** 31
+    logits = torch.zeros(rows, v, dtype=torch.bfloat16, device="cuda")
+    g, x, labels, old, ref, adv = _inputs(1, 4, v, torch.bfloat16)
+    logits[-4:] = x[0].cuda()
+    mask = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    mask[-4:] = True
+    full = [torch.zeros(rows, dtype=t.dtype, device="cuda") for t in (labels, old, adv)]
+    for f, t in zip(full, (labels, old, adv)):
+        f[-4:] = t[0].cuda()
+    opts = dict(mask=mask, clip_low=LOW, clip_high=HIGH)
+    loss, logp, d = policy_loss_and_grad(logits, *full, **opts)
+    assert not d[:-4].any()
+    _compare(x, labels, old, None, adv, None, 0.0, (loss, logp[-4:], d[-4:]))
+    del d
+    logits.requires_grad_(True)
+    loss, logp = policy_loss(logits, *full, **opts)
+    (d,) = torch.autograd.grad(loss, logits)
+    assert not d[:-4].any()
+    _compare(x, labels, old, None, adv, None, 0.0, (loss.detach(), logp[-4:], d[-4:]))
+
+
 def test_refusals():
     announce("policy_loss refusals")
     from cases.policy_loss.op import policy_loss, policy_loss_and_grad
