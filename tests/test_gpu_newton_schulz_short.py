@@ -93,3 +93,32 @@ def test_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("precision", ["half", "full"])
+def test_shapes_together(precision):
+    """Weights of many shapes in one call: products in launches of their own and shared ones,
+    short sides beside long ones, more shapes and matrices than a launch takes."""
+    from cases.newton_schulz.op import muon_step
+    announce(f"muon_step of many shapes {precision}")
+    shapes = ([(70, 130)] * 40 + [(130, 70)] * 3 + [(96, 96)] * 35 + [(200, 520)] * 2 +
+              [(20, 90)] * 33 + [(65, 66)] + [(300, 100)] * 2 + [(64, 64)])
+    g = torch.Generator().manual_seed(3)
+    W = [torch.randn(s, generator=g) * 0.02 for s in shapes]
+    G = [_matrix(*s) * (1 + 0.1 * i) + 0.1 * torch.randn(s, generator=g)
+         for i, s in enumerate(shapes)]
+    M = [0.3 * torch.randn(s, generator=g) for s in shapes]
+    Wd, Gd, Md = ([t.cuda() for t in x] for x in (W, G, M))
+    muon_step(Wd, Gd, Md, lr=0.05, momentum=0.9, precision=precision)
+    again = [w.cuda() for w in W]
+    muon_step(again, Gd, [m.cuda() for m in M], lr=0.05, momentum=0.9, precision=precision)
+    assert all(torch.equal(a, b) for a, b in zip(Wd, again))
+    size = {"half": 2.0 ** -11, "full": 2.0 ** -21}[precision]
+    for i in range(0, len(shapes), 3):
+        U = G[i].double() + 0.9 * (0.9 * M[i].double() + G[i].double())
+        s = max(1.0, shapes[i][0] / shapes[i][1]) ** 0.5
+        O = ons.orthogonalise(U)
+        off = ons.by_products(U, operand=size, product=2.0 ** -22, seed=1)
+        want = W[i].double() - 0.05 * s * O
+        bound = 0.05 * s * 4 * (off - O).norm() + 2.0 ** -22 * (want.norm() + O.norm())
+        assert (Wd[i].cpu().double() - want).norm() <= bound, shapes[i]
