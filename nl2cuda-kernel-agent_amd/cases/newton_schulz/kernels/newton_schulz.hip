@@ -450,18 +450,29 @@ struct LastStore {
   }
 };
 
+// An address that is the same in all lanes, in scalar registers, five issues after whatever
+// wrote them.
+__device__ __forceinline__ const half_t* scalar_base(const half_t* base) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
+  uint64_t q = hi << 32 | lo;
+  asm volatile("s_nop 4" : "+s"(q));
+  return reinterpret_cast<const half_t*>(q);
+}
+
 // 16 bytes a lane from global memory straight to LDS: lane n's land at lds + 16 n.
 // The count of outstanding loads is waited for by hand (wait_tile): the
 // compiler, which does not know which part of LDS a load writes, would have
-// every read of LDS wait for all of them.
+// every read of LDS wait for all of them.  M0 holds the place in LDS.  A scalar
+// register that a vector instruction wrote must not be read by a load within five
+// issues, which the compiler does not see to here: `base` comes from
+// scalar_base and is moved on by scalar additions alone.
 __device__ __forceinline__ void load_lds16(const half_t* base, uint32_t off, uint32_t lds) {
-  const uint64_t p = reinterpret_cast<uint64_t>(base);  // the same in all lanes
-  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
-  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
-               : "s"(lds), "v"(off), "s"(hi << 32 | lo)
-               : "memory");
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
 }
 
 // Waits until at most N of this wave's loads are outstanding.
@@ -556,8 +567,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
   auto permuted = [](int piece, int row) {
     return piece ^ ((kB == 16 ? row : row >> 1) & 7);
   };
-  const half_t* pbase = o.p + matrix * o.p_batch + skip + (int64_t)i0 * o.p_pitch;
-  const half_t* qbase = o.q + matrix * o.q_batch + skip + (int64_t)j0 * o.q_pitch;
+  const half_t* pbase = scalar_base(o.p + matrix * o.p_batch + skip + (int64_t)i0 * o.p_pitch);
+  const half_t* qbase = scalar_base(o.q + matrix * o.q_batch + skip + (int64_t)j0 * o.q_pitch);
   uint32_t off[kLoads];
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) {
@@ -742,7 +753,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Operands o, Store
     for (int u = 0; u < kUnits; ++u) {
       const int at_u = u * 64 + lane, r = at_u / (kCols / 8), c = at_u % (kCols / 8) * 8;
       float* q = pass + r * kPitch + c;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(q);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(q + 4);
       float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       store.row8(b, i + r, j + c, v, pre[m][u]);
       if (columns) {
@@ -1065,8 +1077,9 @@ struct Scales {
 
 int make_scales(int steps, float a, float b, float c, Scales* s) {
   if (!(std::fabs(a) < 1e3f && std::fabs(b) < 1e3f && std::fabs(c) < 1e3f))
-    return nl2k::fail(NL2K_ERR_VALUE, "coefficients must be finite and below 1000, got (%g, %g, %g)",
-                      (double)a, (double)b, (double)c);
+    return nl2k::fail(NL2K_ERR_VALUE,
+                      "coefficients must be finite and below 1000, got (%g, %g, %g)", (double)a,
+                      (double)b, (double)c);
   double top = 1.0, top_x = 1.0, top_b = 0.0;
   for (int i = 0; i < steps; ++i) {
     double next = 0.0;
@@ -1253,8 +1266,8 @@ int run_batch(const Job& job, const Plan& p, const Scales& sc, int first, int nb
           bx, StepStore<PL>{x, xt2, k, l, p.lp, p.kp, p.lcols, p.kcols, p.x, p.xt, 1.f / sc.b,
                             job.a}, nb, stream);
     } else {
-      LastStore<PL> last{{}, x, job.out_dtype, tall, job.update, job.out_stride, k, l, p.lp, p.lcols, p.x,
-                         1.f / (sc.b * sc.x), job.a / sc.x, job.keep, job.rate};
+      LastStore<PL> last{{}, x, job.out_dtype, tall, job.update, job.out_stride, k, l, p.lp,
+                         p.lcols, p.x, 1.f / (sc.b * sc.x), job.a / sc.x, job.keep, job.rate};
       for (int q = 0; q < nb; ++q) last.out[q] = job.out[first + q];
       st = launch_product<PL>(bx, last, nb, stream);
     }
@@ -1341,7 +1354,6 @@ int run_all(const char* what, Job& job, const void* const* grads, void* const* m
                           : run_gram<64>(job, p, (int)first, nb, workspace, stream);
     else
       st = precision == 1 ? run_batch<1>(job, p, sc, (int)first, nb, workspace, stream)
-                        
                           : run_batch<2>(job, p, sc, (int)first, nb, workspace, stream);
     if (st) return st;
   }
