@@ -1,6 +1,6 @@
 """CPU oracle of the Newton-Schulz updates -- TEST INFRASTRUCTURE ONLY.
 
-Float64 torch on the CPU.  ``orthogonalise`` follows the definition on singular
+Float64 torch, on the CPU unless given a GPU's matrix.  ``orthogonalise`` follows the definition on singular
 values (an SVD, no products); ``by_products`` the iteration, optionally with
 every operand and product off by random roundings of given sizes, which says
 how far roundings of that size move the result.
@@ -29,12 +29,13 @@ def by_products(G, coefficients=COEFFICIENTS, steps=5, eps=1e-7, operand=0.0, pr
                 seed=0):
     """The iteration; operands off by a relative `operand`, products by `product`
     of the sum of their terms' sizes, uniformly at random."""
-    gen = torch.Generator().manual_seed(seed)
+    gen = torch.Generator(device=G.device).manual_seed(seed)
 
     def off(x, size, by):
         if size == 0.0:
             return x
-        return x + size * by * (2 * torch.rand(x.shape, generator=gen, dtype=torch.float64) - 1)
+        return x + size * by * (2 * torch.rand(x.shape, generator=gen, dtype=torch.float64,
+                                               device=G.device) - 1)
 
     def mm(p, q):
         return off(p @ q, product, p.abs() @ q.abs())
