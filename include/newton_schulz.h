@@ -21,10 +21,12 @@
  *
  * precision 1 (half): X, A and b A + c A A are held in float16, 11 bits each.
  * precision 2 (full): in two float16, 22 bits, three products in place of one.
- * Products are summed in 32 bits, the norm in 64.  The operands are scaled by
- * powers of two so that their largest possible values fill float16's range;
- * coefficients under which some singular value in [0, 1] leaves [-4, 4] are
- * refused.  A matrix of zeros gives zeros; one with a NaN or an infinity
+ * Products are summed in 32 bits, the norm in 64.  Where the
+ * shorter side is at most 64 and |a|^(2 steps) <= 1e9, all of it is computed in
+ * 64 bits and rounded once, at either precision.  The other operands are
+ * scaled by powers of two so that their largest possible values fill float16's
+ * range; coefficients under which some singular value in [0, 1] leaves [-4, 4]
+ * are refused.  A matrix of zeros gives zeros; one with a NaN or an infinity
  * gives NaN.
  *
  * Device arrays owned by the caller; the library allocates nothing, keeps no

@@ -73,7 +73,8 @@ def newton_schulz(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, precision=Non
 
     precision: "half" holds the iterates in 11 bits, "full" in 22; None takes
     "full" for float32 and "half" for 16-bit matrices, whose own rounding is
-    coarser.
+    coarser.  A matrix whose shorter side is at most 64 is iterated in 64 bits at
+    either (unless |a|^(2 steps) > 1e9).
     """
     capi.require(G.is_cuda, "G must be a GPU tensor")
     capi.require(G.dtype in _DTYPES, "G must be float32, bfloat16 or float16")

@@ -349,9 +349,9 @@ __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(
   if (lead && stats) stats[r] = f32x2{st.m, st.s};
 }
 
-// Backward: a pure stream (244 us for 3448 rows of 50257 float32, 5.7 TB/s), TPR threads and U windows each a workgroup's share
-// of a row.  coef [rows] is the gradient of logp; gout, where given, one
-// number that scales it.
+// Backward: a pure stream (244 us for 3448 rows of 50257 float32, 5.7 TB/s), TPR
+// threads and U windows each a workgroup's share of a row.  coef [rows] is the
+// gradient of logp; gout, where given, one number that scales it.
 template <class T, int TPR, int U>
 __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(
     const typename Elem<T>::type* __restrict__ logits, const int64_t* __restrict__ labels,
