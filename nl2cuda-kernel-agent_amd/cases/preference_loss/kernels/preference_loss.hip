@@ -3,8 +3,8 @@
 //
 // The gradient of a row needs its pair's sums over all tokens, so the logits
 // are read twice: the rows' log-probabilities, a workgroup a pair that sums
-// them and writes the tokens' coefficients, the sum of the pairs' losses, and
-// the stream that makes dlogits.
+// them and writes the tokens' coefficients, the last of which adds up the
+// pairs' losses, and the stream that makes dlogits.
 
 #include "preference_loss.h"
 #include "token_rows.h"
@@ -16,6 +16,8 @@ using nl2k::rows::Shape;
 struct SequenceOp {
   float* __restrict__ logp;
   float* __restrict__ coef;  // zeros until the pairs are known: rows in no sequence keep them
+  uint32_t* __restrict__ done;  // 0 for pair_kernel
+  __device__ void begin(const Shape&) const {}
   __device__ bool counts(const Shape& sh, uint32_t, int64_t lab) const { return lab != sh.ignore; }
   __device__ void skip(uint32_t r, bool lead) const { put(r, 0.f, lead); }
   __device__ float finish(const Shape&, uint32_t r, float lp, bool lead) const {
@@ -26,6 +28,7 @@ struct SequenceOp {
     if (!lead) return;
     logp[r] = lp;
     if (coef) coef[r] = 0.f;
+    if (r == 0) *done = 0;
   }
 };
 
@@ -54,12 +57,17 @@ __device__ __forceinline__ void bounds(const int64_t* __restrict__ cu, int64_t i
   }
 }
 
+__global__ void no_rows_kernel(uint32_t* done) { *done = 0; }
+
+// `loss` counts the workgroups that are done, from 0, until the last of them has their losses' mean
+// to put there.  That takes their sum in a fixed order; a launch of its own for it took 4.6 us.
 __global__ __launch_bounds__(kPairBlock) void pair_kernel(
     const float* __restrict__ logp, const int64_t* __restrict__ labels,
     const float* __restrict__ ref, const int64_t* __restrict__ cu, Shape sh, uint32_t pairs,
     float beta, float eps, int average, float* __restrict__ seq_logp, float* __restrict__ coef,
-    float* __restrict__ pair_loss) {
+    float* __restrict__ pair_loss, uint32_t* __restrict__ loss) {
   __shared__ double red[kPairBlock / 64];
+  __shared__ bool last;
   double h[2];
   float share[2];
   uint32_t lo[2], hi[2];
@@ -99,15 +107,17 @@ __global__ __launch_bounds__(kPairBlock) void pair_kernel(
       for (uint32_t r = lo[j] + threadIdx.x; r < hi[j]; r += kPairBlock)
         coef[r] = (j ? -g : g) * share[j];
   }
-}
-
-__global__ __launch_bounds__(256) void mean_kernel(const float* __restrict__ x, uint32_t n,
-                                                   float* __restrict__ out) {
-  __shared__ double red[4];
+  // the thread that wrote the pair's loss releases it with its count, and has acquired those of
+  // all others with the last
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(loss, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+           pairs - 1;
+  __syncthreads();
+  if (!last) return;
   double s = 0.0;
-  for (uint32_t i = threadIdx.x; i < n; i += 256) s += x[i];
+  for (uint32_t i = threadIdx.x; i < pairs; i += kPairBlock) s += pair_loss[i];
   s = block_sum(s, red);
-  if (threadIdx.x == 0) out[0] = (float)(s / (double)n);
+  if (threadIdx.x == 0) *loss = __float_as_uint((float)(s / (double)pairs));
 }
 
 size_t even(size_t n) { return (n + 1) / 2 * 2; }
@@ -157,17 +167,18 @@ extern "C" int preference_loss_forward(const void* logits, int dtype, const int6
   if ((st = nl2k::rows::check_align(stats, 0, "stats", 8))) return st;
   float* logp = static_cast<float*>(workspace);
   float* pair_loss = logp + even(sh.rows);
+  uint32_t* counter = reinterpret_cast<uint32_t*>(loss);
   if (sh.rows) {
     st = nl2k::rows::launch_forward(logits, dtype, labels, reinterpret_cast<nl2k::f32x2*>(stats),
-                                    sh, SequenceOp{logp, coef}, stream);
+                                    sh, SequenceOp{logp, coef, counter}, stream);
     if (st) return st;
+  } else {
+    hipLaunchKernelGGL(no_rows_kernel, dim3(1), dim3(1), 0, stream, counter);
   }
   hipLaunchKernelGGL(pair_kernel, dim3((unsigned)pairs), dim3(kPairBlock), 0, stream, logp, labels,
                      ref_seq, cu_seqlens, sh, (uint32_t)pairs, beta, label_smoothing, average,
-                     seq_logp, coef, pair_loss);
-  if ((st = nl2k::check_launch("pair_kernel"))) return st;
-  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(256), 0, stream, pair_loss, (uint32_t)pairs, loss);
-  return nl2k::check_launch("mean_kernel");
+                     seq_logp, coef, pair_loss, counter);
+  return nl2k::check_launch("pair_kernel");
 }
 
 extern "C" int preference_loss_backward(const void* logits, int dtype, const int64_t* labels,

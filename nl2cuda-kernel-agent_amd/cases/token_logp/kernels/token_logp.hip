@@ -11,6 +11,7 @@ using nl2k::rows::Shape;
 // The log-probability itself.
 struct LogpOp {
   float* logp;
+  __device__ void begin(const Shape&) const {}
   __device__ bool counts(const Shape& sh, uint32_t, int64_t lab) const { return lab != sh.ignore; }
   __device__ void skip(uint32_t r, bool lead) const {
     if (lead) logp[r] = 0.f;

@@ -332,12 +332,13 @@ __device__ __forceinline__ void zero_row(typename Elem<T>::type* __restrict__ d,
                                          int lane) {
   constexpr int E = Elem<T>::E;
   const int n = V / E;
-  for (int i = lane; i < n; i += TPR) 
+  for (int i = lane; i < n; i += TPR)
     store16<kPast>(d + i * E, u32x4{0u, 0u, 0u, 0u});
   if (lane < V - n * E) d[n * E + lane] = 0;
 }
 
 // What a row's statistics are turned into.  Ops of the kernels below have
+//   void begin()               what all rows need, read beside the row's label
 //   bool counts(r, label)     whether the row counts (read before the row is)
 //   float finish(r, col, logp, lead)   called by every thread with the row's
 //                             logp; the coefficient of its gradient.  The
@@ -355,6 +356,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(
   const int lane = my_lane<TPR>();
   if (r >= sh.rows) return;
   const int64_t lab = labels[r];
+  op.begin(sh);
   const bool lead = lane == 0;
   if (!op.counts(sh, r, lab)) {
     op.skip(r, lead);
@@ -406,7 +408,8 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = first + u * TPR;
-      if (V >= E && base + u * TPR < n) store_window<T, kPast != kNone>(d, i, n, V, u32x4{0u, 0u, 0u, 0u});
+      if (V >= E && base + u * TPR < n)
+        store_window<T, kPast != kNone>(d, i, n, V, u32x4{0u, 0u, 0u, 0u});
     }
     if (V < E && lane < V) d[lane] = 0;
     return;
@@ -451,6 +454,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void fused_kernel(
   const int lane = my_lane<TPR>();
   if (r >= sh.rows) return;
   const int64_t lab = labels[r];
+  op.begin(sh);
   const bool lead = lane == 0;
   const int V = sh.V, n = (V + E - 1) / E;
   if (!op.counts(sh, r, lab)) {
@@ -525,6 +529,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void fused_long_kernel(
   const int lane = my_lane<TPR>();
   if (r >= sh.rows) return;
   const int64_t lab = labels[r];
+  op.begin(sh);
   const bool lead = lane == 0;
   const int V = sh.V, n = (V + E - 1) / E;
   auto* d = dlogits + (int64_t)r * V;
@@ -763,8 +768,9 @@ inline int launch_fused(const void* logits, int dtype, const int64_t* labels, vo
     if (sh.V < Elem<T>::E || n > 16384) {
       unsigned grid;
       if (const int st = row_grid<1024>(sh, 1, &grid)) return st;
-      auto* kernel = bytes_of<T>(sh) > Caches::kGradient ? &fused_long_kernel<T, 1024, 4, true, Op>
-                                                         : &fused_long_kernel<T, 1024, 4, false, Op>;
+      const bool past = bytes_of<T>(sh) > Caches::kGradient;
+      auto* kernel = past ? &fused_long_kernel<T, 1024, 4, true, Op>
+                          : &fused_long_kernel<T, 1024, 4, false, Op>;
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(1024), 0, s,
                          static_cast<const typename Elem<T>::type*>(logits), labels,
                          static_cast<typename Elem<T>::type*>(dlogits), sh, op);
