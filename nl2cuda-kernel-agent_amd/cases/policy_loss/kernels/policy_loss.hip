@@ -144,11 +144,11 @@ struct PolicyOp {
     logp[r] = 0.f;
     if (coef) coef[r] = 0.f;
   }
-  __device__ float finish(const Shape& sh, uint32_t r, float lp, bool lead) const {
+  __device__ float finish(const Shape& sh, uint32_t r, double lp, bool lead) const {
     const uint32_t b = sh.S == sh.rows ? 0u : r / sh.S;
     const float a = adv[(int64_t)b * adv_bs + (int64_t)(r - b * sh.S) * adv_ss];
     const float weight = w.kind == 2 ? static_cast<const float*>(w.mask)[r] : 1.f;
-    const float ratio = expf(lp - old_logp[r]);
+    const float ratio = expf((float)(lp - (double)old_logp[r]));
     // selects that let a NaN through, as the products do
     const float cut = ratio < lo ? lo : ratio > hi ? hi : ratio;
     const float free_term = ratio * a, cut_term = cut * a;
@@ -156,14 +156,14 @@ struct PolicyOp {
     float term = held ? -cut_term : -free_term;
     float g = held ? 0.f : -free_term;
     if (ref) {
-      const float d = ref[r] - lp;
+      const float d = (float)((double)ref[r] - lp);
       const float e = expm1f(d);
       term += kl_coef * (e - d);
       g -= kl_coef * e;
     }
     if (lead) {
       terms[r] = weight * term;
-      logp[r] = lp;
+      logp[r] = (float)lp;
     }
     g *= weight * inv;
     if (lead && coef) coef[r] = g;

@@ -20,8 +20,8 @@ struct SequenceOp {
   __device__ void begin(const Shape&) const {}
   __device__ bool counts(const Shape& sh, uint32_t, int64_t lab) const { return lab != sh.ignore; }
   __device__ void skip(uint32_t r, bool lead) const { put(r, 0.f, lead); }
-  __device__ float finish(const Shape&, uint32_t r, float lp, bool lead) const {
-    put(r, lp, lead);
+  __device__ float finish(const Shape&, uint32_t r, double lp, bool lead) const {
+    put(r, (float)lp, lead);
     return 0.f;
   }
   __device__ void put(uint32_t r, float lp, bool lead) const {

@@ -16,8 +16,8 @@ struct LogpOp {
   __device__ void skip(uint32_t r, bool lead) const {
     if (lead) logp[r] = 0.f;
   }
-  __device__ float finish(const Shape&, uint32_t r, float lp, bool lead) const {
-    if (lead) logp[r] = lp;
+  __device__ float finish(const Shape&, uint32_t r, double lp, bool lead) const {
+    if (lead) logp[r] = (float)lp;
     return 0.f;
   }
 };

@@ -28,7 +28,7 @@ namespace rows {
 enum { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr double kLn2 = 0.6931471805599453;
 
 struct bf16_t {};
 struct f16_t {};
@@ -131,6 +131,7 @@ struct Shape {
   int64_t bs, rs;
   int64_t ignore;   // label of rows that count for nothing
   float inv_tau;
+  double inv_tau64;
   // how a launch goes about it, see `Caches`
   bool once = false;        // rows are read past the caches
   bool last_first = false;  // rows in falling order
@@ -189,10 +190,14 @@ __device__ __forceinline__ Stat row_stat(Stat t, float k, float* red) {
   }
 }
 
-// (x[label] - m) / tau - log S, NaN for a label outside the row.
-__device__ __forceinline__ float logp_of(Stat st, float xl, int col, float inv_tau) {
-  const float v = (xl - finite_max(st.m)) * inv_tau - __builtin_amdgcn_logf(st.s) * kLn2;
-  return col >= 0 ? v : NAN;
+// (x[label] - m) / tau - log S, NaN for a label outside the row.  In 64 bits, the logarithm's
+// whole part apart: around 10, where logp is a row of 50257's, 32 bits round to 5e-7, which the
+// losses' differences of two log-probabilities would keep.
+__device__ __forceinline__ double logp_of(Stat st, float xl, int col, double inv_tau) {
+  const double log2_s = (double)__builtin_amdgcn_frexp_expf(st.s) +
+                        (double)__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(st.s));
+  const double v = ((double)xl - (double)finite_max(st.m)) * inv_tau - log2_s * kLn2;
+  return col >= 0 ? v : (double)NAN;
 }
 
 // Threads of a workgroup that share a row, TPR = 64, 256, 512 or 1024; a wave a
@@ -371,7 +376,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(
                  : sh.once         ? scan_row<T, TPR, U, true>(x, sh.V, k, lane)
                                    : scan_row<T, TPR, U>(x, sh.V, k, lane);
   const Stat st = row_stat<TPR>(t, k, red);
-  op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau), lead);
+  op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau64), lead);
   if (lead && stats) stats[r] = f32x2{st.m, st.s};
 }
 
@@ -503,7 +508,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void fused_kernel(
   // this row passes row_stat's barriers and overwrites it
   asm volatile("" : : "v"(xl));
   const Stat st = row_stat<TPR>(t, k, red);
-  const float g = op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau), lead) * sh.inv_tau;
+  const float g = op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau64), lead) * sh.inv_tau;
   const float m = finite_max(st.m);
   const float scale = g / st.s;
   auto* d = dlogits + (int64_t)r * V;
@@ -547,7 +552,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void fused_long_kernel(
   // this row passes row_stat's barriers and overwrites it
   asm volatile("" : : "v"(xl));
   const Stat st = row_stat<TPR>(t, k, red);
-  const float g = op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau), lead) * sh.inv_tau;
+  const float g = op.finish(sh, r, logp_of(st, xl, col, sh.inv_tau64), lead) * sh.inv_tau;
   const float m = finite_max(st.m);
   const float scale = g / st.s;
   if (V < E) {
@@ -603,7 +608,7 @@ inline int make_shape(int64_t B, int64_t S, int64_t V, int64_t bs, int64_t rs, i
     return fail(NL2K_ERR_OVERFLOW, "at most 2^28 tokens and 2^28 columns, got B=%lld S=%lld V=%lld",
                 (long long)B, (long long)S, (long long)V);
   *sh = Shape{(uint32_t)(B * S), (uint32_t)(B == 1 ? B * S : S), (int32_t)V, bs, rs, ignore,
-              1.f / temperature};
+              1.f / temperature, 1.0 / (double)temperature};
   if (B == 1) sh->bs = 0;
   return NL2K_SUCCESS;
 }
