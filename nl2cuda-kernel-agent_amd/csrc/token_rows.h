@@ -351,7 +351,7 @@ __device__ __forceinline__ void zero_row(typename Elem<T>::type* __restrict__ d,
 //   void skip(r, lead)        for rows that do not count
 
 // Forward: the statistics (m, S) of every row, for a backward, and the op's answers.  Bound by
-// memory: 52 us for 2432 rows of 50257 bfloat16, 154 for 3432 of float32 (4.7 and 4.5 TB/s).
+// memory: 50 us for 2432 rows of 50257 bfloat16, 109 for 3431 of float32 (4.9 and 6.3 TB/s).
 template <class T, int TPR, int U, class Op>
 __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(
     const typename Elem<T>::type* __restrict__ logits, const int64_t* __restrict__ labels,
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(
 // What of a gradient's kernel goes past the caches: nothing, its stores, its loads too.
 enum Past { kNone, kStores, kBoth };
 
-// Backward: a pure stream (244 us for 3448 rows of 50257 float32, 5.7 TB/s), TPR
+// Backward: a pure stream (238 us for 3447 rows of 50257 float32, 5.8 TB/s), TPR
 // threads and U windows each a workgroup's share of a row.  coef [rows] is the
 // gradient of logp; gout, where given, one number that scales it.
 template <class T, int TPR, int U, Past kPast>
@@ -448,7 +448,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(
 
 // Loss terms and gradient in one pass: the row stays in registers, K windows a
 // thread, between its statistics and its gradient.  4096 rows of 128256 bfloat16:
-// 435 us, 4.8 TB/s; apart, the two passes read the logits twice.
+// 415 us, 5.1 TB/s; apart, the two passes read the logits twice.
 template <class T, int TPR, int K, Past kPast, class Op>
 __global__ __launch_bounds__(block_of<TPR>()) void fused_kernel(
     const typename Elem<T>::type* logits, const int64_t* __restrict__ labels,
