@@ -48,9 +48,9 @@ def _workspace_bytes(m, n, count, precision):
     return _lib().newton_schulz_workspace_bytes(m, n, count, precision)
 
 
-def _precision(precision, dtype):
+def _precision(precision):
     if precision is None:
-        return 2 if dtype == torch.float32 else 1
+        return PRECISIONS["full"]
     capi.require(precision in PRECISIONS, "precision must be None, 'half' or 'full'")
     return PRECISIONS[precision]
 
@@ -71,16 +71,17 @@ def newton_schulz(G, steps=5, coefficients=COEFFICIENTS, eps=1e-7, precision=Non
     near 1, after division by its Frobenius norm + eps; of G's type, and without
     a gradient.
 
-    precision: "half" holds the iterates in 11 bits, "full" in 22; None takes
-    "full" for float32 and "half" for 16-bit matrices, whose own rounding is
-    coarser.  A matrix whose shorter side is at most 64 is iterated in 64 bits at
-    either (unless |a|^(2 steps) > 1e9).
+    precision: "full" (or None) holds the iterates in 22 bits whatever G's type,
+    whose own rounding then comes once, at the end; "half" holds them in 11, in
+    less than half the time where the products fill the chip.  A matrix whose
+    shorter side is at most 64 is iterated in 64 bits at either (unless
+    |a|^(2 steps) > 1e9).
     """
     capi.require(G.is_cuda, "G must be a GPU tensor")
     capi.require(G.dtype in _DTYPES, "G must be float32, bfloat16 or float16")
     capi.require(G.dim() >= 2, "G must be [..., m, n]")
     lib = _lib()
-    prec = _precision(precision, G.dtype)
+    prec = _precision(precision)
     m, n = G.shape[-2:]
     G = G.detach()
     out = torch.empty(G.shape, dtype=G.dtype, device=G.device)
@@ -124,8 +125,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
 
     params, grads, momenta: a matrix each or lists of them; weights of one
     shape and type go through the products together.  scale: a number, or None
-    for max(1, m / n) ** 0.5.  precision as in ``newton_schulz``, by the
-    weights' type.  Weights and momenta must have dense rows.
+    for max(1, m / n) ** 0.5.  precision as in ``newton_schulz``.  Weights and
+    momenta must have dense rows.
     """
     params, grads, momenta = _as_list(params), _as_list(grads), _as_list(momenta)
     capi.require(len(params) == len(grads) == len(momenta),
@@ -158,7 +159,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     for (shape, wt, gt, mt, sw, sg, sm, device), (ws_, gs, ms) in groups.items():
         lib = _lib()
         m, n = shape
-        prec = _precision(precision, wt)
+        prec = _precision(precision)
         ws_bytes = _workspace_bytes(m, n, len(ws_), prec)
         ws = torch.empty(ws_bytes // 8, dtype=torch.float64, device=ws_[0].device)
         factor = max(1.0, m / n) ** 0.5 if scale is None else scale
