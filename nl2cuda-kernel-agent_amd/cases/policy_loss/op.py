@@ -89,38 +89,41 @@ def _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
 
 
 def _forward(logits, labels, old_logp, advantages, ref_logp, mask, opts, keep):
-    """(loss, logp, logits and labels as they were read, rows, kept): kept
-    [3, tokens] holds the rows' statistics and coefficients for ``_backward``
-    (None unless ``keep``)."""
+    """(loss, logp, logits and labels as they were read, kept): kept [3, tokens]
+    holds the rows' statistics and coefficients for ``_backward`` (None unless
+    ``keep``)."""
     _check(logits, labels, old_logp, advantages, ref_logp, mask, opts["kl_coef"], opts["denom"])
     lib = _lib()
-    x, B, S, V, bs, rs = token_rows.layout(logits)
+    x, *rows = token_rows.layout(logits)
     held, given = _given(labels, old_logp, advantages, ref_logp, mask)
-    rows = (B, S, V, bs, rs, opts["ignore_index"], opts["temperature"])
     n = labels.numel()
-    ws_bytes = _workspace_bytes(B, S)
+    ws_bytes = _workspace_bytes(*rows[:2])
     ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
     loss, logp = ws.new_empty(()), ws.new_empty(labels.shape)
     kept = ws.new_empty(3 * n) if keep else None
     at = kept.data_ptr() if keep else 0
     st = capi.launch(lib.policy_loss_forward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], *given, loss.data_ptr(), logp.data_ptr(), at,
-                     at + 8 * n if at else 0, *rows, opts["clip_low"], opts["clip_high"],
-                     opts["kl_coef"], opts["denom"] or 0.0, ws.data_ptr(), ws_bytes)
+                     at + 8 * n if at else 0, *rows, opts["ignore_index"], opts["temperature"],
+                     opts["clip_low"], opts["clip_high"], opts["kl_coef"], opts["denom"] or 0.0,
+                     ws.data_ptr(), ws_bytes)
     if st:
         capi.check(st, lib.policy_loss_last_error, "policy_loss")
-    return loss, logp, x, held[0], rows, kept
+    return loss, logp, x, held[0], kept
 
 
-def _backward(x, labels, kept, gout, rows, shape):
+def _backward(logits, labels, kept, gout, opts):
     """dlogits of the loss, times the one-element tensor gout."""
+    token_rows.check(logits, labels, ("kept", kept))
     lib = _lib()
-    dlogits = torch.empty(shape, dtype=x.dtype, device=x.device)
+    x, *rows = token_rows.layout(logits)
+    labels, kept = labels.contiguous(), kept.contiguous()
+    dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
     at = kept.data_ptr()
     st = capi.launch(lib.policy_loss_backward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), at,
                      at + 8 * labels.numel() if at else 0, gout.data_ptr(), dlogits.data_ptr(),
-                     *rows)
+                     *rows, opts["ignore_index"], opts["temperature"])
     if st:
         capi.check(st, lib.policy_loss_last_error, "policy_loss backward")
     return dlogits
@@ -129,9 +132,9 @@ def _backward(x, labels, kept, gout, rows, shape):
 class PolicyLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, old_logp, advantages, ref_logp, mask, opts):
-        loss, logp, x, labels, ctx.rows, kept = _forward(logits, labels, old_logp, advantages,
-                                                         ref_logp, mask, opts, True)
-        ctx.shape = logits.shape
+        loss, logp, x, labels, kept = _forward(logits, labels, old_logp, advantages, ref_logp,
+                                               mask, opts, True)
+        ctx.opts = opts
         ctx.save_for_backward(x, labels, kept)
         ctx.mark_non_differentiable(logp)
         ctx.set_materialize_grads(False)
@@ -141,7 +144,7 @@ class PolicyLossFunction(torch.autograd.Function):
     def backward(ctx, gout, _):
         if gout is None:
             return (None,) * 7
-        return (_backward(*ctx.saved_tensors, gout, ctx.rows, ctx.shape),) + (None,) * 6
+        return (_backward(*ctx.saved_tensors, gout, ctx.opts),) + (None,) * 6
 
 
 def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *, clip_low=0.2,

@@ -42,9 +42,9 @@ def _workspace_bytes(B, S, pairs):
 
 
 def _forward(logits, labels, ref_seq_logp, opts, keep):
-    """(loss, seq_logp, logits and labels as they were read, rows, kept): kept
-    [3, tokens] holds the rows' statistics and coefficients for ``_backward``
-    (None unless ``keep``)."""
+    """(loss, seq_logp, logits and labels as they were read, kept): kept [3,
+    tokens] holds the rows' statistics and coefficients for ``_backward`` (None
+    unless ``keep``)."""
     cu_seqlens = opts["cu_seqlens"]
     token_rows.check(logits, labels, ("ref_seq_logp", ref_seq_logp), ("cu_seqlens", cu_seqlens))
     lib = _lib()
@@ -63,11 +63,10 @@ def _forward(logits, labels, ref_seq_logp, opts, keep):
         capi.require(ref_seq_logp.dtype == torch.float32 and ref_seq_logp.shape == (count,),
                      "ref_seq_logp must be float32 [2 N]")
         ref_seq_logp = ref_seq_logp.contiguous()
-    x, B, S, V, bs, rs = token_rows.layout(logits)
-    rows = (B, S, V, bs, rs, opts["ignore_index"])
+    x, *rows = token_rows.layout(logits)
     labels = labels.contiguous()
     n = labels.numel()
-    ws_bytes = _workspace_bytes(B, S, count // 2)
+    ws_bytes = _workspace_bytes(*rows[:2], count // 2)
     ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device)
     loss, seq = ws.new_empty(()), ws.new_empty(count)
     kept = ws.new_empty(3 * n) if keep else None
@@ -77,22 +76,25 @@ def _forward(logits, labels, ref_seq_logp, opts, keep):
                      0 if ref_seq_logp is None else ref_seq_logp.data_ptr(),
                      0 if cu_seqlens is None else cu_seqlens.data_ptr(), count // 2,
                      loss.data_ptr(), seq.data_ptr(), at, at + 8 * n if at else 0, *rows,
-                     opts["beta"], opts["label_smoothing"], 1 if opts["average"] else 0,
-                     ws.data_ptr(), ws_bytes)
+                     opts["ignore_index"], opts["beta"], opts["label_smoothing"],
+                     1 if opts["average"] else 0, ws.data_ptr(), ws_bytes)
     if st:
         capi.check(st, lib.preference_loss_last_error, "preference_loss")
-    return loss, seq, x, labels, rows, kept
+    return loss, seq, x, labels, kept
 
 
-def _backward(x, labels, kept, gout, rows, shape):
+def _backward(logits, labels, kept, gout, ignore_index):
     """dlogits of the loss, times the one-element tensor gout where given."""
+    token_rows.check(logits, labels, ("kept", kept))
     lib = _lib()
-    dlogits = torch.empty(shape, dtype=x.dtype, device=x.device)
+    x, *rows = token_rows.layout(logits)
+    labels, kept = labels.contiguous(), kept.contiguous()
+    dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
     at = kept.data_ptr()
     st = capi.launch(lib.preference_loss_backward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), at,
                      at + 8 * labels.numel() if at else 0, 0 if gout is None else gout.data_ptr(),
-                     dlogits.data_ptr(), *rows)
+                     dlogits.data_ptr(), *rows, ignore_index)
     if st:
         capi.check(st, lib.preference_loss_last_error, "preference_loss backward")
     return dlogits
@@ -101,8 +103,8 @@ def _backward(x, labels, kept, gout, rows, shape):
 class PreferenceLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref_seq_logp, opts):
-        loss, seq, x, labels, ctx.rows, kept = _forward(logits, labels, ref_seq_logp, opts, True)
-        ctx.shape = logits.shape
+        loss, seq, x, labels, kept = _forward(logits, labels, ref_seq_logp, opts, True)
+        ctx.ignore_index = opts["ignore_index"]
         ctx.save_for_backward(x, labels, kept)
         ctx.mark_non_differentiable(seq)
         ctx.set_materialize_grads(False)
@@ -112,7 +114,7 @@ class PreferenceLossFunction(torch.autograd.Function):
     def backward(ctx, gout, _):
         if gout is None:
             return None, None, None, None
-        return _backward(*ctx.saved_tensors, gout, ctx.rows, ctx.shape), None, None, None
+        return _backward(*ctx.saved_tensors, gout, ctx.ignore_index), None, None, None
 
 
 def preference_loss(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=0.1,
@@ -138,8 +140,8 @@ def preference_loss_and_grad(logits, labels, ref_seq_logp=None, *, cu_seqlens=No
     """(loss, seq_logp, dlogits) of ``preference_loss``, outside autograd."""
     opts = dict(cu_seqlens=cu_seqlens, beta=beta, label_smoothing=label_smoothing,
                 average=average, ignore_index=ignore_index)
-    loss, seq, x, labels, rows, kept = _forward(logits.detach(), labels, ref_seq_logp, opts, True)
-    return loss, seq, _backward(x, labels, kept, None, rows, logits.shape)
+    loss, seq, x, labels, kept = _forward(logits.detach(), labels, ref_seq_logp, opts, True)
+    return loss, seq, _backward(x, labels, kept, None, ignore_index)
 
 
 def _options(params):

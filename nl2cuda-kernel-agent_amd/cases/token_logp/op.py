@@ -38,43 +38,43 @@ def _lib():
 def logp_forward(logits, labels, temperature=1.0, ignore_index=-100, keep_stats=False):
     """(logp, stats): stats [..., 2] hold each row's maximum and sum of
     exponentials for ``logp_backward`` (None unless ``keep_stats``)."""
+    return _forward(logits, labels, temperature, ignore_index, keep_stats)[:2]
+
+
+def _forward(logits, labels, temperature, ignore_index, keep_stats):
+    """(logp, stats, logits and labels as they were read)."""
     token_rows.check(logits, labels)
-    x, B, S, V, bs, rs = token_rows.layout(logits)
-    return _forward(x, labels.contiguous(), (B, S, V, bs, rs, ignore_index, temperature),
-                    keep_stats)
-
-
-def _forward(x, labels, rows, keep_stats):
     lib = _lib()
+    x, *rows = token_rows.layout(logits)
+    labels = labels.contiguous()
     logp = torch.empty(labels.shape, dtype=torch.float32, device=x.device)
     stats = logp.new_empty(labels.shape + (2,)) if keep_stats else None
     st = capi.launch(lib.token_logp_forward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), logp.data_ptr(),
-                     stats.data_ptr() if keep_stats else 0, *rows)
+                     stats.data_ptr() if keep_stats else 0, *rows, ignore_index, temperature)
     if st:
         capi.check(st, lib.token_logp_last_error, "token_logp")
-    return logp, stats
+    return logp, stats, x, labels
 
 
 def logp_backward(logits, labels, stats, dlogp, temperature=1.0, ignore_index=-100):
     """dlogits = dlogp / temperature (onehot(labels) - softmax(logits / temperature))."""
-    token_rows.check(logits, labels, ("stats", stats), ("dlogp", dlogp))
     capi.require(dlogp.dtype == torch.float32 and dlogp.shape == labels.shape,
                  "dlogp must be float32 of the labels' shape")
     capi.require(stats.dtype == torch.float32 and stats.shape == labels.shape + (2,),
                  "stats must be the forward's")
-    x, B, S, V, bs, rs = token_rows.layout(logits)
-    return _backward(x, labels.contiguous(), stats.contiguous(), dlogp,
-                     (B, S, V, bs, rs, ignore_index, temperature), logits.shape)
+    return _backward(logits, labels, stats, dlogp, temperature, ignore_index)
 
 
-def _backward(x, labels, stats, dlogp, rows, shape):
+def _backward(logits, labels, stats, dlogp, temperature, ignore_index):
+    token_rows.check(logits, labels, ("stats", stats), ("dlogp", dlogp))
     lib = _lib()
-    dlogp = dlogp.contiguous()
-    dlogits = torch.empty(shape, dtype=x.dtype, device=x.device)
+    x, *rows = token_rows.layout(logits)
+    labels, stats, dlogp = labels.contiguous(), stats.contiguous(), dlogp.contiguous()
+    dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
     st = capi.launch(lib.token_logp_backward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), stats.data_ptr(),
-                     dlogp.data_ptr(), 0, dlogits.data_ptr(), *rows)
+                     dlogp.data_ptr(), 0, dlogits.data_ptr(), *rows, ignore_index, temperature)
     if st:
         capi.check(st, lib.token_logp_last_error, "token_logp backward")
     return dlogits
@@ -83,17 +83,15 @@ def _backward(x, labels, stats, dlogp, rows, shape):
 class TokenLogpFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, temperature, ignore_index):
-        token_rows.check(logits, labels)
-        x, B, S, V, bs, rs = token_rows.layout(logits)
-        labels = labels.contiguous()
-        ctx.rows, ctx.shape = (B, S, V, bs, rs, ignore_index, temperature), logits.shape
-        logp, stats = _forward(x, labels, ctx.rows, True)
+        logp, stats, x, labels = _forward(logits, labels, temperature, ignore_index, True)
+        ctx.temperature, ctx.ignore_index = temperature, ignore_index
         ctx.save_for_backward(x, labels, stats)
         return logp
 
     @staticmethod
     def backward(ctx, dlogp):
-        return _backward(*ctx.saved_tensors, dlogp, ctx.rows, ctx.shape), None, None, None
+        return (_backward(*ctx.saved_tensors, dlogp, ctx.temperature, ctx.ignore_index),
+                None, None, None)
 
 
 def token_logp(logits, labels, temperature=1.0, ignore_index=-100):

@@ -31,20 +31,20 @@ def check(logits, labels, *others):
 
 
 def layout(logits):
-    """(logits, B, S, V, batch stride, row stride), copied only if it must be."""
-    V = logits.size(-1)
-    if logits.dim() > 3 or (V > 1 and logits.stride(-1) != 1):
-        shape = logits.shape
+    """(logits, B, S, V, batch stride, row stride), copied only if it must be.
+
+    A backward takes it anew, of the tensor that autograd gives back: what a
+    saved-tensor hook put elsewhere returns as a copy with strides of its own.
+    """
+    V, d = logits.size(-1), logits.dim()
+    if d > 3 or (V > 1 and logits.stride(-1) != 1):
         logits = logits.contiguous()
-        if len(shape) > 3:
-            logits = logits.view(shape.numel() // V, V)
-    d = logits.dim()
     if d == 3:
         B, S = logits.size(0), logits.size(1)
         return logits, B, S, V, logits.stride(0), logits.stride(1)
     if d == 2:
         return logits, 1, logits.size(0), V, 0, logits.stride(0)
-    return logits, 1, 1, V, 0, V
+    return logits, 1, logits.numel() // V, V, 0, V
 
 
 def per_token(t, name, shape):

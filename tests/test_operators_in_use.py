@@ -52,3 +52,100 @@ def test_16_bit_weights_are_updated_from_full_iterates():
     O = ons.orthogonalise(G)
     off = ons.by_products(G, operand=2.0 ** -21, product=2.0 ** -22, seed=1) - O
     _within_a_rounding(Wd, W.double() - 0.05 * O, off, 2.0 ** -8, 0.05)
+
+
+# ---------------------------------------------------- a recorder for the library
+class _Library:
+    """Stands for a case's library: an entry is its name."""
+
+    def __getattr__(self, name):
+        return name
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """[(entry, arguments)] of the calls that the row operators would make, on CPU tensors."""
+    import cases.policy_loss.op as policy
+    import cases.preference_loss.op as preference
+    import cases.token_logp.op as logp
+    from framework import capi, token_rows
+    calls = []
+
+    def launch(entry, device, *args):
+        calls.append((entry, args))
+        return 0
+    monkeypatch.setattr(capi, "launch", launch)
+    monkeypatch.setattr(token_rows, "check", lambda *a: None)
+    for op in (logp, policy, preference):
+        monkeypatch.setattr(op, "_lib", _Library)
+    for op in (policy, preference):
+        monkeypatch.setattr(op, "_workspace_bytes", lambda *a: 1024)
+    return calls
+
+
+def _call(name, logits, labels):
+    """The differentiable answer of an operator."""
+    if name == "token_logp":
+        from cases.token_logp.op import token_logp
+        return token_logp(logits, labels).sum()
+    zeros = torch.zeros(labels.shape, device=labels.device)
+    if name == "policy_loss":
+        from cases.policy_loss.op import policy_loss
+        return policy_loss(logits, labels, zeros, zeros + 1.0)[0]
+    from cases.preference_loss.op import preference_loss
+    return preference_loss(logits, labels)[0]
+
+
+NAMES = ["token_logp", "policy_loss", "preference_loss"]
+
+
+def _view(layout, base):
+    """A view of base [4, 6, V] whose rows are not one after the other."""
+    return {"next_token": base[:, :-1], "every_other": base[:, ::2], "batch": base[::2],
+            "expanded": base[:, :1].expand(-1, 5, -1), "sequence_first": base.transpose(0, 1)}[layout]
+
+
+LAYOUTS = ["next_token", "every_other", "batch", "expanded", "sequence_first"]
+
+
+# ------------------------------------------------ tensors that hooks put elsewhere
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("name", NAMES)
+def test_backward_reads_the_saved_tensor_as_it_lies(name, layout, recorded):
+    """Hooks may return a dense copy of what was saved as a view: the backward's strides are those
+    of the copy, and its rows within it."""
+    base = torch.randn(4, 6, 7, requires_grad=True)
+    logits = _view(layout, base)
+    labels = torch.zeros(logits.shape[:-1], dtype=torch.int64)
+    packed = []
+
+    def pack(t):
+        packed.append(t.detach().clone(memory_format=torch.contiguous_format))
+        return len(packed) - 1
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda i: packed[i]):
+        out = _call(name, logits, labels)
+    out.backward()
+    (entry, args), = [c for c in recorded if c[0].endswith("_backward")]
+    copy, = [t for t in packed if t.data_ptr() == args[0]]
+    assert copy.shape == logits.shape
+    at = 7     # before them: tensors, the type, the gradient that comes in
+    assert args[at:at + 5] == (*logits.shape, copy.stride(0), copy.stride(1))
+    B, S, V, bs, rs = args[at:at + 5]
+    assert (B - 1) * bs + (S - 1) * rs + V <= copy.numel()
+    assert base.grad.shape == base.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("name", NAMES)
+def test_gradients_of_offloaded_views(name, layout):
+    announce(f"{name} offloaded {layout}")
+    base = torch.randn(4, 6, 700, generator=torch.Generator().manual_seed(1)).cuda()
+    base.requires_grad_(True)
+    shape = _view(layout, base).shape[:-1]
+    labels = torch.randint(0, 700, shape, generator=torch.Generator().manual_seed(2)).cuda()
+    (want,) = torch.autograd.grad(_call(name, _view(layout, base), labels), base)
+    with torch.autograd.graph.save_on_cpu():
+        out = _call(name, _view(layout, base), labels)
+    (got,) = torch.autograd.grad(out, base)
+    assert torch.equal(got, want)
