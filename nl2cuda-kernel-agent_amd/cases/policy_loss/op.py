@@ -170,7 +170,8 @@ def policy_loss_and_grad(logits, labels, old_logp, advantages, ref_logp=None, ma
                          ignore_index=-100, inplace=False):
     """(loss, logp, dlogits) of ``policy_loss`` in one pass over the logits,
     outside autograd.  ``inplace`` writes dlogits over the logits, which must
-    be dense then."""
+    be dense then; autograd knows of it, as of torch's own in-place operations:
+    a graph that needs the logits themselves raises in its backward."""
     _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
     lib = _lib()
     logits = logits.detach()
@@ -190,6 +191,8 @@ def policy_loss_and_grad(logits, labels, old_logp, advantages, ref_logp=None, ma
     if st:
         capi.check(st, lib.policy_loss_last_error, "policy_loss_and_grad")
     del keep
+    if inplace:  # for graphs that hold the logits
+        torch.autograd.graph.increment_version(logits)
     return loss, logp, dlogits
 
 

@@ -149,3 +149,41 @@ def test_gradients_of_offloaded_views(name, layout):
         out = _call(name, _view(layout, base), labels)
     (got,) = torch.autograd.grad(out, base)
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------- version counters
+def _in_place(logits):
+    from cases.policy_loss.op import policy_loss_and_grad
+    labels = torch.zeros(logits.shape[:-1], dtype=torch.int64, device=logits.device)
+    zeros = torch.zeros(labels.shape, device=logits.device)
+    loss, logp, dlogits = policy_loss_and_grad(logits, labels, zeros, zeros + 1.0, inplace=True)
+    return dlogits
+
+
+def _overwritten_logits_are_noticed(device):
+    base = torch.randn(2, 3, 8, device=device, requires_grad=True)
+    plain = base * 2.0
+    at = plain._version
+    plain.backward(_in_place(plain))         # the product did not keep its result
+    assert plain._version > at and base.grad is not None
+    for head in (torch.tanh, torch.exp, lambda t: torch.log_softmax(t, -1)):
+        logits = head(base)
+        with pytest.raises(RuntimeError, match="inplace"):
+            logits.backward(_in_place(logits))
+    logits = base * 2.0
+    earlier = _call("token_logp", logits, torch.zeros(2, 3, dtype=torch.int64, device=device))
+    _in_place(logits)
+    with pytest.raises(RuntimeError, match="inplace"):
+        earlier.backward()
+    with torch.inference_mode():
+        _in_place(torch.randn(2, 3, 8, device=device))
+
+
+def test_overwritten_logits_are_noticed(recorded):
+    _overwritten_logits_are_noticed("cpu")
+
+
+@pytest.mark.gpu
+def test_logits_overwritten_on_the_gpu_are_noticed():
+    announce("policy_loss in place, version counters")
+    _overwritten_logits_are_noticed("cuda")
