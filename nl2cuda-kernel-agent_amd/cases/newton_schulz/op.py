@@ -169,6 +169,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
                          ws.data_ptr(), ws_bytes)
         if st:
             capi.check(st, lib.newton_schulz_last_error, "muon_step")
+        torch.autograd.graph.increment_version(ws_ + ms)  # for graphs that hold them
 
 
 class Muon(torch.optim.Optimizer):

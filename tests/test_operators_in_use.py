@@ -187,3 +187,50 @@ def test_overwritten_logits_are_noticed(recorded):
 def test_logits_overwritten_on_the_gpu_are_noticed():
     announce("policy_loss in place, version counters")
     _overwritten_logits_are_noticed("cuda")
+
+
+@pytest.fixture
+def recorded_updates(monkeypatch):
+    """The same for muon_step, whose checks of devices are left out too."""
+    import cases.newton_schulz.op as op
+    from framework import capi
+    calls = []
+
+    def launch(entry, device, *args):
+        calls.append((entry, args))
+        return 0
+    monkeypatch.setattr(capi, "launch", launch)
+    monkeypatch.setattr(capi, "require", lambda *a: None)
+    monkeypatch.setattr(op, "_lib", _Library)
+    monkeypatch.setattr(op, "_workspace_bytes", lambda *a: 1024)
+    return calls
+
+
+def _updated_weights_are_noticed(device):
+    from cases.newton_schulz.op import Muon, muon_step
+    x = torch.randn(5, 8, device=device)
+    W = torch.nn.Parameter(torch.randn(8, 6, device=device))
+    V = torch.nn.Parameter(torch.randn(6, 4, device=device))
+    momenta = [torch.zeros(8, 6, device=device), torch.zeros(6, 4, device=device)]
+    opt = Muon([W, V], lr=0.1)
+    for step in (lambda: muon_step([W, V], [W.grad, V.grad], momenta, lr=0.1), opt.step):
+        W.grad = V.grad = None
+        out = (x @ W @ V).square().sum()
+        out.backward(retain_graph=True)
+        held = [W, V] + (momenta if step != opt.step else [opt.state[p]["momentum"]
+                                                           for p in (W, V) if p in opt.state])
+        before = [t._version for t in held]
+        step()
+        assert all(t._version > v for t, v in zip(held, before))
+        with pytest.raises(RuntimeError, match="inplace"):
+            out.backward()                      # the gradient of x @ W needs the old V
+
+
+def test_updated_weights_are_noticed(recorded_updates):
+    _updated_weights_are_noticed("cpu")
+
+
+@pytest.mark.gpu
+def test_weights_updated_on_the_gpu_are_noticed():
+    announce("muon_step, version counters")
+    _updated_weights_are_noticed("cuda")
