@@ -160,7 +160,7 @@ def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, 
     """
     opts = dict(clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, temperature=temperature,
                 denom=denom, ignore_index=ignore_index)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if token_rows.differentiated(logits):
         return PolicyLossFunction.apply(logits, labels, old_logp, advantages, ref_logp, mask, opts)
     return _forward(logits, labels, old_logp, advantages, ref_logp, mask, opts, False)[:2]
 

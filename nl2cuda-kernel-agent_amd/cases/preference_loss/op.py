@@ -130,7 +130,7 @@ def preference_loss(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=
     """
     opts = dict(cu_seqlens=cu_seqlens, beta=beta, label_smoothing=label_smoothing,
                 average=average, ignore_index=ignore_index)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if token_rows.differentiated(logits):
         return PreferenceLossFunction.apply(logits, labels, ref_seq_logp, opts)
     return _forward(logits, labels, ref_seq_logp, opts, False)[:2]
 

@@ -100,7 +100,7 @@ def token_logp(logits, labels, temperature=1.0, ignore_index=-100):
     Rows labelled ``ignore_index`` give 0 and a gradient of zeros, whatever
     their logits hold; another label outside [0, V) gives NaN.
     """
-    if logits.requires_grad and torch.is_grad_enabled():
+    if token_rows.differentiated(logits):
         return TokenLogpFunction.apply(logits, labels, temperature, ignore_index)
     return logp_forward(logits, labels, temperature, ignore_index)[0]
 

@@ -8,6 +8,7 @@ dense is copied.  Labels have the logits' leading shape and are int64.
 """
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from framework import capi
 
@@ -28,6 +29,13 @@ def check(logits, labels, *others):
         if t is not None:
             capi.require(t.is_cuda and t.get_device() == device,
                          f"{name} must be a tensor on the GPU of the logits")
+
+
+def differentiated(logits):
+    """Whether a call goes through its autograd function: where logits need a
+    gradient, and where they carry a tangent, which is refused there."""
+    return (logits.requires_grad and torch.is_grad_enabled() or
+            unpack_dual(logits).tangent is not None)
 
 
 def layout(logits):

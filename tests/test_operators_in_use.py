@@ -234,3 +234,29 @@ def test_updated_weights_are_noticed(recorded_updates):
 def test_weights_updated_on_the_gpu_are_noticed():
     announce("muon_step, version counters")
     _updated_weights_are_noticed("cuda")
+
+
+# ---------------------------------------------------- derivatives that are not there
+def _tangents_are_refused(name, device):
+    import torch.autograd.forward_ad as forward_ad
+    base = torch.randn(2, 3, 8, device=device)
+    labels = torch.zeros(2, 3, dtype=torch.int64, device=device)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(base, torch.ones_like(base))
+        with pytest.raises(NotImplementedError):
+            _call(name, dual, labels)
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            _call(name, dual, labels)
+        _call(name, base, labels)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_are_refused(name, recorded):
+    _tangents_are_refused(name, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_on_the_gpu_are_refused(name):
+    announce(f"{name} with a tangent")
+    _tangents_are_refused(name, "cuda")
