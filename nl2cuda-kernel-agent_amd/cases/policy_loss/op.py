@@ -144,7 +144,8 @@ class PolicyLossFunction(torch.autograd.Function):
     def backward(ctx, gout, _):
         if gout is None:
             return (None,) * 7
-        return (_backward(*ctx.saved_tensors, gout, ctx.opts),) + (None,) * 6
+        d = _backward(*ctx.saved_tensors, gout, ctx.opts)
+        return (token_rows.once(d),) + (None,) * 6
 
 
 def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, *, clip_low=0.2,

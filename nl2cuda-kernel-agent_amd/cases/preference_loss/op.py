@@ -114,7 +114,8 @@ class PreferenceLossFunction(torch.autograd.Function):
     def backward(ctx, gout, _):
         if gout is None:
             return None, None, None, None
-        return _backward(*ctx.saved_tensors, gout, ctx.ignore_index), None, None, None
+        d = _backward(*ctx.saved_tensors, gout, ctx.ignore_index)
+        return token_rows.once(d), None, None, None
 
 
 def preference_loss(logits, labels, ref_seq_logp=None, *, cu_seqlens=None, beta=0.1,

@@ -90,8 +90,8 @@ class TokenLogpFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dlogp):
-        return (_backward(*ctx.saved_tensors, dlogp, ctx.temperature, ctx.ignore_index),
-                None, None, None)
+        d = _backward(*ctx.saved_tensors, dlogp, ctx.temperature, ctx.ignore_index)
+        return token_rows.once(d), None, None, None
 
 
 def token_logp(logits, labels, temperature=1.0, ignore_index=-100):

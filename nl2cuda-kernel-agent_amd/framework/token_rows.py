@@ -38,6 +38,27 @@ def differentiated(logits):
             unpack_dual(logits).tangent is not None)
 
 
+class _Once(torch.autograd.Function):
+    """A gradient of the logits that refuses to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, dlogits, _):
+        return dlogits.view_as(dlogits)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("operators over rows of logits have no second derivatives")
+
+
+def once(dlogits):
+    """A backward's answer, which autograd takes for a constant.  Where a graph of the
+    gradients is made (create_graph) it refuses a second derivative instead, also
+    where the gradient that came in needs none: dlogits depends on the logits."""
+    if not torch.is_grad_enabled():
+        return dlogits
+    return _Once.apply(dlogits, dlogits.new_empty(0).requires_grad_(True))
+
+
 def layout(logits):
     """(logits, B, S, V, batch stride, row stride), copied only if it must be.
 

@@ -260,3 +260,33 @@ def test_tangents_are_refused(name, recorded):
 def test_tangents_on_the_gpu_are_refused(name):
     announce(f"{name} with a tangent")
     _tangents_are_refused(name, "cuda")
+
+
+def _second_derivatives_are_refused(name, device):
+    base = torch.randn(2, 3, 8, device=device, requires_grad=True)
+    labels = torch.zeros(2, 3, dtype=torch.int64, device=device)
+    for logits in (base, base[..., ::2]):        # read where they lie, and copied
+        out = _call(name, logits, labels)
+        (grad,) = torch.autograd.grad(out, base, create_graph=True)
+        with pytest.raises(RuntimeError, match="second"):
+            (out + grad.square().sum()).backward()
+        out = _call(name, logits, labels)
+        out.backward(create_graph=True)          # fine where nobody goes on from it
+        base.grad = None
+        out = _call(name, logits, labels)
+        (grad,) = torch.autograd.grad(out, base)
+        assert not grad.requires_grad
+
+
+@pytest.mark.filterwarnings("ignore:Using backward")
+@pytest.mark.parametrize("name", NAMES)
+def test_second_derivatives_are_refused(name, recorded):
+    _second_derivatives_are_refused(name, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore:Using backward")
+@pytest.mark.parametrize("name", NAMES)
+def test_second_derivatives_on_the_gpu_are_refused(name):
+    announce(f"{name} differentiated twice")
+    _second_derivatives_are_refused(name, "cuda")
