@@ -189,6 +189,28 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 capi.require(p.dim() == 2, "Muon updates matrices only")
 
+    def load_state_dict(self, state_dict):
+        """As torch's, which rounds state to its weight's type; momenta keep their 32 bits."""
+        taken = []
+
+        def restore(_):
+            state = taken[-1]
+            ids = [i for group in state["param_groups"] for i in group["params"]]
+            params = [p for group in self.param_groups for p in group["params"]]
+            for i, p in zip(ids, params):
+                if "momentum" in state["state"].get(i, ()):
+                    self.state[p]["momentum"] = state["state"][i]["momentum"].to(
+                        p.device, torch.float32, copy=True,
+                        memory_format=torch.contiguous_format)
+        # the state after all other hooks that may replace it, restored before those that see it
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, state: taken.append(state)),
+                 self.register_load_state_dict_post_hook(restore, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -290,3 +290,72 @@ def test_second_derivatives_are_refused(name, recorded):
 def test_second_derivatives_on_the_gpu_are_refused(name):
     announce(f"{name} differentiated twice")
     _second_derivatives_are_refused(name, "cuda")
+
+
+# ------------------------------------------------------------- saved optimisers
+def _momenta(opt):
+    return [opt.state[p]["momentum"] for g in opt.param_groups for p in g["params"]
+            if p in opt.state]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_a_loaded_optimiser_keeps_its_momenta(dtype):
+    from cases.newton_schulz.op import Muon
+    g = torch.Generator().manual_seed(5)
+
+    def weights():
+        return [torch.nn.Parameter(torch.zeros(4, 6, dtype=dtype)) for _ in range(3)]
+    first = Muon([{"params": weights()}, {"params": weights(), "lr": 0.5}])
+    for p in first.param_groups[0]["params"][:2] + first.param_groups[1]["params"]:
+        first.state[p]["momentum"] = torch.randn(4, 6, generator=g)
+    saved = first.state_dict()
+    seen = []
+    second = Muon([{"params": weights()}, {"params": weights()}])
+    second.register_load_state_dict_post_hook(lambda o: seen.append([m.dtype for m in _momenta(o)]))
+    second.load_state_dict(saved)
+    assert seen == [[torch.float32] * 5] and second.param_groups[1]["lr"] == 0.5
+    for a, b in zip(_momenta(first), _momenta(second)):
+        assert torch.equal(a, b) and b.dtype == torch.float32
+        assert a.data_ptr() != b.data_ptr()      # each updates its own
+    # what hooks put in the place of the saved state counts; and a 16-bit momentum is widened
+    third = Muon([{"params": weights()}, {"params": weights()}])
+
+    def narrow(_, state):
+        state["state"] = {k: {"momentum": v["momentum"].bfloat16()}
+                          for k, v in state["state"].items()}
+        return state
+    third.register_load_state_dict_pre_hook(narrow)
+    third.load_state_dict(first.state_dict())
+    for a, b in zip(_momenta(first), _momenta(third)):
+        assert b.dtype == torch.float32 and torch.equal(a.bfloat16().float(), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_a_resumed_run_goes_on_as_it_was(dtype, tmp_path):
+    from cases.newton_schulz.op import Muon
+    announce(f"Muon saved and loaded {dtype}")
+    g = torch.Generator().manual_seed(6)
+    start = [(0.02 * torch.randn(s, generator=g)).to(dtype) for s in ((70, 90), (40, 30))]
+    grads = [[torch.randn(p.shape, generator=g).to(dtype) for p in start] for _ in range(4)]
+
+    def make(values):
+        ps = [torch.nn.Parameter(v.cuda()) for v in values]
+        return ps, Muon(ps, lr=0.05)
+
+    def run(ps, opt, steps):
+        for step in steps:
+            for p, x in zip(ps, grads[step]):
+                p.grad = x.cuda()
+            opt.step()
+    whole, opt = make(start)
+    run(whole, opt, range(4))
+    half, opt2 = make(start)
+    run(half, opt2, range(2))
+    torch.save({"weights": [p.detach() for p in half], "muon": opt2.state_dict()}, tmp_path / "at2")
+    saved = torch.load(tmp_path / "at2", weights_only=True)
+    resumed, opt3 = make(saved["weights"])
+    opt3.load_state_dict(saved["muon"])
+    run(resumed, opt3, range(2, 4))
+    assert all(torch.equal(a, b) for a, b in zip(whole, resumed))
+    assert all(torch.equal(a, b) for a, b in zip(_momenta(opt), _momenta(opt3)))
