@@ -131,8 +131,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     params, grads, momenta = _as_list(params), _as_list(grads), _as_list(momenta)
     capi.require(len(params) == len(grads) == len(momenta),
                  "params, grads and momenta must be lists of one length")
-    capi.require(len({t.data_ptr() for t in params + momenta}) == 2 * len(params) or
-                 any(t.numel() == 0 for t in params), "a weight or momentum is listed twice")
+    written = [t.data_ptr() for t in params + momenta if t.numel()]
+    capi.require(len(set(written)) == len(written), "a weight or momentum is listed twice")
     groups = {}
     for W, G, M in zip(params, grads, momenta):
         capi.require(W.is_cuda and G.is_cuda and M.is_cuda and

@@ -359,3 +359,27 @@ def test_a_resumed_run_goes_on_as_it_was(dtype, tmp_path):
     run(resumed, opt3, range(2, 4))
     assert all(torch.equal(a, b) for a, b in zip(whole, resumed))
     assert all(torch.equal(a, b) for a, b in zip(_momenta(opt), _momenta(opt3)))
+
+
+# ------------------------------------------------------ operands that share memory
+def test_a_weight_listed_twice_is_refused_beside_empty_ones():
+    from cases.newton_schulz.op import muon_step
+    W, V, M, N, G = (torch.randn(4, 6) for _ in range(5))
+    empty = torch.empty(0, 6)
+    for weights, momenta in (([W, W], [M, N]), ([W, V], [M, M]), ([W, V], [V, N])):
+        with pytest.raises(RuntimeError, match="twice"):
+            muon_step(weights, [G, G], momenta, lr=0.1)
+        with pytest.raises(RuntimeError, match="twice"):
+            muon_step(weights + [empty], [G, G, empty], momenta + [empty], lr=0.1)
+
+
+@pytest.mark.gpu
+def test_empty_weights_are_passed_over():
+    from cases.newton_schulz.op import muon_step
+    announce("muon_step with empty weights")
+    W, G, M = (torch.randn(4, 6, device="cuda") for _ in range(3))
+    V, N = W.clone(), M.clone()
+    empty = torch.empty(0, 6, device="cuda")
+    muon_step([empty, W, empty], [empty, G, empty], [empty, M, empty], lr=0.1)
+    muon_step(V, G, N, lr=0.1)
+    assert torch.equal(W, V) and torch.equal(M, N)
