@@ -60,7 +60,8 @@ int newton_schulz(const void* const* in, int in_dtype, int64_t in_row_stride, vo
                   int steps, float a, float b, float c, float eps, int precision, void* workspace,
                   size_t workspace_bytes, hipStream_t stream);
 
-/* One step of every weight: updates the momenta and the weights in place. */
+/* One step of every weight: updates the momenta and the weights in place.  None
+ * of them may overlap another, nor a gradient (but for that of the same weight). */
 int muon_update(void* const* weights, int weight_dtype, int64_t weight_row_stride,
                 const void* const* grads, int grad_dtype, int64_t grad_row_stride,
                 void* const* momenta, int momentum_dtype, int64_t momentum_row_stride, int64_t m,

@@ -126,13 +126,15 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     params, grads, momenta: a matrix each or lists of them; weights of one
     shape and type go through the products together.  scale: a number, or None
     for max(1, m / n) ** 0.5.  precision as in ``newton_schulz``.  Weights and
-    momenta must have dense rows.
+    momenta must have dense rows, and no weight, momentum or gradient may overlap
+    another that the call writes.
     """
     params, grads, momenta = _as_list(params), _as_list(grads), _as_list(momenta)
     capi.require(len(params) == len(grads) == len(momenta),
                  "params, grads and momenta must be lists of one length")
     written = [t.data_ptr() for t in params + momenta if t.numel()]
     capi.require(len(set(written)) == len(written), "a weight or momentum is listed twice")
+    written = set(written)
     groups = {}
     for W, G, M in zip(params, grads, momenta):
         capi.require(W.is_cuda and G.is_cuda and M.is_cuda and
@@ -151,6 +153,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         if sg is None or sg < n:
             G = G.contiguous()
             sg = n
+        capi.require(G.data_ptr() not in written or G.data_ptr() == W.data_ptr(),
+                     "a gradient shares memory with a momentum or another's weight")
         key = (W.shape, W.dtype, G.dtype, M.dtype, sw, sg, sm, W.get_device())
         groups.setdefault(key, ([], [], []))
         for to, t in zip(groups[key], (W, G, M)):

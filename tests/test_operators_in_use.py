@@ -199,8 +199,9 @@ def recorded_updates(monkeypatch):
     def launch(entry, device, *args):
         calls.append((entry, args))
         return 0
+    require = capi.require
     monkeypatch.setattr(capi, "launch", launch)
-    monkeypatch.setattr(capi, "require", lambda *a: None)
+    monkeypatch.setattr(capi, "require", lambda cond, msg: require(cond or "one GPU" in msg, msg))
     monkeypatch.setattr(op, "_lib", _Library)
     monkeypatch.setattr(op, "_workspace_bytes", lambda *a: 1024)
     return calls
@@ -383,3 +384,21 @@ def test_empty_weights_are_passed_over():
     muon_step([empty, W, empty], [empty, G, empty], [empty, M, empty], lr=0.1)
     muon_step(V, G, N, lr=0.1)
     assert torch.equal(W, V) and torch.equal(M, N)
+
+
+def test_a_gradient_that_the_call_writes_is_refused(recorded_updates):
+    """The momentum is stored before the gradient is read for the last time, and a weight while
+    others' gradients still are."""
+    from cases.newton_schulz.op import muon_step
+    W, V, M, N, G, H = (torch.randn(6, 6) for _ in range(6))
+    for grads in ([M, H], [G, M], [N, H], [V, H], [G, W]):
+        with pytest.raises(RuntimeError, match="gradient shares"):
+            muon_step([W, V], grads, [M, N], lr=0.1)
+    assert not recorded_updates
+    muon_step([W, V], [G, G], [M, N], lr=0.1)           # one gradient for both
+    muon_step([W, V], [M.T, H], [M, N], lr=0.1)         # columns: copied before the first launch
+    muon_step([W, V], [W, V], [M, N], lr=0.1)           # each read whole before it is written
+    flat = torch.randn(6, 6 * 6)                        # columns of one buffer
+    muon_step([flat[:, :6], flat[:, 6:12]], [flat[:, 12:18], flat[:, 18:24]],
+              [flat[:, 24:30], flat[:, 30:]], lr=0.1)
+    assert len(recorded_updates) == 4
