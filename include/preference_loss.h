@@ -16,8 +16,8 @@
  * 2 N sequences are the batch entries, B = 2 N; with it the rows of B = 1 hold
  * them one after the other, sequence i from cu_seqlens[i] to cu_seqlens[i + 1]
  * (int64, 2 N + 1 of them, on the device; not validated: rows in no sequence
- * get zeros, offsets are clamped into the rows).  ref_seq [2 N] (NULL: zeros)
- * and seq_logp [2 N] float32.
+ * get zeros, offsets are clamped into the rows).  N is at most 2^24 - 1.
+ * ref_seq [2 N] (NULL: zeros) and seq_logp [2 N] float32.
  *
  * Sums over tokens and pairs are taken in 64 bits in a fixed order: all
  * results are bitwise repeatable.  Workspace: scratch without initial

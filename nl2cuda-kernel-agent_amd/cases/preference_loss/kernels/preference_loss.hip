@@ -33,6 +33,7 @@ struct SequenceOp {
 };
 
 constexpr int kPairBlock = 256;
+constexpr int64_t kMostPairs = nl2k::max_blocks(kPairBlock);  // a workgroup each
 
 __device__ __forceinline__ double block_sum(double v, double* red) {
   v = nl2k::wave_sum(v);
@@ -125,8 +126,7 @@ size_t even(size_t n) { return (n + 1) / 2 * 2; }
 }  // namespace
 
 extern "C" size_t preference_loss_workspace_bytes(int64_t B, int64_t S, int64_t pairs) {
-  if (B < 0 || S < 0 || pairs < 1 || pairs > (int64_t)1 << 28 ||
-      (S && B > ((int64_t)1 << 28) / S))
+  if (B < 0 || S < 0 || pairs < 1 || pairs > kMostPairs || (S && B > ((int64_t)1 << 28) / S))
     return 0;
   return 4 * (even((size_t)(B * S)) + even((size_t)pairs));
 }
@@ -143,8 +143,10 @@ extern "C" int preference_loss_forward(const void* logits, int dtype, const int6
   int st = nl2k::rows::make_shape(B, S, V, batch_stride, row_stride, ignore_index, 1.f, dtype,
                                   &sh);
   if (st) return st;
-  if (pairs < 1 || pairs > (int64_t)1 << 28 || (!cu_seqlens && B != 2 * pairs) ||
-      (cu_seqlens && B != 1))
+  if (pairs > kMostPairs)
+    return nl2k::fail(NL2K_ERR_OVERFLOW, "at most %lld pairs, got %lld", (long long)kMostPairs,
+                      (long long)pairs);
+  if (pairs < 1 || (!cu_seqlens && B != 2 * pairs) || (cu_seqlens && B != 1))
     return nl2k::fail(NL2K_ERR_SHAPE,
                       "need pairs >= 1 and B = 2 pairs, or B = 1 with cu_seqlens, got pairs=%lld "
                       "B=%lld", (long long)pairs, (long long)B);

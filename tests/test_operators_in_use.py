@@ -402,3 +402,23 @@ def test_a_gradient_that_the_call_writes_is_refused(recorded_updates):
     muon_step([flat[:, :6], flat[:, 6:12]], [flat[:, 12:18], flat[:, 18:24]],
               [flat[:, 24:30], flat[:, 30:]], lr=0.1)
     assert len(recorded_updates) == 4
+
+
+# --------------------------------------------------------------- sizes and scalars
+def test_more_pairs_than_a_launch_has_are_refused():
+    import ctypes
+
+    from test_capi import STATUS, _load
+    lib = _load("cases.preference_loss.op")
+    P = ctypes.c_void_p(1 << 20)                        # never dereferenced
+    most = (2 ** 32 - 1) // 256                         # workgroups of 256, one a pair
+    assert lib.preference_loss_workspace_bytes(1, 8, most) == 4 * (8 + most + 1)
+    assert lib.preference_loss_workspace_bytes(1, 8, most + 1) == 0
+
+    def call(pairs, cu, B, workspace_bytes):
+        return lib.preference_loss_forward(P, 0, P, P, cu, pairs, P, P, P, P, B, 1, 8, 8, 8, -100,
+                                           0.1, 0.0, 0, P, workspace_bytes, None)
+    for cu, B in ((P, 1), (None, 2 * (most + 1))):
+        assert call(most + 1, cu, B, 1 << 40) == STATUS["NL2K_ERR_OVERFLOW"]
+        assert b"pairs" in lib.preference_loss_last_error()
+    assert call(most, P, 1, 8) == STATUS["NL2K_ERR_WORKSPACE"]      # as many as that are taken
