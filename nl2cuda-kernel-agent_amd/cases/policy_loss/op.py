@@ -9,6 +9,7 @@ GPU the library refuses to load.
 """
 
 import functools
+import math
 import os
 
 import torch
@@ -85,7 +86,9 @@ def _check(logits, labels, old_logp, advantages, ref_logp, mask, kl_coef, denom)
     token_rows.check(logits, labels, ("old_logp", old_logp), ("advantages", advantages),
                      ("ref_logp", ref_logp), ("mask", mask))
     capi.require(kl_coef == 0.0 or ref_logp is not None, "kl_coef needs ref_logp")
-    capi.require(denom is None or denom > 0, "denom must be positive")
+    # as the C entry gets it: a 0 there stands for the sum of the weights
+    capi.require(denom is None or 0.0 < capi.c_float(denom).value < math.inf,
+                 "denom must be positive and finite in 32 bits")
 
 
 def _forward(logits, labels, old_logp, advantages, ref_logp, mask, opts, keep):
@@ -157,7 +160,7 @@ def policy_loss(logits, labels, old_logp, advantages, ref_logp=None, mask=None, 
     advantages too, or one a sequence ([B] or [B, 1]); mask bool or float32
     weights.  A token counts unless its label is ``ignore_index`` or its weight
     0; what it and its other inputs hold then is not looked at.  The weighted
-    terms are divided by ``denom`` (> 0), or by the sum of the weights.
+    terms are divided by ``denom`` (> 0 in float32), or by the sum of the weights.
     """
     opts = dict(clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, temperature=temperature,
                 denom=denom, ignore_index=ignore_index)

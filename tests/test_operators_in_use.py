@@ -422,3 +422,15 @@ def test_more_pairs_than_a_launch_has_are_refused():
         assert call(most + 1, cu, B, 1 << 40) == STATUS["NL2K_ERR_OVERFLOW"]
         assert b"pairs" in lib.preference_loss_last_error()
     assert call(most, P, 1, 8) == STATUS["NL2K_ERR_WORKSPACE"]      # as many as that are taken
+
+
+@pytest.mark.parametrize("denom", [1e-46, 1e39, 0.0, -1.0, float("nan"), float("inf")])
+def test_a_denominator_that_32_bits_do_not_hold_is_refused(denom, recorded):
+    from cases.policy_loss.op import policy_loss, policy_loss_and_grad
+    logits, labels = torch.randn(2, 3, 8), torch.zeros(2, 3, dtype=torch.int64)
+    zeros = torch.zeros(2, 3)
+    for call in (policy_loss, policy_loss_and_grad):
+        with pytest.raises(RuntimeError, match="denom"):
+            call(logits, labels, zeros, zeros, denom=denom)
+        call(logits, labels, zeros, zeros, denom=1e-40)
+    assert len(recorded) == 2
