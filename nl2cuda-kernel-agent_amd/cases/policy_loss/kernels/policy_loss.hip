@@ -299,7 +299,9 @@ extern "C" int policy_loss_and_grad(const void* logits, int dtype, const int64_t
     if (!dlogits)
       return nl2k::fail(NL2K_ERR_NULL, "policy_loss_and_grad: dlogits is required");
     if ((st = nl2k::rows::check_align(dlogits, dtype, "dlogits"))) return st;
-    if (dlogits == logits && (row_stride != V || (B > 1 && batch_stride != S * V)))
+    // a dimension of one has no stride to speak of
+    if (dlogits == logits &&
+        ((S > 1 && row_stride != V) || (B > 1 && batch_stride != S * V)))
       return nl2k::fail(NL2K_ERR_SHAPE, "policy_loss_and_grad: in place needs dense logits");
     sum_weights(c, stream);
     st = nl2k::rows::launch_fused(logits, dtype, labels, dlogits, c.sh, c.op, stream);

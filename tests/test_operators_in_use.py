@@ -434,3 +434,23 @@ def test_a_denominator_that_32_bits_do_not_hold_is_refused(denom, recorded):
             call(logits, labels, zeros, zeros, denom=denom)
         call(logits, labels, zeros, zeros, denom=1e-40)
     assert len(recorded) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["one_token", "one_row", "one_sequence"])
+def test_in_place_where_a_stride_stands_for_nothing(layout):
+    """Contiguous logits whose dimensions of one element have strides of their own."""
+    from cases.policy_loss.op import policy_loss_and_grad
+    announce(f"policy_loss in place {layout}")
+    base = torch.randn(1, 5, 40, generator=torch.Generator().manual_seed(3)).cuda()
+    logits = {"one_token": base.transpose(0, 1),            # [5, 1, 40], strides 40, 200, 1
+              "one_row": base[0, ::2][:1],                  # [1, 40], strides 80, 1
+              "one_sequence": base.expand(3, 5, 40)[:1]}[layout]
+    assert logits.is_contiguous()
+    shape = logits.shape[:-1]
+    labels = torch.randint(0, 40, shape, generator=torch.Generator().manual_seed(4)).cuda()
+    old = torch.full(shape, -4.0, device="cuda")
+    want = policy_loss_and_grad(logits, labels, old, old)
+    got = policy_loss_and_grad(logits, labels, old, old, inplace=True)
+    assert got[2].data_ptr() == logits.data_ptr()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
