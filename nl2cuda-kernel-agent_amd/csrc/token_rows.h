@@ -760,6 +760,21 @@ inline int launch_fused_at(const void* logits, const int64_t* labels, void* dlog
   return check_launch("fused_kernel");
 }
 
+// Rows that no registers hold take a workgroup of 1024, those below a window a wave.
+template <class T, int TPR, class Op>
+inline int launch_fused_long_at(const void* logits, const int64_t* labels, void* dlogits,
+                                const Shape& sh, const Op& op, hipStream_t s) {
+  unsigned grid;
+  if (const int st = row_grid<TPR>(sh, 1, &grid)) return st;
+  const bool past = bytes_of<T>(sh) > Caches::kGradient;
+  auto* kernel = past ? &fused_long_kernel<T, TPR, 4, true, Op>
+                      : &fused_long_kernel<T, TPR, 4, false, Op>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(block_of<TPR>()), 0, s,
+                     static_cast<const typename Elem<T>::type*>(logits), labels,
+                     static_cast<typename Elem<T>::type*>(dlogits), sh, op);
+  return check_launch("fused_long_kernel");
+}
+
 // The fewest lanes whose registers hold a row, 16 windows each at most.
 template <class Op>
 inline int launch_fused(const void* logits, int dtype, const int64_t* labels, void* dlogits,
@@ -770,17 +785,9 @@ inline int launch_fused(const void* logits, int dtype, const int64_t* labels, vo
     // what made the logits left its last rows in the caches, what reads the gradient begins with
     // the first: as quick alone, with such a reader 369 us against 396 at 512 MiB
     sh.last_first = true;
-    if (sh.V < Elem<T>::E || n > 16384) {
-      unsigned grid;
-      if (const int st = row_grid<1024>(sh, 1, &grid)) return st;
-      const bool past = bytes_of<T>(sh) > Caches::kGradient;
-      auto* kernel = past ? &fused_long_kernel<T, 1024, 4, true, Op>
-                          : &fused_long_kernel<T, 1024, 4, false, Op>;
-      hipLaunchKernelGGL(kernel, dim3(grid), dim3(1024), 0, s,
-                         static_cast<const typename Elem<T>::type*>(logits), labels,
-                         static_cast<typename Elem<T>::type*>(dlogits), sh, op);
-      return check_launch("fused_long_kernel");
-    }
+    if (sh.V < Elem<T>::E)
+      return launch_fused_long_at<T, 64>(logits, labels, dlogits, sh, op, s);
+    if (n > 16384) return launch_fused_long_at<T, 1024>(logits, labels, dlogits, sh, op, s);
     if (n <= 128) return launch_fused_at<T, 64, 2>(logits, labels, dlogits, sh, op, s);
     if (n <= 512) return launch_fused_at<T, 64, 8>(logits, labels, dlogits, sh, op, s);
     if (n <= 1024) return launch_fused_at<T, 256, 4>(logits, labels, dlogits, sh, op, s);

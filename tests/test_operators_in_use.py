@@ -454,3 +454,24 @@ def test_in_place_where_a_stride_stands_for_nothing(layout):
     got = policy_loss_and_grad(logits, labels, old, old, inplace=True)
     assert got[2].data_ptr() == logits.data_ptr()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,dtype", [(2, torch.bfloat16), (3, torch.float32)])
+def test_millions_of_rows_of_a_few_classes(v, dtype):
+    """More rows than there are workgroups of 1024: a policy over a few actions."""
+    from cases.policy_loss.op import policy_loss, policy_loss_and_grad
+    rows = 2 ** 22 + 5
+    announce(f"policy_loss {rows} rows of {v} {dtype}")
+    g = torch.Generator(device="cuda").manual_seed(v)
+    logits = torch.randn(rows, v, generator=g, device="cuda").to(dtype)
+    labels = torch.randint(0, v, (rows,), generator=g, device="cuda")
+    old = -torch.rand(rows, generator=g, device="cuda")
+    adv = torch.randn(rows, generator=g, device="cuda")
+    loss, logp, d = policy_loss_and_grad(logits, labels, old, adv, denom=1000.0)
+    whole, lp = policy_loss(logits, labels, old, adv, denom=1000.0)
+    assert torch.equal(loss, whole) and torch.equal(logp, lp)
+    for part in (slice(0, 1000), slice(2 ** 21, 2 ** 21 + 1000), slice(rows - 1000, rows)):
+        _, lp, dp = policy_loss_and_grad(logits[part], labels[part], old[part], adv[part],
+                                         denom=1000.0)
+        assert torch.equal(logp[part], lp) and torch.equal(d[part], dp)
