@@ -475,3 +475,33 @@ def test_millions_of_rows_of_a_few_classes(v, dtype):
         _, lp, dp = policy_loss_and_grad(logits[part], labels[part], old[part], adv[part],
                                          denom=1000.0)
         assert torch.equal(logp[part], lp) and torch.equal(d[part], dp)
+
+
+# ------------------------------------------------------------ types and the case API
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["step", "inplace", "train"])
+@pytest.mark.parametrize("v", [1, 7, 33, 2050, 8190, 65540, 131080])
+def test_policy_loss_of_float16(v, how):
+    import test_gpu_policy_loss as policy
+    announce(f"policy_loss float16, width {v} {how}")
+    b, s = (3, 5) if v < 5000 else (2, 2)
+    g, x, labels, old, ref, adv = policy._inputs(b, s, v, torch.float16)
+    mask = torch.rand(b, s, generator=g) < 0.7
+    mask[0, 0] = True
+    labels[-1, -1] = policy.orow.IGNORE
+    got = policy._run(x, labels, old, ref, adv, mask, 0.05, how)
+    assert got[2].dtype == torch.float16
+    policy._compare(x, labels, old, ref, adv, mask, 0.05, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES + ["newton_schulz"])
+def test_the_case_passes_the_framework_s_own_check(name):
+    import importlib
+
+    from framework.verify import verify_all
+    announce(f"verify_all {name}")
+    case = importlib.import_module(f"cases.{name}").CASE
+    op = importlib.import_module(f"cases.{name}.op")
+    ok, report = verify_all(case, op.candidate, device="cuda")
+    assert ok, report
