@@ -117,10 +117,8 @@ def _forward(logits, labels, old_logp, advantages, ref_logp, mask, opts, keep):
 
 def _backward(logits, labels, kept, gout, opts):
     """dlogits of the loss, times the one-element tensor gout."""
-    token_rows.check(logits, labels, ("kept", kept))
     lib = _lib()
-    x, *rows = token_rows.layout(logits)
-    labels, kept = labels.contiguous(), kept.contiguous()
+    labels, kept, x, *rows = token_rows.saved(logits, labels, kept, 3)
     dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
     at = kept.data_ptr()
     st = capi.launch(lib.policy_loss_backward, x.get_device(), x.data_ptr(),

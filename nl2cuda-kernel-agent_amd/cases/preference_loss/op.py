@@ -85,10 +85,8 @@ def _forward(logits, labels, ref_seq_logp, opts, keep):
 
 def _backward(logits, labels, kept, gout, ignore_index):
     """dlogits of the loss, times the one-element tensor gout where given."""
-    token_rows.check(logits, labels, ("kept", kept))
     lib = _lib()
-    x, *rows = token_rows.layout(logits)
-    labels, kept = labels.contiguous(), kept.contiguous()
+    labels, kept, x, *rows = token_rows.saved(logits, labels, kept, 3)
     dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
     at = kept.data_ptr()
     st = capi.launch(lib.preference_loss_backward, x.get_device(), x.data_ptr(),

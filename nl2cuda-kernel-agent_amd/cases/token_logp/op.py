@@ -59,6 +59,7 @@ def _forward(logits, labels, temperature, ignore_index, keep_stats):
 
 def logp_backward(logits, labels, stats, dlogp, temperature=1.0, ignore_index=-100):
     """dlogits = dlogp / temperature (onehot(labels) - softmax(logits / temperature))."""
+    token_rows.check(logits, labels, ("stats", stats), ("dlogp", dlogp))
     capi.require(dlogp.dtype == torch.float32 and dlogp.shape == labels.shape,
                  "dlogp must be float32 of the labels' shape")
     capi.require(stats.dtype == torch.float32 and stats.shape == labels.shape + (2,),
@@ -67,10 +68,9 @@ def logp_backward(logits, labels, stats, dlogp, temperature=1.0, ignore_index=-1
 
 
 def _backward(logits, labels, stats, dlogp, temperature, ignore_index):
-    token_rows.check(logits, labels, ("stats", stats), ("dlogp", dlogp))
     lib = _lib()
-    x, *rows = token_rows.layout(logits)
-    labels, stats, dlogp = labels.contiguous(), stats.contiguous(), dlogp.contiguous()
+    labels, stats, x, *rows = token_rows.saved(logits, labels, stats, 2)
+    dlogp = dlogp.contiguous()
     dlogits = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
     st = capi.launch(lib.token_logp_backward, x.get_device(), x.data_ptr(),
                      token_rows.DTYPES[x.dtype], labels.data_ptr(), stats.data_ptr(),

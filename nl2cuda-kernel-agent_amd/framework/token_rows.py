@@ -60,11 +60,7 @@ def once(dlogits):
 
 
 def layout(logits):
-    """(logits, B, S, V, batch stride, row stride), copied only if it must be.
-
-    A backward takes it anew, of the tensor that autograd gives back: what a
-    saved-tensor hook put elsewhere returns as a copy with strides of its own.
-    """
+    """(logits, B, S, V, batch stride, row stride), copied only if it must be."""
     V, d = logits.size(-1), logits.dim()
     if d > 3 or (V > 1 and logits.stride(-1) != 1):
         logits = logits.contiguous()
@@ -74,6 +70,17 @@ def layout(logits):
     if d == 2:
         return logits, 1, logits.size(0), V, 0, logits.stride(0)
     return logits, 1, logits.numel() // V, V, 0, V
+
+
+def saved(logits, labels, kept, per_row):
+    """``layout`` of the logits that a backward gets back, with labels and ``kept``,
+    of ``per_row`` numbers a row, dense.  It is that of the tensor given: what a
+    saved-tensor hook put elsewhere comes back as a copy with strides of its own."""
+    rows, n = layout(logits), labels.numel()
+    capi.require(0 <= logits.get_device() == labels.get_device() == kept.get_device() and
+                 rows[1] * rows[2] == n and kept.numel() == per_row * n,
+                 "autograd gave back other tensors than were saved")
+    return labels.contiguous(), kept.contiguous(), *rows
 
 
 def per_token(t, name, shape):

@@ -76,6 +76,7 @@ def recorded(monkeypatch):
         return 0
     monkeypatch.setattr(capi, "launch", launch)
     monkeypatch.setattr(token_rows, "check", lambda *a: None)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
     for op in (logp, policy, preference):
         monkeypatch.setattr(op, "_lib", _Library)
     for op in (policy, preference):
@@ -133,6 +134,29 @@ def test_backward_reads_the_saved_tensor_as_it_lies(name, layout, recorded):
     B, S, V, bs, rs = args[at:at + 5]
     assert (B - 1) * bs + (S - 1) * rs + V <= copy.numel()
     assert base.grad.shape == base.shape
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_other_tensors_than_were_saved_are_refused(name, recorded):
+    """A hook that returns another tensor, here one row short, is refused before a launch."""
+    for which in range(3):              # logits, labels, statistics
+        logits = torch.randn(4, 6, 7, requires_grad=True)
+        labels = torch.zeros(4, 6, dtype=torch.int64)
+        packed = []
+
+        def pack(t):
+            packed.append(t.detach())
+            return len(packed) - 1
+
+        def unpack(i):
+            t = packed[i]
+            return t[:-1] if i == which else t
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = _call(name, logits, labels)
+        del recorded[:]
+        with pytest.raises(RuntimeError, match="saved"):
+            out.backward()
+        assert not recorded
 
 
 @pytest.mark.gpu
