@@ -791,9 +791,9 @@ constexpr int kGramBlocks = 32;      // most workgroups that sum a Gram matrix
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-// U's columns j0 .. j0 + 63 (rows, where U is tall) into LDS, zeros past its edges.  The momentum
-// is updated on the way if `first` is set.
-// Row r, column c at tile[r][c], or tile[c][r].
+// Columns j0 .. j0 + 63 of U (of its transpose, where U is tall) into LDS, zeros past its edges:
+// row r of column j0 + c at tile[r][c], or at tile[c][r] if `kByColumn` is set.  The momentum is
+// updated on the way if `first` is.
 template <int KP, bool kByColumn, class Tile>
 __device__ __forceinline__ void load_block(const Source& s, int b, int j0, bool first,
                                            Tile& tile) {

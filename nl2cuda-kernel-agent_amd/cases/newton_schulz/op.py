@@ -20,7 +20,8 @@ KERNEL_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kernels")
 LIB_NAME = "newton_schulz_hip"
 SOURCES = ["newton_schulz.hip"]
 
-# p(s) = a s + b s^3 + c s^5: steep at 0, its fixed band around 1 wide
+# p(s) = a s + b s^3 + c s^5: steep at 0, its fixed band around 1 wide.  The coefficients published
+# with the Muon optimiser (K. Jordan and others, 2024)
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 PRECISIONS = {"half": 1, "full": 2}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -13,8 +13,9 @@
 //
 // x - m is formed before it is scaled: rows of a type's lowest value stay
 // finite (their softmax is uniform), and a common offset of the logits costs
-// no bits.  Maxima, sums and everything per token are held in 32 bits; only
-// dlogits is rounded, once, to the type of the logits.
+// no bits.  Maxima and sums are held in 32 bits, a log-probability in 64 until
+// it is stored or has had another taken from it, in 32 then; only dlogits is
+// rounded, once, to the type of the logits.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -343,12 +344,12 @@ __device__ __forceinline__ void zero_row(typename Elem<T>::type* __restrict__ d,
 }
 
 // What a row's statistics are turned into.  Ops of the kernels below have
-//   void begin()               what all rows need, read beside the row's label
-//   bool counts(r, label)     whether the row counts (read before the row is)
-//   float finish(r, col, logp, lead)   called by every thread with the row's
-//                             logp; the coefficient of its gradient.  The
-//                             thread with `lead` writes what is per token.
-//   void skip(r, lead)        for rows that do not count
+//   void begin(shape)               what all rows need, read beside the row's label
+//   bool counts(shape, r, label)    whether the row counts (read before the row is)
+//   float finish(shape, r, logp, lead)   called by every thread with the row's logp, in
+//                                   64 bits; the coefficient of its gradient.  The thread
+//                                   with `lead` writes what is per token.
+//   void skip(r, lead)              for rows that do not count
 
 // Forward: the statistics (m, S) of every row, for a backward, and the op's answers.  Bound by
 // memory: 50 us for 2432 rows of 50257 bfloat16, 109 for 3431 of float32 (4.9 and 6.3 TB/s).
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(
 
 // Loss terms and gradient in one pass: the row stays in registers, K windows a
 // thread, between its statistics and its gradient.  4096 rows of 128256 bfloat16:
-// 415 us, 5.1 TB/s; apart, the two passes read the logits twice.
+// 407 us a call, 5.2 TB/s; apart, the two passes read the logits twice.
 template <class T, int TPR, int K, Past kPast, class Op>
 __global__ __launch_bounds__(block_of<TPR>()) void fused_kernel(
     const typename Elem<T>::type* logits, const int64_t* __restrict__ labels,
