@@ -1,0 +1,58 @@
+/*
+ * libblock_matmul_hip.so -- matrix product in 8-bit floating point (e4m3) with
+ * a scale for each block of 128, for MI355X (gfx950).
+ *
+ *   out[m, n] = sum_b sa[m, b] sb[n, b] sum_{k in block b} a[m, k] b[n, k]
+ *
+ * a: M rows of K codes, b: N rows of K codes, `pitch` bytes between rows (a
+ * multiple of 16, at least K); the memory of the last row reaches up to the
+ * next multiple of 16 after K, and what lies from K on does not count.
+ * Blocks are 128 numbers of a row, or (tiles != 0) 128 rows by 128 columns;
+ * the scale of block b of row r (or of row of tiles r / 128) is at
+ * r * row_stride + b * block_stride, in scales.  scale_type 0: float32,
+ * 1: exponent + 127 in a byte (e8m0, 255 NaN), for both operands.
+ *
+ * out: M rows of N numbers of out_dtype (0 float32, 1 bfloat16, 2 float16),
+ * dense.  A block's sum and the sum over blocks are held in float32; the
+ * result is rounded once.  For 16-bit results a block's products are added by
+ * the 8-bit matrix instruction, which drops what lies 13 bits below the largest
+ * of each eight (1.5e-5 of a result's size where rounding costs 1.7e-3); for
+ * float32 results by the 16-bit one, at half its rate, which drops nothing.
+ * Products of two float32 scales are formed in float32.
+ *
+ * Device arrays owned by the caller; the library allocates nothing, keeps no
+ * state, never synchronises and launches on `stream`.  The workspace is
+ * scratch: calls that run at once need one each.  Arguments are validated
+ * before any HIP call (NL2K_* codes, message from block_matmul_last_error()).
+ * All results are bitwise repeatable for one set of sizes.
+ */
+#ifndef NL2K_BLOCK_MATMUL_H
+#define NL2K_BLOCK_MATMUL_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <hip/hip_runtime_api.h>
+
+#include "nl2k_status.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Bytes of scratch (0: none is needed, or the call refuses these sizes). */
+size_t block_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, int out_dtype);
+
+int block_matmul(const void* a, int64_t a_pitch, const void* a_scales, int64_t a_row_stride,
+                 int64_t a_block_stride, int a_tiles, const void* b, int64_t b_pitch,
+                 const void* b_scales, int64_t b_row_stride, int64_t b_block_stride, int b_tiles,
+                 int scale_type, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
+                 void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+const char* block_matmul_last_error(void);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* NL2K_BLOCK_MATMUL_H */

@@ -1,0 +1,209 @@
+"""Matrix product in 8-bit floating point with a scale for each block of 128
+numbers, and the trainable layer made of it: wrapper over the HIP library
+(kernels/block_matmul.hip).
+
+``block_matmul`` multiplies what ``quantize_rows``, ``quantize_tiles`` and
+``rms_norm_quantized`` give; ``block_linear`` is x weight^T with all three of
+its products in 8 bits, forward and backward.  There is no CPU path: without a
+GPU the library refuses to load.
+"""
+
+import collections
+import functools
+import os
+
+import torch
+
+from cases.block_quant.op import quantize_rows, quantize_tiles
+from framework import capi, e4m3
+from framework.loader import load_kernel
+from framework.once import differentiated, once
+
+KERNEL_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kernels")
+LIB_NAME = "block_matmul_hip"
+SOURCES = ["block_matmul.hip"]
+LONGEST = 1 << 22     # of the kernels' offsets within a tile
+
+QuantizedWeight = collections.namedtuple("QuantizedWeight", "codes scales codes_t scales_t")
+
+
+def bind_library(lib):
+    V, I64, I, S = capi.c_void_p, capi.c_int64, capi.c_int, capi.c_size_t
+    capi.bind(lib, "block_matmul_workspace_bytes", [I64, I64, I64, I], S)
+    capi.bind(lib, "block_matmul", [V, I64, V, I64, I64, I] * 2 + [I, V, I, I64, I64, I64, V, S, V])
+    capi.bind_last_error(lib, "block_matmul_last_error")
+    return lib
+
+
+@functools.lru_cache(maxsize=1)
+def _lib():
+    return bind_library(load_kernel(LIB_NAME, SOURCES, base_dir=KERNEL_DIR))
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(M, N, K, out_dtype):
+    return _lib().block_matmul_workspace_bytes(M, N, K, out_dtype)
+
+
+def _codes(c, rows, K):
+    """(codes, bytes between rows) as the kernels read them: rows 16 bytes apart or a multiple, the
+    last one's memory up to the next 16; copied only if they lie otherwise."""
+    pitch, whole = c.stride(0) if rows > 1 else e4m3.pitch(K), e4m3.pitch(K)
+    if ((K == 1 or c.stride(1) == 1) and pitch >= K and pitch % 16 == 0 and
+            pitch <= 2 * LONGEST and c.data_ptr() % 16 == 0 and
+            c.storage_offset() + (rows - 1) * pitch + whole <= c.untyped_storage().nbytes()):
+        return c, pitch
+    copy, pitch = e4m3.new_codes((rows,), K, c.device)
+    copy.view(torch.uint8).copy_(c.view(torch.uint8))
+    return copy, pitch
+
+
+def _scales(name, s, rows, K):
+    """(scales, row stride, block stride, whether they are of tiles)."""
+    n = e4m3.blocks(K)
+    capi.require(s.dim() == 2 and s.size(1) == n and s.size(0) in (rows, e4m3.blocks(rows)),
+                 f"{name}_scales must be [rows, {n}] or, of tiles, [{e4m3.blocks(rows)}, {n}], "
+                 f"got {tuple(s.shape)}")
+    if s.stride(0) > LONGEST:
+        s = s.contiguous()
+    return s, s.stride(0), s.stride(1), int(s.size(0) == e4m3.blocks(rows))
+
+
+def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
+    """a b^T for a [..., K] and b [N, K], codes with a scale for each block of 128:
+    [..., N] of out_dtype (float32, bfloat16 or float16); without a gradient.
+
+    Scales are of rows, [..., ceil(K / 128)], or of tiles of 128 x 128,
+    [ceil(rows / 128), ceil(K / 128)]; float32 or float8_e8m0fnu, the same for
+    both.  Codes in another layout than the quantisers' are copied.  Sums are
+    held in float32.  A 16-bit result is off by 1.5e-5 of its size before it is
+    rounded, which is what the 8-bit matrix instruction's additions cost; a
+    float32 one takes the 16-bit instruction, half as fast, and has its 24 bits.
+    """
+    tensors = (a, a_scales, b, b_scales)
+    capi.require(all(t.is_cuda for t in tensors), "codes and scales must be GPU tensors")
+    device = a.get_device()
+    capi.require(all(t.get_device() == device for t in tensors[1:]),
+                 "codes and scales must be on one GPU")
+    capi.require(a.dtype == b.dtype == e4m3.CODES, "a and b must be float8_e4m3fn")
+    capi.require(a_scales.dtype == b_scales.dtype and a_scales.dtype in e4m3.SCALES,
+                 "scales must both be float32 or both float8_e8m0fnu")
+    capi.require(out_dtype in e4m3.DTYPES, "out_dtype must be float32, bfloat16 or float16")
+    capi.require(a.dim() >= 1 and b.dim() == 2 and a.size(-1) == b.size(1) >= 1,
+                 "a must be [..., K] and b [N, K] with K >= 1")
+    capi.require(not differentiated(*tensors),
+                 "block_matmul has no gradient: use block_linear, or torch.no_grad()")
+    lib = _lib()
+    lead, K, N = a.shape[:-1], a.size(-1), b.size(0)
+    out = torch.empty((*lead, N), dtype=out_dtype, device=a.device)
+    M = out.numel() // N if N else 0
+    if M == 0:
+        return out
+    if a.dim() != 2:
+        capi.require(a_scales.shape == (*lead, e4m3.blocks(K)),
+                     f"a_scales must be {(*lead, e4m3.blocks(K))}, got {tuple(a_scales.shape)}")
+        a, a_scales = a.reshape(M, K), a_scales.reshape(M, -1)
+    a, a_pitch = _codes(a, M, K)
+    b, b_pitch = _codes(b, N, K)
+    a_scales, *a_how = _scales("a", a_scales, M, K)
+    b_scales, *b_how = _scales("b", b_scales, N, K)
+    ws_bytes = _workspace_bytes(M, N, K, e4m3.DTYPES[out_dtype])
+    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=a.device) if ws_bytes else None
+    st = capi.launch(lib.block_matmul, device, a.data_ptr(), a_pitch, a_scales.data_ptr(), *a_how,
+                     b.data_ptr(), b_pitch, b_scales.data_ptr(), *b_how,
+                     e4m3.SCALES[a_scales.dtype], out.data_ptr(), e4m3.DTYPES[out_dtype], M, N, K,
+                     ws.data_ptr() if ws_bytes else 0, ws_bytes)
+    if st:
+        capi.check(st, lib.block_matmul_last_error, "block_matmul")
+    return out
+
+
+def quantize_weight(weight, scale_dtype=torch.float8_e8m0fnu):
+    """What ``block_linear`` makes of a weight [N, K] in every call, for programs that
+    use it more than once between two updates."""
+    return QuantizedWeight(*quantize_tiles(weight, scale_dtype, transposed=True))
+
+
+class BlockLinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, quantized, scale_dtype):
+        want_x, want_w = ctx.needs_input_grad[:2]
+        rows = x.reshape(-1, x.size(-1))
+        if want_w:
+            codes, scales, codes_t, scales_t = quantize_rows(rows, scale_dtype, transposed=True)
+        else:
+            codes, scales, codes_t, scales_t = *quantize_rows(rows, scale_dtype), None, None
+        if quantized is None:
+            quantized = quantize_tiles(weight, scale_dtype, transposed=want_x)
+        y = block_matmul(codes, scales, quantized[0], quantized[1], x.dtype)
+        ctx.scale_dtype, ctx.dtypes, ctx.x_shape = scale_dtype, (x.dtype, weight.dtype), x.shape
+        ctx.w_shape = weight.shape
+        ctx.save_for_backward(codes_t, scales_t, *(quantized[2:] if want_x else (None, None)))
+        return y.view(*x.shape[:-1], weight.size(0))
+
+    @staticmethod
+    def backward(ctx, dy):
+        codes_t, scales_t, w_codes, w_scales = ctx.saved_tensors
+        N, K = ctx.w_shape
+        dy = dy.reshape(-1, N)
+        M = dy.size(0)
+        if codes_t is not None:
+            capi.require(codes_t.shape == (K, M), "autograd gave back other tensors than were saved")
+        if w_codes is not None:
+            capi.require(w_codes.shape == (K, N), "autograd gave back other tensors than were saved")
+        dx = dw = None
+        if codes_t is None:
+            codes, scales = quantize_rows(dy, ctx.scale_dtype)
+        else:
+            codes, scales, dy_t, dy_scales_t = quantize_rows(dy, ctx.scale_dtype, transposed=True)
+            if M:
+                dw = block_matmul(dy_t, dy_scales_t, codes_t, scales_t, ctx.dtypes[1])
+            else:
+                dw = torch.zeros(N, K, dtype=ctx.dtypes[1], device=dy.device)
+        if w_codes is not None:
+            dx = block_matmul(codes, scales, w_codes, w_scales, ctx.dtypes[0]).view(ctx.x_shape)
+        return *once("block_linear", dx, dw), None, None
+
+
+def block_linear(x, weight, quantized=None, scale_dtype=torch.float8_e8m0fnu):
+    """x weight^T, x [..., K] and weight [N, K] of float32, bfloat16 or float16, in 8
+    bits: [..., N] of x's type.
+
+        y  = Q(x) Q(weight)^T          blocks along K, tiles of the weight
+        dx = Q(dy) Q(weight)           blocks along N, the same tiles
+        dweight = Q(dy^T) Q(x^T)^T     blocks along the tokens
+
+    Gradients pass through the roundings Q as if they were not there; dx and
+    dweight come in x's and the weight's type.  Differentiable once and in
+    reverse.  quantized: what ``quantize_weight`` gave for this weight.
+    """
+    capi.require(x.is_cuda and weight.is_cuda and x.get_device() == weight.get_device(),
+                 "x and weight must be GPU tensors on one GPU")
+    capi.require(x.dtype in e4m3.DTYPES and weight.dtype in e4m3.DTYPES,
+                 "x and weight must be float32, bfloat16 or float16")
+    capi.require(x.dim() >= 1 and weight.dim() == 2 and x.size(-1) == weight.size(1) >= 1 and
+                 weight.size(0) >= 1, "x must be [..., K] and weight [N, K] with N, K >= 1")
+    e4m3.require_scales(scale_dtype)
+    if quantized is not None:
+        capi.require(quantized[0].shape == weight.shape and
+                     quantized[2].shape == weight.shape[::-1] and
+                     quantized[1].dtype == scale_dtype,
+                     "quantized must be quantize_weight's, of this weight and scale_dtype")
+    if differentiated(x, weight):
+        return BlockLinearFunction.apply(x, weight, quantized, scale_dtype)
+    codes, scales = quantize_rows(x, scale_dtype)
+    if quantized is None:
+        quantized = quantize_tiles(weight, scale_dtype)
+    return block_matmul(codes, scales, quantized[0], quantized[1], x.dtype)
+
+
+def candidate(inputs, params):
+    """Framework candidate contract: inputs={"X","W"} -> X W^T in 8 bits."""
+    return block_linear(inputs["X"], inputs["W"],
+                        scale_dtype=params.get("scale_dtype", torch.float8_e8m0fnu))
+
+
+def forward_only(inputs, params):
+    """Forward without autograd."""
+    with torch.no_grad():
+        return candidate(inputs, params)

@@ -19,11 +19,13 @@
 #include <cmath>
 
 #include "common.h"
+#include "lds_direct.h"
 
 namespace {
 
 using nl2k::f32x4;
 using nl2k::u32x4;
+using namespace nl2k::lds;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half_t;
@@ -449,57 +451,6 @@ struct LastStore {
     emit(b, j, i, j < l ? k - i : 0, v);
   }
 };
-
-// An address that is the same in all lanes, in scalar registers, five issues after whatever
-// wrote them.
-__device__ __forceinline__ const half_t* scalar_base(const half_t* base) {
-  const uint64_t p = reinterpret_cast<uint64_t>(base);
-  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p);
-  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));
-  uint64_t q = hi << 32 | lo;
-  asm volatile("s_nop 4" : "+s"(q));
-  return reinterpret_cast<const half_t*>(q);
-}
-
-// 16 bytes a lane from global memory straight to LDS: lane n's land at lds + 16 n.
-// The count of outstanding loads is waited for by hand (wait_tile): the
-// compiler, which does not know which part of LDS a load writes, would have
-// every read of LDS wait for all of them.  M0 holds the place in LDS.  A scalar
-// register that a vector instruction wrote must not be read by a load within five
-// issues, which the compiler does not see to here: `base` comes from
-// scalar_base and is moved on by scalar additions alone.
-__device__ __forceinline__ void load_lds16(const half_t* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
-}
-
-// Waits until at most N of this wave's loads are outstanding.
-template <int N>
-__device__ __forceinline__ void wait_tile() {
-  static_assert(N < 64, "the counter has six bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0xf70);
-}
-
-// Waits until none of its LDS reads are.
-__device__ __forceinline__ void wait_reads() { __builtin_amdgcn_s_waitcnt(0xc07f); }
-
-// The barrier alone: what it waits for, wait_tile has waited for.  The compiler may move no
-// access across it.
-__device__ __forceinline__ void workgroup_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// Between what the lanes of a wave write to its part of LDS and read there: LDS keeps a wave's
-// accesses in order, so the compiler has to keep them too.
-__device__ __forceinline__ void wave_order() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  asm volatile("" ::: "memory");
-}
 
 // T x T tiles of WM x WN waves, kB x kB matrix products, S stages of 128 bytes a row in LDS.
 // Bound by LDS, written at 64 and read at 128 bytes a clock: a stage of one tile on an idle chip

@@ -1,0 +1,565 @@
+// Root-mean-square norm with the residual's addition, for MI355X (gfx950).
+// C-ABI in include/rms_norm.h.
+//
+// A lane holds windows of eight numbers of a row, so that 16 lanes next to each
+// other hold a block of 128; a wave, a workgroup of 256 or one of 1024 takes a
+// row, which stays in registers from its sum of squares to its result.
+
+#include "rms_norm.h"
+
+#include "e4m3.h"
+
+namespace {
+
+using namespace nl2k::e4m3;
+
+struct Forward {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* y;        // numbers, or codes
+  void* scales;
+  void* h;
+  float* rstd;
+  int64_t x_stride, r_stride, pitch;
+  int32_t rows, D;
+  int w_dtype, scale_type;
+  float eps;
+};
+
+// Eight weights.
+__device__ __forceinline__ void weights8(const void* w, int dtype, int at, int count,
+                                         float (&v)[8]) {
+  if (dtype == kF32)
+    values<float>(load8<float>(static_cast<const float*>(w) + at, count), v);
+  else if (dtype == kBF16)
+    values<bf16_t>(load8<bf16_t>(static_cast<const unsigned short*>(w) + at, count), v);
+  else
+    values<f16_t>(load8<f16_t>(static_cast<const unsigned short*>(w) + at, count), v);
+}
+
+// The sum over all TPR threads of a row; red has TPR / 64 floats.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = nl2k::wave_sum_dpp(v);
+  if constexpr (TPR > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; ++i) v += red[i];
+  }
+  return v;
+}
+
+template <int TPR>
+constexpr int block_of() {
+  return TPR < 256 ? 256 : TPR;
+}
+
+template <int TPR>
+__device__ __forceinline__ int row_in(int block) {
+  return TPR == 64 ? block * 4 + (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : block;
+}
+
+template <int TPR>
+__device__ __forceinline__ int lane_in() {
+  return TPR == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+}
+
+// h of a window: what is stored, widened again.
+template <class T, class R, bool kRes>
+__device__ __forceinline__ void sum8(const Raw<T>& x, const Raw<R>& r, float (&h)[8]) {
+  values<T>(x, h);
+  if constexpr (kRes) {
+    float v[8];
+    values<R>(r, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = widen<R>(narrow<R>(h[e] + v[e]));
+  }
+}
+
+// y of a window at column k, from its h.
+template <class T, bool kCodes>
+__device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, float rstd,
+                                        float (&v)[8], const float (&w)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = v[e] * rstd * w[e];
+  if constexpr (kCodes) {
+    const float top = nl2k::row16_max_dpp(magnitude(v));
+    const Scale s =
+        f.scale_type == kScaleF32 ? scale_of<kScaleF32>(top) : scale_of<kScaleE8M0>(top);
+    if (k < (f.D + 15) / 16 * 16)
+      *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(f.y) + row * f.pitch + k) =
+          pack8(v, s.inverse);
+    if ((threadIdx.x & 15) == 0 && k < f.D) {
+      const int64_t at = (int64_t)(k / kBlock) * f.rows + row;
+      if (f.scale_type == kScaleF32)
+        keep<kScaleF32>(f.scales, at, s.kept);
+      else
+        keep<kScaleE8M0>(f.scales, at, s.kept);
+    }
+  } else {
+    store8<T>(static_cast<typename Elem<T>::type*>(f.y) + row * f.D + k, f.D - k, v);
+  }
+}
+
+template <class T, class R, bool kRes, bool kCodes, int TPR, int U>
+__global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(Forward f) {
+  __shared__ float red[TPR / 64];
+  const int64_t row = row_in<TPR>(blockIdx.x);
+  if (row >= f.rows) return;
+  const int lane = lane_in<TPR>();
+  const auto* x = static_cast<const typename Elem<T>::type*>(f.x) + row * f.x_stride;
+  const auto* res = static_cast<const typename Elem<R>::type*>(f.residual) + row * f.r_stride;
+  Raw<T> xr[U];
+  Raw<R> rr[kRes ? U : 1];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = (u * TPR + lane) * 8;
+    xr[u] = load8<T>(x + k, f.D - k);
+    if constexpr (kRes) rr[u] = load8<R>(res + k, f.D - k);
+  }
+  float w[U][8];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = (u * TPR + lane) * 8;
+    weights8(f.weight, f.w_dtype, k, f.D - k, w[u]);
+  }
+  float h[U][8], sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = (u * TPR + lane) * 8;
+    sum8<T, R, kRes>(xr[u], rr[kRes ? u : 0], h[u]);
+    if constexpr (kRes)
+      store8<R>(static_cast<typename Elem<R>::type*>(f.h) + row * f.D + k, f.D - k, h[u]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(h[u][e], h[u][e], sum);
+  }
+  const float rstd = 1.f / sqrtf(row_sum<TPR>(sum, red) / (float)f.D + f.eps);
+  if (f.rstd && lane == 0) f.rstd[row] = rstd;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    finish8<T, kCodes>(f, row, (u * TPR + lane) * 8, rstd, h[u], w[u]);
+}
+
+// Rows that registers do not hold: read again for the result.
+template <class T, class R, bool kRes, bool kCodes>
+__global__ __launch_bounds__(1024) void forward_long_kernel(Forward f) {
+  __shared__ float red[16];
+  const int64_t row = blockIdx.x;
+  const auto* x = static_cast<const typename Elem<T>::type*>(f.x) + row * f.x_stride;
+  const auto* res = static_cast<const typename Elem<R>::type*>(f.residual) + row * f.r_stride;
+  auto* hs = static_cast<typename Elem<R>::type*>(f.h) + row * f.D;
+  auto load = [&](int k, float(&h)[8]) {
+    const Raw<T> xr = load8<T>(x + k, f.D - k);
+    Raw<R> rr{};
+    if constexpr (kRes) rr = load8<R>(res + k, f.D - k);
+    sum8<T, R, kRes>(xr, rr, h);
+  };
+  float sum = 0.f;
+  for (int64_t c = threadIdx.x * 8; c < f.D; c += 8192) {
+    const int k = (int)c;
+    float h[8];
+    load(k, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(h[e], h[e], sum);
+  }
+  const float rstd = 1.f / sqrtf(row_sum<1024>(sum, red) / (float)f.D + f.eps);
+  if (f.rstd && threadIdx.x == 0) f.rstd[row] = rstd;
+  // whole waves: the lanes of a block take their maximum together
+  for (int64_t c = threadIdx.x * 8; c - threadIdx.x * 8 < f.D; c += 8192) {
+    const int k = (int)min(c, (int64_t)INT32_MAX);
+    float h[8], w[8];
+    load(k, h);
+    weights8(f.weight, f.w_dtype, k, f.D - k, w);
+    if constexpr (kRes) store8<R>(hs + k, f.D - k, h);
+    finish8<T, kCodes>(f, row, k, rstd, h, w);
+  }
+}
+
+struct Backward {
+  const void* dy;
+  const void* h;
+  const void* dh;
+  const void* weight;
+  const float* rstd;
+  void* dx;
+  void* dres;
+  float* partial;  // [workgroups][D], null without a gradient of the weight
+  int64_t dy_stride, h_stride, dh_stride;
+  int32_t rows, D;
+  int w_dtype;
+};
+
+// dx of a window, stored; u = h r in place of h, d = dy.
+template <class T, class R>
+__device__ __forceinline__ void gradient8(const Backward& b, int64_t row, int k, float rstd,
+                                          float mean, const float (&u)[8], const float (&d)[8],
+                                          const float (&w)[8], const Raw<R>& dh) {
+  float v[8], add[8];
+  values<R>(dh, add);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = fmaf(rstd, d[e] * w[e] - u[e] * mean, add[e]);
+  if (b.dx) store8<T>(static_cast<typename Elem<T>::type*>(b.dx) + row * b.D + k, b.D - k, v);
+  if (b.dres) store8<R>(static_cast<typename Elem<R>::type*>(b.dres) + row * b.D + k, b.D - k, v);
+}
+
+// A workgroup takes every gridDim.x-th row (or four), and adds up their share of dweight.
+template <class T, class R, int TPR, int U>
+__global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(Backward b) {
+  constexpr int kRows = block_of<TPR>() / TPR;
+  __shared__ float red[TPR / 64];
+  __shared__ float shared_dw[kRows > 1 ? TPR * U * 8 : 1];
+  const int lane = lane_in<TPR>();
+  float w[U][8], dw[U][8];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = (u * TPR + lane) * 8;
+    weights8(b.weight, b.w_dtype, k, b.D - k, w[u]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[u][e] = 0.f;
+  }
+  for (int64_t row = row_in<TPR>(blockIdx.x); row < b.rows; row += (int64_t)gridDim.x * kRows) {
+    const auto* dy = static_cast<const typename Elem<T>::type*>(b.dy) + row * b.dy_stride;
+    const auto* h = static_cast<const typename Elem<R>::type*>(b.h) + row * b.h_stride;
+    const auto* dh = static_cast<const typename Elem<R>::type*>(b.dh) + row * b.dh_stride;
+    Raw<T> dr[U];
+    Raw<R> hr[U], ar[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (u * TPR + lane) * 8;
+      dr[u] = load8<T>(dy + k, b.D - k);
+      hr[u] = load8<R>(h + k, b.D - k);
+      ar[u] = load8<R>(dh + k, b.dh ? b.D - k : 0);
+    }
+    const float rstd = b.rstd[row];
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float d[8], v[8];
+      values<T>(dr[u], d);
+      values<R>(hr[u], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] *= rstd;
+        sum = fmaf(d[e] * w[u][e], v[e], sum);
+        dw[u][e] = fmaf(d[e], v[e], dw[u][e]);
+      }
+    }
+    const float mean = row_sum<TPR>(sum, red) / (float)b.D;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float d[8], v[8];
+      values<T>(dr[u], d);
+      values<R>(hr[u], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= rstd;
+      gradient8<T, R>(b, row, (u * TPR + lane) * 8, rstd, mean, v, d, w[u], ar[u]);
+    }
+  }
+  if (!b.partial) return;
+  if constexpr (kRows > 1) {  // the waves' sums, added in their order
+    for (int i = 0; i < kRows; ++i) {
+      if (i) __syncthreads();
+      if ((int)(threadIdx.x >> 6) != i) continue;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float* at = shared_dw + (u * 8 + e) * 64 + lane;
+          dw[u][e] += i ? *at : 0.f;
+          *at = dw[u][e];
+        }
+    }
+    if ((int)(threadIdx.x >> 6) != kRows - 1) return;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int k = (u * TPR + lane) * 8;
+    store8<float>(b.partial + (int64_t)blockIdx.x * b.D + k, b.D - k, dw[u]);
+  }
+}
+
+template <class T, class R>
+__global__ __launch_bounds__(1024) void backward_long_kernel(Backward b) {
+  __shared__ float red[16];
+  float* mine = b.partial ? b.partial + (int64_t)blockIdx.x * b.D : nullptr;
+  bool first = true;
+  for (int64_t row = blockIdx.x; row < b.rows; row += gridDim.x) {
+    const auto* dy = static_cast<const typename Elem<T>::type*>(b.dy) + row * b.dy_stride;
+    const auto* h = static_cast<const typename Elem<R>::type*>(b.h) + row * b.h_stride;
+    const auto* dh = static_cast<const typename Elem<R>::type*>(b.dh) + row * b.dh_stride;
+    const float rstd = b.rstd[row];
+    float sum = 0.f;
+    for (int64_t c = threadIdx.x * 8; c < b.D; c += 8192) {
+      const int k = (int)c;
+      float d[8], v[8], w[8];
+      values<T>(load8<T>(dy + k, b.D - k), d);
+      values<R>(load8<R>(h + k, b.D - k), v);
+      weights8(b.weight, b.w_dtype, k, b.D - k, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(d[e] * w[e], v[e] * rstd, sum);
+    }
+    const float mean = row_sum<1024>(sum, red) / (float)b.D;
+    for (int64_t c = threadIdx.x * 8; c < b.D; c += 8192) {
+      const int k = (int)c;
+      float d[8], v[8], w[8];
+      values<T>(load8<T>(dy + k, b.D - k), d);
+      values<R>(load8<R>(h + k, b.D - k), v);
+      weights8(b.weight, b.w_dtype, k, b.D - k, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= rstd;
+      if (mine) {  // this thread's columns alone
+        float p[8];
+        values<float>(load8<float>(mine + k, first ? 0 : b.D - k), p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = fmaf(d[e], v[e], p[e]);
+        store8<float>(mine + k, b.D - k, p);
+      }
+      gradient8<T, R>(b, row, k, rstd, mean, v, d, w, load8<R>(dh + k, b.dh ? b.D - k : 0));
+    }
+    first = false;
+  }
+}
+
+// dweight: the workgroups' sums, 16 columns a workgroup, 16 threads a column.
+__global__ __launch_bounds__(256) void columns_kernel(const float* __restrict__ partial, int count,
+                                                      int D, void* dw, int w_dtype) {
+  __shared__ float part[16][17];
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  float sum = 0.f;
+  if (col < D) {
+#pragma unroll 8
+    for (int i = g; i < count; i += 16) sum += partial[(int64_t)i * D + col];
+  }
+  part[g][c] = sum;
+  __syncthreads();
+  if (g == 0 && col < D) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += part[i][c];
+    if (w_dtype == kF32)
+      static_cast<float*>(dw)[col] = s;
+    else
+      static_cast<unsigned short*>(dw)[col] =
+          w_dtype == kBF16 ? narrow<bf16_t>(s) : narrow<f16_t>(s);
+  }
+}
+
+// Threads a row and windows a thread for a row of D numbers.
+struct Plan {
+  int tpr, u;
+};
+
+Plan plan(int64_t D) {
+  const int64_t n = nl2k::ceil_div(D, 8);
+  if (n <= 64) return {64, 1};
+  if (n <= 128) return {64, 2};
+  if (n <= 256) return {256, 1};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {256, 4};
+  if (n <= 2048) return {1024, 2};
+  if (n <= 4096) return {1024, 4};
+  return {0, 0};
+}
+
+// Workgroups of a backward.
+int64_t backward_blocks(int64_t rows, int64_t D) {
+  const Plan p = plan(D);
+  const int64_t most = p.tpr == 1024 || p.tpr == 0 ? 256 : 512;
+  return std::min(p.tpr == 64 ? nl2k::ceil_div(rows, 4) : rows, most);
+}
+
+template <class F>
+int with_types(int dtype, int r_dtype, F&& f) {
+  if (dtype == kF32) return f(float{}, float{});
+  if (dtype == kBF16) return r_dtype == kF32 ? f(bf16_t{}, float{}) : f(bf16_t{}, bf16_t{});
+  return r_dtype == kF32 ? f(f16_t{}, float{}) : f(f16_t{}, f16_t{});
+}
+
+template <class T, class R, bool kRes, bool kCodes>
+int launch_forward(const Forward& f, hipStream_t s) {
+  const Plan p = plan(f.D);
+  const dim3 grid(p.tpr == 64 ? (uint32_t)nl2k::ceil_div(f.rows, 4) : (uint32_t)f.rows);
+  auto is = [&](int t, int u) { return p.tpr == t && p.u == u; };
+  if (is(64, 1))
+    forward_kernel<T, R, kRes, kCodes, 64, 1><<<grid, 256, 0, s>>>(f);
+  else if (is(64, 2))
+    forward_kernel<T, R, kRes, kCodes, 64, 2><<<grid, 256, 0, s>>>(f);
+  else if (is(256, 1))
+    forward_kernel<T, R, kRes, kCodes, 256, 1><<<grid, 256, 0, s>>>(f);
+  else if (is(256, 2))
+    forward_kernel<T, R, kRes, kCodes, 256, 2><<<grid, 256, 0, s>>>(f);
+  else if (is(256, 4))
+    forward_kernel<T, R, kRes, kCodes, 256, 4><<<grid, 256, 0, s>>>(f);
+  else if (is(1024, 2))
+    forward_kernel<T, R, kRes, kCodes, 1024, 2><<<grid, 1024, 0, s>>>(f);
+  else if (is(1024, 4))
+    forward_kernel<T, R, kRes, kCodes, 1024, 4><<<grid, 1024, 0, s>>>(f);
+  else
+    forward_long_kernel<T, R, kRes, kCodes><<<grid, 1024, 0, s>>>(f);
+  return nl2k::check_launch("rms_norm");
+}
+
+template <class T, class R>
+int launch_backward(const Backward& b, hipStream_t s) {
+  const Plan p = plan(b.D);
+  const dim3 grid((uint32_t)backward_blocks(b.rows, b.D));
+  auto is = [&](int t, int u) { return p.tpr == t && p.u == u; };
+  if (is(64, 1))
+    backward_kernel<T, R, 64, 1><<<grid, 256, 0, s>>>(b);
+  else if (is(64, 2))
+    backward_kernel<T, R, 64, 2><<<grid, 256, 0, s>>>(b);
+  else if (is(256, 1))
+    backward_kernel<T, R, 256, 1><<<grid, 256, 0, s>>>(b);
+  else if (is(256, 2))
+    backward_kernel<T, R, 256, 2><<<grid, 256, 0, s>>>(b);
+  else if (is(256, 4))
+    backward_kernel<T, R, 256, 4><<<grid, 256, 0, s>>>(b);
+  else if (is(1024, 2))
+    backward_kernel<T, R, 1024, 2><<<grid, 1024, 0, s>>>(b);
+  else
+    backward_long_kernel<T, R><<<grid, 1024, 0, s>>>(b);
+  return nl2k::check_launch("rms_norm_backward");
+}
+
+// Sizes and types that all entries share.
+int check_sizes(const char* who, int64_t rows, int64_t D, int dtype, int r_dtype, int w_dtype) {
+  if (rows < 0 || D < 1)
+    return nl2k::fail(NL2K_ERR_SHAPE, "%s: need rows >= 0 and D >= 1 (got %lld, %lld)", who,
+                      (long long)rows, (long long)D);
+  if (D > INT32_MAX - 16384 || rows > nl2k::max_blocks(1024) || (rows && D > INT64_MAX / 8 / rows))
+    return nl2k::fail(NL2K_ERR_OVERFLOW, "%s: sizes too large (rows=%lld D=%lld)", who,
+                      (long long)rows, (long long)D);
+  if (dtype < kF32 || dtype > kF16 || w_dtype < kF32 || w_dtype > kF16 ||
+      (r_dtype != dtype && r_dtype != kF32))
+    return nl2k::fail(NL2K_ERR_VALUE,
+                      "%s: types must be 0, 1 or 2, the residual's that of x or 0 (got %d, %d, %d)",
+                      who, dtype, r_dtype, w_dtype);
+  return NL2K_SUCCESS;
+}
+
+int check_rows(const char* who, const char* name, const void* p, int dtype, int64_t stride,
+               int64_t rows) {
+  if (reinterpret_cast<uintptr_t>(p) % bytes_of(dtype))
+    return nl2k::fail(NL2K_ERR_ALIGN, "%s: %s must be aligned to its type", who, name);
+  if (stride < 0 || (rows > 1 && stride > INT64_MAX / 8 / rows))
+    return nl2k::fail(NL2K_ERR_SHAPE, "%s: the stride of %s is negative or too large (%lld)", who,
+                      name, (long long)stride);
+  return NL2K_SUCCESS;
+}
+
+int forward(const char* who, Forward f, int dtype, int r_dtype, bool codes, int64_t rows,
+            int64_t D, hipStream_t stream) {
+  int st = check_sizes(who, rows, D, dtype, f.residual ? r_dtype : dtype, f.w_dtype);
+  if (st) return st;
+  if (!(f.eps > 0.f && f.eps <= 3.4e38f))
+    return nl2k::fail(NL2K_ERR_VALUE, "%s: eps must be positive and finite", who);
+  if (codes && f.scale_type != kScaleF32 && f.scale_type != kScaleE8M0)
+    return nl2k::fail(NL2K_ERR_VALUE, "%s: scale_type must be 0 or 1 (got %d)", who, f.scale_type);
+  if (rows == 0) return nl2k::succeed();
+  if (!f.x || !f.weight || !f.y || (codes && !f.scales) || !f.residual != !f.h)
+    return nl2k::fail(NL2K_ERR_NULL,
+                      "%s: x, weight and the output are required, residual and h together", who);
+  if ((st = check_rows(who, "x", f.x, dtype, f.x_stride, rows))) return st;
+  if ((st = check_rows(who, "residual", f.residual, r_dtype, f.r_stride, rows))) return st;
+  if ((st = check_rows(who, "h", f.h, r_dtype, 0, rows))) return st;
+  if ((st = check_rows(who, "weight", f.weight, f.w_dtype, 0, rows))) return st;
+  if ((st = check_rows(who, "rstd", f.rstd, kF32, 0, rows))) return st;
+  if (codes) {
+    if (f.pitch < D || f.pitch % 16 || f.pitch > INT64_MAX / 8 / rows)
+      return nl2k::fail(NL2K_ERR_SHAPE, "%s: the pitch of codes must be >= D, a multiple of 16",
+                        who);
+    if (!nl2k::aligned16(f.y) ||
+        reinterpret_cast<uintptr_t>(f.scales) % scale_bytes(f.scale_type))
+      return nl2k::fail(NL2K_ERR_ALIGN, "%s: codes must be aligned to 16 bytes, scales to their type",
+                        who);
+  } else if ((st = check_rows(who, "y", f.y, dtype, 0, rows))) {
+    return st;
+  }
+  f.rows = (int32_t)rows;
+  f.D = (int32_t)D;
+  return with_types(dtype, f.residual ? r_dtype : dtype, [&](auto t, auto r) {
+    using T = decltype(t);
+    using R = decltype(r);
+    if (f.residual)
+      return codes ? launch_forward<T, R, true, true>(f, stream)
+                   : launch_forward<T, R, true, false>(f, stream);
+    if constexpr (__is_same(T, R))
+      return codes ? launch_forward<T, T, false, true>(f, stream)
+                   : launch_forward<T, T, false, false>(f, stream);
+    return nl2k::succeed();  // not reached: without a residual the types agree
+  });
+}
+
+}  // namespace
+
+extern "C" int rms_norm_forward(const void* x, int dtype, int64_t x_stride, const void* residual,
+                                int residual_dtype, int64_t residual_stride, const void* weight,
+                                int weight_dtype, void* y, void* h, float* rstd, int64_t rows,
+                                int64_t D, float eps, hipStream_t stream) {
+  const Forward f{x,  residual, weight,          y, nullptr, h, rstd, x_stride, residual_stride,
+                  0,  0,        0, weight_dtype, 0, eps};
+  return forward("rms_norm_forward", f, dtype, residual_dtype, false, rows, D, stream);
+}
+
+extern "C" int rms_norm_quant(const void* x, int dtype, int64_t x_stride, const void* residual,
+                              int residual_dtype, int64_t residual_stride, const void* weight,
+                              int weight_dtype, void* codes, int64_t pitch, void* scales,
+                              int scale_type, void* h, int64_t rows, int64_t D, float eps,
+                              hipStream_t stream) {
+  const Forward f{x,     residual, weight, codes, scales, h, nullptr, x_stride, residual_stride,
+                  pitch, 0,        0,      weight_dtype, scale_type, eps};
+  return forward("rms_norm_quant", f, dtype, residual_dtype, true, rows, D, stream);
+}
+
+extern "C" size_t rms_norm_backward_workspace_bytes(int64_t rows, int64_t D) {
+  if (check_sizes("rms_norm_backward_workspace_bytes", rows, D, kF32, kF32, kF32)) return 0;
+  return (size_t)backward_blocks(rows, D) * D * 4;
+}
+
+extern "C" int rms_norm_backward(const void* dy, int dtype, int64_t dy_stride, const void* h,
+                                 int h_dtype, int64_t h_stride, const void* dh, int64_t dh_stride,
+                                 const void* weight, int weight_dtype, const float* rstd, void* dx,
+                                 void* dresidual, void* dweight, int64_t rows, int64_t D,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  const char* who = "rms_norm_backward";
+  int st = check_sizes(who, rows, D, dtype, h_dtype, weight_dtype);
+  if (st) return st;
+  if (rows && (!dy || !h || !weight || !rstd))
+    return nl2k::fail(NL2K_ERR_NULL, "%s: dy, h, weight and rstd are required", who);
+  if ((st = check_rows(who, "dy", dy, dtype, dy_stride, rows))) return st;
+  if ((st = check_rows(who, "h", h, h_dtype, h_stride, rows))) return st;
+  if ((st = check_rows(who, "dh", dh, h_dtype, dh_stride, rows))) return st;
+  if ((st = check_rows(who, "weight", weight, weight_dtype, 0, rows))) return st;
+  if ((st = check_rows(who, "rstd", rstd, kF32, 0, rows))) return st;
+  if ((st = check_rows(who, "dx", dx, dtype, 0, rows))) return st;
+  if ((st = check_rows(who, "dresidual", dresidual, h_dtype, 0, rows))) return st;
+  if ((st = check_rows(who, "dweight", dweight, weight_dtype, 0, rows))) return st;
+  const size_t need = dweight ? (size_t)backward_blocks(rows, D) * D * 4 : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return nl2k::fail(NL2K_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes (got %zu)", who, need,
+                      workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 4)
+    return nl2k::fail(NL2K_ERR_ALIGN, "%s: the workspace must be aligned to 4 bytes", who);
+  const Backward b{dy, h, dh, weight, rstd, dx, dresidual,
+                   dweight ? static_cast<float*>(workspace) : nullptr, dy_stride, h_stride,
+                   dh_stride, (int32_t)rows, (int32_t)D, weight_dtype};
+  if (rows) {
+    st = with_types(dtype, h_dtype, [&](auto t, auto r) {
+      return launch_backward<decltype(t), decltype(r)>(b, stream);
+    });
+    if (st) return st;
+  }
+  if (dweight) {
+    columns_kernel<<<dim3((uint32_t)nl2k::ceil_div(D, 16)), 256, 0, stream>>>(
+        b.partial, rows ? (int)backward_blocks(rows, D) : 0, (int)D, dweight, weight_dtype);
+    return nl2k::check_launch(who);
+  }
+  return nl2k::succeed();
+}
+
+extern "C" const char* rms_norm_last_error(void) { return nl2k::error_slot().text; }
