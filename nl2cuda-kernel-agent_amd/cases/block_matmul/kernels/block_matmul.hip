@@ -2,7 +2,9 @@
 // (gfx950).  C-ABI in include/block_matmul.h.
 //
 // The matrix instruction takes 16 rows of each operand and 128 numbers of k, a
-// block: 32 a lane, lane l rows l % 16, k from 32 (l / 16) on.  b's rows are its
+// block: 32 a lane, lane l of row l % 16; which 32 does not matter, so long as both
+// operands' lanes hold the same: the 16 from 16 (l / 16) on and those from 64 on
+// after them, so that four lanes read 64 bytes of a row.  b's rows are its
 // first operand and a's its second, so that a lane's sums are of one row of a
 // and of numbers next to each other in a row of the result.
 //
@@ -50,8 +52,8 @@ struct Args {
   Side a, b;
   void* out;
   float* partial;  // sums of parts of k, [splits][M][N], or null
-  int32_t K, steps;
-  int32_t per;     // steps of a part
+  int32_t K, steps;  // numbers of a row, and its blocks
+  int32_t per;     // blocks of k of a part
   int32_t tiles_a, tiles_b, tiles;
   int out_dtype;
 };
@@ -60,7 +62,7 @@ struct Args {
 __device__ __forceinline__ void cut(i32x8& f, int valid, int group) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int n = valid - 32 * group - 4 * i;
+    const int n = valid - (i < 4 ? 0 : 64) - 16 * group - 4 * (i & 3);
     f[i] &= n >= 4 ? ~0 : (n <= 0 ? 0 : (1 << (8 * n)) - 1);
   }
 }
@@ -105,41 +107,55 @@ __device__ __forceinline__ Operand<kFull> operand(const i32x8& f) {
   return o;
 }
 
-// Scales as the sums are multiplied by them: an exponent as its power of two.
-template <Mode kMode>
-__device__ __forceinline__ float factor(uint32_t kept) {
-  if constexpr (kMode != kHardware) return __builtin_bit_cast(float, kept);
-  return kept == 255 ? NAN : __builtin_bit_cast(float, kept ? kept << 23 : 0x00400000u);
+// Whether scales are applied to a block's sums, and how many of b's a lane then needs for its four:
+// one, or four; the instruction takes that of the lane's row.
+template <Mode kMode, bool kFull>
+constexpr bool applied_later() {
+  return kMode != kHardware || kFull;
+}
+template <Mode kMode, bool kFull>
+constexpr int scales_of_b() {
+  return kMode == kTiles || !applied_later<kMode, kFull>() ? 1 : 4;
 }
 
-// A block's products added to c.
+// A scale as it is read, for the instruction or as the bits of what sums are multiplied by.
+template <Mode kMode, bool kFull>
+__device__ __forceinline__ uint32_t ready(uint32_t kept) {
+  if constexpr (kMode != kHardware || !kFull) return kept;
+  return kept == 255 ? 0x7fc00000u : (kept ? kept << 23 : 0x00400000u);
+}
+__device__ __forceinline__ float as_float(uint32_t bits) {
+  return __builtin_bit_cast(float, bits);
+}
+
+// A block's products, without scales.
+template <bool kFull>
+__device__ __forceinline__ f32x4 sums(const Operand<kFull>& b, const Operand<kFull>& a) {
+  f32x4 v = nl2k::zero4();
+  if constexpr (kFull) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.f[i], a.f[i], v, 0, 0, 0);
+  } else {
+    v = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.f, a.f, v, 0, 0, 0, 0, 0, 0);
+  }
+  return v;
+}
+
+// A block's products, scaled and added to c.
 template <Mode kMode, bool kFull>
 __device__ __forceinline__ f32x4 block(const Operand<kFull>& b, const Operand<kFull>& a, f32x4 c,
                                        const uint32_t* sb, uint32_t sa) {
-  if constexpr (kMode == kHardware && !kFull) {
+  if constexpr (!applied_later<kMode, kFull>()) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.f, a.f, c, 0, 0, 0, (int)sb[0], 0,
                                                             (int)sa);
   } else {
-    f32x4 v = nl2k::zero4();
-    if constexpr (kFull) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.f[i], a.f[i], v, 0, 0, 0);
-    } else {
-      v = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.f, a.f, v, 0, 0, 0, 0, 0, 0);
-    }
+    const f32x4 v = sums<kFull>(b, a);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      c[r] = fmaf(factor<kMode>(sa) * factor<kMode>(sb[kMode == kTiles ? 0 : r]), v[r], c[r]);
+      c[r] = fmaf(as_float(sa) * as_float(sb[kMode == kTiles ? 0 : r]), v[r], c[r]);
     return c;
   }
-}
-
-// Scales of b that a lane needs for its sums: its row's, for the instruction; one for all four; or
-// four.
-template <Mode kMode, bool kFull>
-constexpr int scales_of_b() {
-  return kMode == kTiles || (kMode == kHardware && !kFull) ? 1 : 4;
 }
 
 // `count` of eight numbers of a row of the result.
@@ -153,18 +169,66 @@ __device__ __forceinline__ void put8(const Args& g, int64_t at, int count, const
     store8<f16_t>(static_cast<unsigned short*>(g.out) + at, count, v);
 }
 
-// BM rows of a by BN of b, WM x WN waves, two stages of 128 bytes a row in LDS.
-template <int BM, int BN, int WM, int WN, Mode kMode, bool kFull>
+// One sum.
+__device__ __forceinline__ void put1(const Args& g, int part, int64_t row, int64_t col, float v) {
+  const int64_t at = row * g.b.rows + col;
+  if (g.partial)
+    g.partial[(int64_t)part * g.a.rows * g.b.rows + at] = v;
+  else if (g.out_dtype == kF32)
+    static_cast<float*>(g.out)[at] = v;
+  else
+    static_cast<unsigned short*>(g.out)[at] =
+        g.out_dtype == kBF16 ? narrow<bf16_t>(v) : narrow<f16_t>(v);
+}
+
+// The pieces of 16 bytes of a row in LDS are permuted by the row's number, so that the 64 banks
+// give a wave its 1024 bytes in four clocks: lanes read pieces `group` and `group` + 4 of 16 rows
+// (pieces 2 group and 2 group + 1 took eight).
+__device__ __forceinline__ i32x8 read_row(const uint8_t* row, int group, int key) {
+  const u32x4 lo = *reinterpret_cast<const u32x4*>(row + (group ^ key) * 16);
+  const u32x4 hi = *reinterpret_cast<const u32x4*>(row + ((group + 4) ^ key) * 16);
+  i32x8 f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (int)lo[i], f[4 + i] = (int)hi[i];
+  return f;
+}
+
+// All of this wave's reads of LDS are done and all but N of its loads have arrived; after the
+// barrier all waves'.
+template <int N>
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_reads();
+  wait_tile<N>();
+  workgroup_barrier();
+}
+
+// BM x BN tiles of WM x WN waves, two stages of 128 bytes a row in LDS.
+//
+// A wave goes through its rows of a with all its rows of b in registers.  The last kLast rows of a
+// it keeps back: once every wave has read the stage for the last time, these are multiplied column
+// by column, and between them the next stage's rows of b come into the registers that become free.
+// So the barrier, and the reads after it, lie under products; a stage's loads have a stage's time.
+// The loop has no branch, without which the compiler keeps everything in registers: the last block
+// of k, inside which rows may end, is taken first and its zeros are put in before the loop, and past
+// the last stage the last one is loaded again, to where nobody reads.
+//
+// Bound by power: 8192 x 8192 x 8192 takes 425 us, 2590 TFLOP/s, at a clock that falls to 1.8 GHz,
+// the matrix cores busy 68 in 100 clocks; with 32-bit scales for tiles 456 us, for rows 512.  Scales
+// that are applied afterwards are two products behind, which hides them: 495 and 575 us at once
+// after each product.  Four waves of 128 x 128 took 445 us, b straight to registers 764.
+template <int BM, int BN, int WM, int WN, int kLast, Mode kMode, bool kFull>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   constexpr int kWaves = WM * WN;
   constexpr int kRowsAll = BM + BN;
   constexpr int kCodes = kRowsAll * 128;
-  constexpr int kStage = kCodes + kRowsAll * 4;       // codes, then a scale for every row
-  constexpr int kLoads = kRowsAll / 8 / kWaves;       // of eight rows, a wave and stage
-  constexpr int kScaleLoads = kRowsAll / 64 / kWaves;  // of 64 rows' scales
+  constexpr int kStage = kCodes + kRowsAll * 4;  // codes, then a scale for every row
+  constexpr int kLoads = kRowsAll / 8 / kWaves;  // of eight rows, a wave and stage
+  constexpr int kScaleParts = kRowsAll / 64;     // loads of 64 rows' scales
+  constexpr int kScaleLoads = (kScaleParts + kWaves - 1) / kWaves;
   constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
-  static_assert(kLoads * 8 * kWaves == kRowsAll && BM % (8 * kWaves) == 0 &&
-                    kScaleLoads * 64 * kWaves == kRowsAll && NT % 4 == 0 && BM % 64 == 0,
+  static_assert(kLoads * 8 * kWaves == kRowsAll && BM % (8 * kWaves) == 0 && NT % 4 == 0 &&
+                    BM % 64 == 0 && BN % 64 == 0 && kLast > 1 && kLast <= MT,
                 "tile shape");
   constexpr int kBytes = kMode == kHardware ? 1 : 4;  // of a scale
   __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
@@ -187,62 +251,68 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   const int tn = x / high, tm = top + x - tn * high;
   const int m0 = tm * BM, n0 = tn * BN;
   const int from = part * g.per, steps = min(g.per, g.steps - from);
-  const int left = g.K - (from + steps - 1) * 128;  // numbers of the last step
+  const int64_t last_block = from + steps - 1;
+  const int left = min(g.K - (int)last_block * 128, 128);  // numbers of it
 
-  // A wave's load fills eight rows of a stage.  The 16-byte pieces of a row are permuted by its
-  // number so that the eight rows of which lanes next to each other read a piece lie in
-  // different banks: rows 0 .. 7 of a; of b, whose rows a product takes as row_of_b says, four
-  // and the four that are 16 on.
+  // A wave's load fills eight rows.  Keys of rows: of a, its number; of b, whose rows a product
+  // takes as row_of_b says, four rows and the four that are 16 on.
   auto key = [](bool second, int row) { return second ? (row & 3) | ((row >> 2) & 4) : row & 7; };
-  const uint8_t* abase = scalar_base(g.a.codes + (int64_t)m0 * g.a.pitch + (int64_t)from * 128);
-  const uint8_t* bbase = scalar_base(g.b.codes + (int64_t)n0 * g.b.pitch + (int64_t)from * 128);
+  const uint8_t* abase = scalar_base(g.a.codes + (int64_t)m0 * g.a.pitch + last_block * 128);
+  const uint8_t* bbase = scalar_base(g.b.codes + (int64_t)n0 * g.b.pitch + last_block * 128);
+  auto row_of_load = [&](int q) {
+    return (q * kWaves + wave) * 8 + lane / 8 - (q * kWaves * 8 >= BM ? BM : 0);
+  };
+  auto piece_of_load = [&](int q) {
+    return ((lane & 7) ^ key(q * kWaves * 8 >= BM, row_of_load(q))) * 16;
+  };
+  // by how much a lane's piece lies past the last that may be read of the last block
+  auto past_end = [&](int q) {
+    return (uint32_t)max(piece_of_load(q) - (((left + 15) & ~15) - 16), 0);
+  };
   uint32_t off[kLoads];
-  auto row_of_load = [&](int q) { return (q * kWaves + wave) * 8 + lane / 8; };
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) {
     const bool second = q * kWaves * 8 >= BM;
-    const int r = row_of_load(q) - (second ? BM : 0);
     const Side& s = second ? g.b : g.a;
-    const int last = s.rows - (second ? n0 : m0) - 1;
-    off[q] = (uint32_t)min(r, last) * (uint32_t)s.pitch + ((lane & 7) ^ key(second, r)) * 16;
+    // rows past the operand's last are copies of it, whose sums are not stored
+    const int row = min(row_of_load(q), s.rows - (second ? n0 : m0) - 1);
+    off[q] = (uint32_t)row * (uint32_t)s.pitch + piece_of_load(q) - past_end(q);
   }
-  // rows' scales, 64 a load
   const uint8_t* sbase[kScaleLoads];
   uint32_t soff[kScaleLoads];
+  auto scale_part = [&](int q) { return min(q * kWaves + wave, kScaleParts - 1); };
 #pragma unroll
   for (int q = 0; q < kScaleLoads; ++q) {
-    const bool second = (q * kWaves + wave) * 64 >= BM;
+    const bool second = scale_part(q) * 64 >= BM;
     const Side& s = second ? g.b : g.a;
     const int first = second ? n0 : m0;
-    const int r = min((q * kWaves + wave) * 64 - (second ? BM : 0) + lane, s.rows - first - 1);
-    sbase[q] = scalar_base(s.scales + (int64_t)(first >> s.shift) * s.s_row + from * s.s_block);
+    const int r = min(scale_part(q) * 64 - (second ? BM : 0) + lane, s.rows - first - 1);
+    sbase[q] = scalar_base(s.scales + (int64_t)(first >> s.shift) * s.s_row +
+                           last_block * s.s_block);
     soff[q] = (uint32_t)(((first + r) >> s.shift) - (first >> s.shift)) * (uint32_t)s.s_row;
   }
   const int64_t a_step = g.a.s_block, b_step = g.b.s_block;
   const uint32_t lds0 = offset_of(lds);
-  auto load = [&](int s) {
+  auto load_some = [&](int s, int q0, int q1) {
     const uint32_t to = lds0 + (s & 1) * kStage;
-    const bool tail = s == steps - 1 && left < 128;
-    const int end = ((left + 15) & ~15) - 16;  // the last piece that may be read
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
-      const bool second = q * kWaves * 8 >= BM;
-      uint32_t o = off[q];
-      if (tail) {
-        const int p = ((lane & 7) ^ key(second, row_of_load(q) - (second ? BM : 0))) * 16;
-        o -= max(p - end, 0);
-      }
-      load_lds16(second ? bbase : abase, o,
-                 __builtin_amdgcn_readfirstlane(to + (q * kWaves + wave) * 1024));
-    }
+    for (int q = 0; q < kLoads; ++q)
+      if (q >= q0 && q < q1)
+        load_lds16(q * kWaves * 8 >= BM ? bbase : abase, off[q],
+                   __builtin_amdgcn_readfirstlane(to + (q * kWaves + wave) * 1024));
+  };
+  // the scales, and on to the next block: after the last the first
+  auto load_rest = [&](int s) {
+    const uint32_t to = lds0 + (s & 1) * kStage;
+    const int64_t by = s == 0 ? 1 - steps : s + 1 < steps ? 1 : 0;
 #pragma unroll
     for (int q = 0; q < kScaleLoads; ++q) {
       load_lds4<kBytes>(sbase[q], soff[q],
-                        __builtin_amdgcn_readfirstlane(to + kCodes + (q * kWaves + wave) * 256));
-      sbase[q] += (q * kWaves + wave) * 64 >= BM ? b_step : a_step;
+                        __builtin_amdgcn_readfirstlane(to + kCodes + scale_part(q) * 256));
+      sbase[q] += by * (scale_part(q) * 64 >= BM ? b_step : a_step);
     }
-    abase += 128;
-    bbase += 128;
+    abase += by * 128;
+    bbase += by * 128;
   };
 
   f32x4 acc[MT][NT];
@@ -260,57 +330,107 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   const int ka = key(false, piece), kb = key(true, row_of_b(0, piece));
   const uint8_t* const fa0 = lds + (wi + piece) * 128;
   const uint8_t* const fb0 = lds + (BM + row_of_b(0, piece)) * 128;
-  auto read = [&](const uint8_t* row, int k) {
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(row + ((2 * group) ^ k) * 16);
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(row + ((2 * group + 1) ^ k) * 16);
-    i32x8 f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = (int)lo[i], f[4 + i] = (int)hi[i];
-    return f;
-  };
   constexpr int kB = scales_of_b<kMode, kFull>();
-
-  load(0);
-  for (int s = 0; s < steps; ++s) {
-    // this wave's share of the stage is there, and its reads of the one before are done; after
-    // the barrier all waves'
-    wait_reads();
-    wait_tile<0>();
-    workgroup_barrier();
-    if (s + 1 < steps) load(s + 1);
+  Operand<kFull> fb[NT], fa[kLast];  // row m of a in fa[m % kLast]
+  uint32_t sb[NT][kB], sa[kLast];
+  auto get_b = [&](int s, int n) {
     const int stage = (s & 1) * kStage;
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(lds + stage + kCodes);
-    if (s == steps - 1 && left < 128) {  // what lies past the end of a row: zeros
-      for (int i = threadIdx.x; i < kRowsAll * 8; i += 64 * kWaves) {
-        const int row = i >> 3, r = row < BM ? row : row - BM;
-        const int valid = left - ((i & 7) ^ key(row >= BM, r)) * 16;
-        if (valid < 16) cut16(reinterpret_cast<u32x4*>(lds + stage + i * 16), valid);
-      }
-      __syncthreads();
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(lds + stage + kCodes) + BM;
+    fb[n] = operand<kFull>(
+        read_row(fb0 + stage + ((n >> 2) * 64 + 4 * (n & 3)) * 128, group, kb));
+#pragma unroll
+    for (int r = 0; r < kB; ++r)
+      sb[n][r] = ready<kMode, kFull>(
+          scales[kMode == kTiles ? wj + (n >> 2) * 64
+                                 : (kB == 1 ? row_of_b(n, piece) : row_of_b(n, 4 * group) + r)]);
+  };
+  auto get_a = [&](int s, int m) {
+    const int stage = (s & 1) * kStage;
+    fa[m % kLast] = operand<kFull>(read_row(fa0 + stage + m * 2048, group, ka));
+    sa[m % kLast] = ready<kMode, kFull>(
+        reinterpret_cast<const uint32_t*>(lds + stage + kCodes)[wi + m * 16 + piece]);
+  };
+
+  // Product j of a stage: rows one after the other, the last ones column by column.
+  constexpr int kFirst = (MT - kLast) * NT;
+  auto row_of = [&](int j) { return j < kFirst ? j / NT : MT - kLast + (j - kFirst) % kLast; };
+  auto col_of = [&](int j) { return j < kFirst ? j % NT : (j - kFirst) / kLast; };
+  // Scales that are applied afterwards: two products behind, while the next ones run.
+  constexpr bool kLater = applied_later<kMode, kFull>();
+  constexpr int kBehind = 2;
+  f32x4 ring[kBehind];
+  float factors[kBehind][kB];
+  auto retire = [&](int j) {
+    const int m = row_of(j), n = col_of(j);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      acc[m][n][r] =
+          fmaf(factors[j % kBehind][kB == 1 ? 0 : r], ring[j % kBehind][r], acc[m][n][r]);
+  };
+  auto multiply = [&](int j) {
+    const int m = row_of(j), n = col_of(j);
+    if constexpr (!kLater) {
+      acc[m][n] = block<kMode, kFull>(fb[n], fa[m % kLast], acc[m][n], sb[n], sa[m % kLast]);
+    } else {
+      if (j >= kBehind) retire(j - kBehind);
+#pragma unroll
+      for (int r = 0; r < kB; ++r)
+        factors[j % kBehind][r] = as_float(sa[m % kLast]) * as_float(sb[n][r]);
+      ring[j % kBehind] = sums<kFull>(fb[n], fa[m % kLast]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    Operand<kFull> fb[NT];
-    uint32_t sb[NT][kB];
+  };
+
+  load_some(0, 0, kLoads);
+  if (steps > 1) {
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) off[q] += past_end(q);
+  }
+  load_rest(0);
+  arrive<0>();
+  load_some(1, 0, kLoads);
+  load_rest(1);
+  if (left < 128) {  // zeros where rows have ended
+    for (int i = threadIdx.x; i < kRowsAll * 8; i += 64 * kWaves) {
+      const int row = i >> 3;
+      const int valid = left - ((i & 7) ^ key(row >= BM, row < BM ? row : row - BM)) * 16;
+      if (valid < 16) cut16(reinterpret_cast<u32x4*>(lds + i * 16), valid);
+    }
+    wait_reads();
+    workgroup_barrier();
+  }
+  get_a(0, 0);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) get_b(0, n);
+  for (int s = 0; s < steps; ++s) {
+#pragma unroll
+    for (int m = 0; m < MT - kLast; ++m) {
+      get_a(s, m + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) multiply(m * NT + n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int m = MT - kLast + 1; m < MT; ++m) get_a(s, m);
+    arrive<0>();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      fb[n] = operand<kFull>(read(fb0 + stage + ((n >> 2) * 64 + 4 * (n & 3)) * 128, kb));
-      if constexpr (kMode == kTiles) {
-        sb[n][0] = scales[BM + wj + (n >> 2) * 64];
-      } else if constexpr (kB == 1) {
-        sb[n][0] = scales[BM + row_of_b(n, piece)];
-      } else {
+      load_some(s + 2, n * kLoads / NT, (n + 1) * kLoads / NT);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sb[n][r] = scales[BM + row_of_b(n, 4 * group) + r];
-      }
+      for (int m = 0; m < kLast; ++m) multiply(kFirst + n * kLast + m);
+      __builtin_amdgcn_sched_barrier(0);
+      get_b(s + 1, n);
+      if (n == NT - 1) get_a(s + 1, 0);
     }
+    load_rest(s + 2);
+    if constexpr (kLater) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const Operand<kFull> fa = operand<kFull>(read(fa0 + stage + m * 2048, ka));
-      const uint32_t sa = scales[wi + m * 16 + piece];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-        acc[m][n] = block<kMode, kFull>(fb[n], fa, acc[m][n], sb[n], sa);
+      for (int j = MT * NT - kBehind; j < MT * NT; ++j) retire(j);
     }
   }
+  wait_tile<0>();  // nothing is on its way to LDS when it is given back
 
   // a lane's 16 sums of a row, next to each other
 #pragma unroll
@@ -334,41 +454,146 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   }
 }
 
-// Few rows of a: 16 rows of b a workgroup, straight to registers, its eight waves taking blocks
-// of k in turn and their sums added at the end in a fixed order.  Bound by the reading of b.
+// Few rows of a, many numbers of b: 64 rows of b a workgroup of four waves, S stages of 128 bytes a
+// row in LDS, so that 100 KB a CU are on their way.  Bound by the reading of b: 37 rows times 16384 x
+// 2048 8.8 us, times 8192 x 4096 11.5, where thin_kernel, which reads a from L2 for every 16 rows of
+// b, takes 15.8 and 15.9.
+template <int MT, int S, Mode kMode, bool kFull>
+__global__ __launch_bounds__(256) void slim_kernel(Args g) {
+  constexpr int kWaves = 4, BM = (MT * 16 + 31) / 32 * 32, BN = 64, kRowsAll = BM + BN;
+  constexpr int kCodes = kRowsAll * 128, kStage = kCodes + 128 * 4;
+  constexpr int kLoads = kRowsAll / 8 / kWaves;
+  constexpr int kBytes = kMode == kHardware ? 1 : 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
+  const int lane = threadIdx.x & 63, group = lane >> 4, piece = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * BN, part = blockIdx.y;
+  const int from = part * g.per, steps = min(g.per, g.steps - from);
+  const int64_t last_block = from + steps - 1;  // taken first, as in tile_kernel
+  const int left = min(g.K - (int)last_block * 128, 128);
+  const uint8_t* abase = scalar_base(g.a.codes + last_block * 128);
+  const uint8_t* bbase = scalar_base(g.b.codes + (int64_t)n0 * g.b.pitch + last_block * 128);
+  const int swapped = ((lane & 7) ^ (lane >> 3)) * 16;
+  const uint32_t past = (uint32_t)max(swapped - (((left + 15) & ~15) - 16), 0);
+  uint32_t off[kLoads];
+#pragma unroll
+  for (int q = 0; q < kLoads; ++q) {
+    const bool second = q * kWaves * 8 >= BM;
+    const Side& s = second ? g.b : g.a;
+    const int r = (q * kWaves + wave) * 8 + lane / 8 - (second ? BM : 0);
+    off[q] = (uint32_t)min(r, s.rows - (second ? n0 : 0) - 1) * (uint32_t)s.pitch + swapped - past;
+  }
+  // scales: a's by the first and the third wave, b's by the others
+  const bool sb_wave = wave & 1;
+  const Side& ss = sb_wave ? g.b : g.a;
+  const int sfirst = sb_wave ? n0 : 0;
+  const int sr = min(lane, ss.rows - sfirst - 1);
+  const uint8_t* sbase = scalar_base(ss.scales + (int64_t)(sfirst >> ss.shift) * ss.s_row +
+                                     last_block * ss.s_block);
+  const uint32_t soff =
+      (uint32_t)(((sfirst + sr) >> ss.shift) - (sfirst >> ss.shift)) * (uint32_t)ss.s_row;
+  const int64_t sstep = ss.s_block;
+  const uint32_t lds0 = offset_of(lds);
+  uint32_t to = lds0;
+  int done = 0;
+  auto load = [&]() {
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q)
+      load_lds16(q * kWaves * 8 >= BM ? bbase : abase, off[q],
+                 __builtin_amdgcn_readfirstlane(to + (q * kWaves + wave) * 1024));
+    load_lds4<kBytes>(sbase, soff, __builtin_amdgcn_readfirstlane(to + kCodes + (wave & 1) * 256));
+    const int64_t by = done == 0 ? 1 - steps : done + 1 < steps ? 1 : 0;
+    ++done;
+    abase += by * 128;
+    bbase += by * 128;
+    sbase += by * sstep;
+    to += kStage;
+    if (to == lds0 + S * kStage) to = lds0;
+  };
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = nl2k::zero4();
+  const int ka = piece & 7;
+  const uint8_t* const fa0 = lds + piece * 128;
+  const uint8_t* const fb0 = lds + (BM + wave * 16 + piece) * 128;
+  constexpr int kB = scales_of_b<kMode, kFull>();
+  load();
+  if (steps > 1) {
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) off[q] += past;
+  }
+#pragma unroll
+  for (int s = 1; s < S - 1; ++s) load();
+  int stage = 0;
+  for (int s = 0; s < steps; ++s) {
+    arrive<(S - 2) * (kLoads + 1)>();
+    load();
+    if (s == 0 && left < 128) {
+      for (int i = threadIdx.x; i < kRowsAll * 8; i += 64 * kWaves) {
+        const int valid = left - ((i & 7) ^ ((i >> 3) & 7)) * 16;
+        if (valid < 16) cut16(reinterpret_cast<u32x4*>(lds + i * 16), valid);
+      }
+      wait_reads();
+      workgroup_barrier();
+    }
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(lds + stage + kCodes);
+    const Operand<kFull> fb = operand<kFull>(read_row(fb0 + stage, group, ka));
+    uint32_t sb[kB];
+#pragma unroll
+    for (int r = 0; r < kB; ++r)
+      sb[r] = ready<kMode, kFull>(
+          scales[64 + wave * 16 + (kB == 4 ? 4 * group + r : (kMode == kTiles ? 0 : piece))]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      acc[m] = block<kMode, kFull>(
+          fb, operand<kFull>(read_row(fa0 + stage + m * 2048, group, ka)), acc[m], sb,
+          ready<kMode, kFull>(scales[m * 16 + piece]));
+    stage += kStage;
+    if (stage == S * kStage) stage = 0;
+  }
+  wait_tile<0>();
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int row = m * 16 + piece, col = n0 + wave * 16 + 4 * group;
+    if (row >= g.a.rows) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r < g.b.rows) put1(g, part, row, col + r, acc[m][r]);
+  }
+}
+
+// Few rows of a: 16 rows of b a workgroup, straight to registers, its eight waves taking U blocks of
+// k in turn, the next ones on their way, and their sums added at the end in a fixed order.  Bound by
+// the reading of b: one row times 8192 x 4096 7.6 us (4.4 TB/s), times 4096 x 14336 12.2 (4.8).
 constexpr int kThinWaves = 8;
 
-template <int MT, Mode kMode, bool kFull>
+template <int MT, int U, Mode kMode, bool kFull>
 __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
-  constexpr int U = MT <= 2 ? 4 : 2;  // blocks in flight
-  __shared__ __attribute__((aligned(16))) float sums[kThinWaves][MT * 256];
+  __shared__ __attribute__((aligned(16))) float red[kThinWaves][MT * 256];
   const int lane = threadIdx.x & 63, group = lane >> 4, piece = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * 16, part = blockIdx.y;
   const int from = part * g.per, upto = min(from + g.per, g.steps);
   const int left = g.K - (g.steps - 1) * 128;  // numbers of the last block
   const uint32_t end = (uint32_t)((g.K + 15) & ~15) - 16;
+  constexpr int kB = scales_of_b<kMode, kFull>();
+  const uint8_t *pa[MT], *qa[MT], *qb[kB];
   const uint8_t* pb = g.b.codes + (int64_t)min(n0 + piece, g.b.rows - 1) * g.b.pitch;
-  const uint8_t* pa[MT];
-  const uint8_t* qa[MT];
+#pragma unroll
+  for (int r = 0; r < kB; ++r) {
+    const int row = n0 + (kB == 4 ? 4 * group + r : (kMode == kTiles ? 0 : piece));
+    qb[r] = g.b.scales + (int64_t)(min(row, g.b.rows - 1) >> g.b.shift) * g.b.s_row;
+  }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int row = min(m * 16 + piece, g.a.rows - 1);
     pa[m] = g.a.codes + (int64_t)row * g.a.pitch;
     qa[m] = g.a.scales + (int64_t)(row >> g.a.shift) * g.a.s_row;
   }
-  constexpr int kB = scales_of_b<kMode, kFull>();
-  const uint8_t* qb[kB];
-#pragma unroll
-  for (int r = 0; r < kB; ++r) {
-    // by the instruction: of this lane's row; afterwards: of the rows of its sums
-    const int row = kB == 4 ? n0 + 4 * group + r : (kMode == kTiles ? n0 : n0 + piece);
-    qb[r] = g.b.scales + (int64_t)(min(row, g.b.rows - 1) >> g.b.shift) * g.b.s_row;
-  }
   auto fragment = [&](const uint8_t* p, int s) {
-    const uint32_t k = s * 128 + group * 32;
+    const uint32_t k = s * 128 + group * 16;
     const u32x4 lo = *reinterpret_cast<const u32x4*>(p + min(k, end));
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(p + min(k + 16, end));
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(p + min(k + 64, end));
     i32x8 f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = (int)lo[i], f[4 + i] = (int)hi[i];
@@ -376,26 +601,31 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
   };
   auto scale = [&](const uint8_t* p, int64_t step, int s) {
     p += s * step;
-    return kMode == kHardware ? (uint32_t)*p : *reinterpret_cast<const uint32_t*>(p);
+    return ready<kMode, kFull>(kMode == kHardware ? (uint32_t)*p
+                                                  : *reinterpret_cast<const uint32_t*>(p));
+  };
+  struct Batch {
+    i32x8 fb[U], fa[U][MT];
+    uint32_t sb[U][kB], sa[U][MT];
+  };
+  auto fetch = [&](int s0, Batch& t) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + u * kThinWaves, upto - 1);
+      t.fb[u] = fragment(pb, s);
+#pragma unroll
+      for (int r = 0; r < kB; ++r) t.sb[u][r] = scale(qb[r], g.b.s_block, s);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        t.fa[u][m] = fragment(pa[m], s);
+        t.sa[u][m] = scale(qa[m], g.a.s_block, s);
+      }
+    }
   };
   f32x4 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = nl2k::zero4();
-  for (int s0 = from + wave; s0 < upto; s0 += kThinWaves * U) {
-    i32x8 fb[U], fa[U][MT];
-    uint32_t sb[U][kB], sa[U][MT];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = min(s0 + u * kThinWaves, upto - 1);
-      fb[u] = fragment(pb, s);
-#pragma unroll
-      for (int r = 0; r < kB; ++r) sb[u][r] = scale(qb[r], g.b.s_block, s);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        fa[u][m] = fragment(pa[m], s);
-        sa[u][m] = scale(qa[m], g.a.s_block, s);
-      }
-    }
+  auto use = [&](int s0, Batch& t) {
     // All that depends on where k ends comes before the products, and a block past the end is
     // taken as zeros: no branch lies between a product and what reads it.  (Across one, hipcc of
     // ROCm 7.2 left a sum's first reader two instructions behind the matrix instruction, which
@@ -405,38 +635,44 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
       const int s = s0 + u * kThinWaves;
       const int valid = s >= upto ? 0 : (s == g.steps - 1 ? left : 128);
       if (valid < 128) {
-        cut(fb[u], valid, group);
+        cut(t.fb[u], valid, group);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) cut(fa[u][m], valid, group);
+        for (int m = 0; m < MT; ++m) cut(t.fa[u][m], valid, group);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Operand<kFull> ob = operand<kFull>(fb[u]);
+      const Operand<kFull> ob = operand<kFull>(t.fb[u]);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
         acc[m] =
-            block<kMode, kFull>(ob, operand<kFull>(fa[u][m]), acc[m], sb[u], sa[u][m]);
+            block<kMode, kFull>(ob, operand<kFull>(t.fa[u][m]), acc[m], t.sb[u], t.sa[u][m]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  Batch t0, t1;
+  int s0 = from + wave;
+  fetch(s0, t0);
+  while (s0 < upto) {
+    if (s0 + kThinWaves * U < upto) fetch(s0 + kThinWaves * U, t1);
+    use(s0, t0);
+    s0 += kThinWaves * U;
+    if (s0 >= upto) break;
+    if (s0 + kThinWaves * U < upto) fetch(s0 + kThinWaves * U, t0);
+    use(s0, t1);
+    s0 += kThinWaves * U;
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m)
-    *reinterpret_cast<f32x4*>(&sums[wave][m * 256 + piece * 16 + group * 4]) = acc[m];
+    *reinterpret_cast<f32x4*>(&red[wave][m * 256 + piece * 16 + group * 4]) = acc[m];
   __syncthreads();
   for (int i = threadIdx.x; i < MT * 256; i += 64 * kThinWaves) {
-    float v = sums[0][i];
+    float v = red[0][i];
 #pragma unroll
-    for (int w = 1; w < kThinWaves; ++w) v += sums[w][i];
+    for (int w = 1; w < kThinWaves; ++w) v += red[w][i];
     const int m = i >> 4, n = n0 + (i & 15);
-    if (m >= g.a.rows || n >= g.b.rows) continue;
-    const int64_t at = (int64_t)m * g.b.rows + n;
-    if (g.partial)
-      g.partial[(int64_t)part * g.a.rows * g.b.rows + at] = v;
-    else if (g.out_dtype == kF32)
-      static_cast<float*>(g.out)[at] = v;
-    else
-      static_cast<unsigned short*>(g.out)[at] =
-          g.out_dtype == kBF16 ? narrow<bf16_t>(v) : narrow<f16_t>(v);
+    if (m < g.a.rows && n < g.b.rows) put1(g, part, m, n, v);
   }
 }
 
@@ -458,47 +694,96 @@ __global__ __launch_bounds__(256) void join_kernel(Args g, int parts) {
 }
 
 // The kernel and the parts of k for a product's sizes.
+enum Kernel { kThin, kSlim, kTile128, kTile256x128, kTile256 };
+
+constexpr int64_t kMostParts = 16;
+
 struct Plan {
-  int tile;   // rows of a and of b a workgroup takes, 0: few rows
-  int parts, per;
-  int64_t blocks;
+  Kernel kernel;
+  int bm, bn;        // rows of a and of b a workgroup takes
+  int parts, per;    // parts of k, and the blocks of one
+  int64_t blocks;    // workgroups of a part
 };
 
 Plan plan(int64_t M, int64_t N, int64_t K, bool full) {
-  const int64_t steps = nl2k::ceil_div(K, 128);
-  Plan p{};
-  int64_t wanted;
+  const int64_t steps = nl2k::ceil_div(K, kBlock);
+  auto divide = [&](Kernel kernel, int bm, int bn, int64_t wanted) {
+    Plan p{};
+    p.kernel = kernel, p.bm = bm, p.bn = bn;
+    p.blocks = nl2k::ceil_div(M, bm) * nl2k::ceil_div(N, bn);
+    wanted = std::max(std::min(wanted, std::min(steps, kMostParts)), (int64_t)1);
+    p.per = (int)nl2k::ceil_div(steps, wanted);
+    p.parts = (int)nl2k::ceil_div(steps, p.per);
+    return p;
+  };
   if (M <= 64) {
-    p.tile = 0;
-    p.blocks = nl2k::ceil_div(N, 16);
-    wanted = std::min(256 / p.blocks, steps / (4 * kThinWaves));
-  } else {
-    p.tile = !full && nl2k::ceil_div(M, 256) * nl2k::ceil_div(N, 256) >= 192 ? 256 : 128;
-    p.blocks = nl2k::ceil_div(M, p.tile) * nl2k::ceil_div(N, p.tile);
-    wanted = std::min(256 / p.blocks, steps / 8);
+    const int64_t n64 = nl2k::ceil_div(N, 64), n16 = nl2k::ceil_div(N, 16);
+    // below 2^24 numbers of b a workgroup for every 16 rows of it is faster: 5.6 us for 7.7 at 37
+    // rows times 2048 x 2048
+    if (M > 16 && N * K > (int64_t)1 << 24) return divide(kSlim, 64, 64, 256 / n64);
+    return divide(kThin, 64, 16, std::min(256 / n16, steps / 32));
   }
-  wanted = std::max(std::min(wanted, (int64_t)16), (int64_t)1);
-  p.per = (int)nl2k::ceil_div(steps, wanted);
-  p.parts = (int)nl2k::ceil_div(steps, p.per);
-  return p;
+  // Microseconds of a stage on an idle chip, and on one whose every CU has a tile, or two of the
+  // 128-wide ones; with scales in 8 bits.  Products in full precision leave registers for those alone.
+  struct Tile {
+    Kernel kernel;
+    int bm, bn, a_round;
+    double idle, busy;
+  };
+  static const Tile kFast[] = {{kTile256, 256, 256, 256, 1.2, 1.6},
+                               {kTile256x128, 256, 128, 256, 0.72, 1.0},
+                               {kTile128, 128, 128, 512, 0.65, 1.15}};
+  static const Tile kPrecise[] = {{kTile128, 128, 128, 512, 1.35, 2.4}};
+  Plan best{};
+  double least = 1e30;
+  for (int i = 0; i < (full ? 1 : 3); ++i) {
+    const Tile& t = full ? kPrecise[i] : kFast[i];
+    for (int64_t wanted = 1; wanted <= kMostParts; ++wanted) {
+      const Plan p = divide(t.kernel, t.bm, t.bn, wanted);
+      const int64_t n = p.blocks * p.parts, rounds = nl2k::ceil_div(n, t.a_round);
+      const double share = t.a_round == 256 ? std::min(n / 256.0, 1.0) : (n > 256 ? 1.0 : 0.0);
+      double us = (double)(rounds * p.per) * (t.idle + (t.busy - t.idle) * share);
+      // the parts' sums: a launch, and their bytes
+      if (p.parts > 1) us += 3.0 + 2e-6 * (double)p.parts * (double)(M * N);
+      if (us < least) least = us, best = p;
+    }
+  }
+  return best;
 }
 
 template <Mode kMode, bool kFull>
 int launch(const Args& g, const Plan& p, hipStream_t s) {
-  if (p.tile == 0) {
-    const dim3 grid((uint32_t)p.blocks, (uint32_t)p.parts);
+  const dim3 grid((uint32_t)p.blocks, (uint32_t)p.parts), tiles((uint32_t)g.tiles);
+  const int mt = (g.a.rows + 15) / 16;
+  if (p.kernel == kThin) {
     const int threads = 64 * kThinWaves;
-    switch ((g.a.rows + 15) / 16) {
-      case 1: thin_kernel<1, kMode, kFull><<<grid, threads, 0, s>>>(g); break;
-      case 2: thin_kernel<2, kMode, kFull><<<grid, threads, 0, s>>>(g); break;
-      case 3: thin_kernel<3, kMode, kFull><<<grid, threads, 0, s>>>(g); break;
-      default: thin_kernel<4, kMode, kFull><<<grid, threads, 0, s>>>(g); break;
-    }
-  } else if (p.tile == 256) {
-    if constexpr (!kFull)
-      tile_kernel<256, 256, 2, 4, kMode, kFull><<<dim3((uint32_t)g.tiles), 512, 0, s>>>(g);
-  } else {
-    tile_kernel<128, 128, 2, 2, kMode, kFull><<<dim3((uint32_t)g.tiles), 256, 0, s>>>(g);
+    // two blocks at a time where a wave has three to eight: 7.6 us for 8.3 at 32 blocks of 8192 rows,
+    // but 8.3 for 7.5 at 16 of 16384 rows and 12.9 for 12.2 at 112 of 4096
+    const bool two = g.per > 2 * kThinWaves && g.per <= 8 * kThinWaves;
+    if (mt == 1 && two)
+      thin_kernel<1, 2, kMode, kFull><<<grid, threads, 0, s>>>(g);
+    else if (mt == 1)
+      thin_kernel<1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+    else if (mt == 2)
+      thin_kernel<2, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+    else if (mt == 3)
+      thin_kernel<3, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+    else
+      thin_kernel<4, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+  } else if (p.kernel == kSlim) {
+    if (mt <= 2)
+      slim_kernel<2, 4, kMode, kFull><<<grid, 256, 0, s>>>(g);
+    else if (mt == 3)
+      slim_kernel<3, 4, kMode, kFull><<<grid, 256, 0, s>>>(g);
+    else
+      slim_kernel<4, 4, kMode, kFull><<<grid, 256, 0, s>>>(g);
+  } else if (p.kernel == kTile128) {
+    tile_kernel<128, 128, 2, 2, 2, kMode, kFull><<<tiles, 256, 0, s>>>(g);
+  } else if constexpr (!kFull) {  // 16 bits an operand do not leave registers for more
+    if (p.kernel == kTile256x128)
+      tile_kernel<256, 128, 4, 2, 2, kMode, kFull><<<tiles, 512, 0, s>>>(g);
+    else
+      tile_kernel<256, 256, 2, 4, 3, kMode, kFull><<<tiles, 512, 0, s>>>(g);
   }
   int st = nl2k::check_launch("block_matmul");
   if (st || p.parts == 1) return st;
@@ -600,11 +885,9 @@ extern "C" int block_matmul(const void* a, int64_t a_pitch, const void* a_scales
   g.steps = (int32_t)nl2k::ceil_div(K, 128);
   g.per = p.per;
   g.out_dtype = out_dtype;
-  if (p.tile) {
-    g.tiles_a = (int32_t)nl2k::ceil_div(M, p.tile);
-    g.tiles_b = (int32_t)nl2k::ceil_div(N, p.tile);
-    g.tiles = (int32_t)(p.blocks * p.parts);
-  }
+  g.tiles_a = (int32_t)nl2k::ceil_div(M, p.bm);
+  g.tiles_b = (int32_t)nl2k::ceil_div(N, p.bn);
+  g.tiles = (int32_t)(p.blocks * p.parts);
   const bool full = out_dtype == kF32;
   if (scale_type == kScaleE8M0)
     return full ? launch<kHardware, true>(g, p, stream) : launch<kHardware, false>(g, p, stream);

@@ -75,6 +75,39 @@ def test_many_tiles(tiles, scale_dtype):
     _check(half[rows.cuda()][:, cols.cuda()], av[rows], bv[cols], torch.bfloat16)
 
 
+@pytest.mark.parametrize("scale_dtype", SCALES, ids=str)
+@pytest.mark.parametrize("tiles", [(False, True), (False, False)])
+@pytest.mark.parametrize("m,n,k", [
+    (16, 16390, 1030),        # a token or a few: two blocks at a time, and one
+    (1, 700, 16500),
+    (17, 16390, 1030),        # few rows, many numbers of b: stages, one part
+    (40, 4099, 4111),         # and parts of k
+    (64, 1200, 14345),
+    (1300, 3100, 515),        # tiles of 128
+    (2100, 4000, 300),        # of 256 x 128
+    (4100, 4000, 130),        # of 256
+])
+def test_every_kernel(m, n, k, tiles, scale_dtype):
+    """Sizes that take each kernel, ragged at every end: all against 64 bits, 16-bit results also
+    against the float32 ones."""
+    from cases.block_matmul.op import block_matmul
+    announce(f"block_matmul kernels {m} x {n} x {k} tiles {tiles} {scale_dtype}")
+    ((a, av), (b, bv)) = _operands(m, n, k, tiles, scale_dtype)
+    out = block_matmul(*a, *b, out_dtype=torch.float32).double()
+    av, bv = av.cuda(), bv.cuda()
+    want, size = av @ bv.t().contiguous(), av.abs() @ bv.abs().t().contiguous()
+    assert torch.all((out - want).abs() <= tol.matmul_error(av, bv, size, want, torch.float32))
+    # seven of eight products are off by 2^-13 of the largest, which their sum of magnitudes bounds
+    for dtype in (torch.bfloat16, torch.float16):
+        half = block_matmul(*a, *b, out_dtype=dtype).double()
+        err = tol.rounded(size * (2 * tol.U * (128 + 5 * (k // 128 + 1) + 16) + 7 * 2.0 ** -13), want,
+                          dtype)
+        assert torch.all((half - want).abs() <= err)
+        # as a whole nearer: of independent numbers a result's variance is at least that of the
+        # largest products, and that of what is dropped, evenly spread, 7 / 3 * 2^-26 of it
+        assert (half - want).norm() <= (tol.EPS[dtype] + 2.0 ** -12) * want.norm()
+
+
 def test_exact_sums():
     """Small whole numbers: every sum is exact in 32 bits, and eight products in 13, so the answers
     are equal, to their last rounding."""
