@@ -46,27 +46,53 @@ def _workspace_bytes(M, N, K, out_dtype):
 
 
 def _codes(c, rows, K):
-    """(codes, bytes between rows) as the kernels read them: rows 16 bytes apart or a multiple, the
+    """(codes, bytes between rows) as the kernels read them: rows a multiple of 16 bytes apart, the
     last one's memory up to the next 16; copied only if they lie otherwise."""
-    pitch, whole = c.stride(0) if rows > 1 else e4m3.pitch(K), e4m3.pitch(K)
+    whole = (K + 15) // 16 * 16
+    pitch = c.stride(0) if rows > 1 else whole
     if ((K == 1 or c.stride(1) == 1) and pitch >= K and pitch % 16 == 0 and
             pitch <= 2 * LONGEST and c.data_ptr() % 16 == 0 and
-            c.storage_offset() + (rows - 1) * pitch + whole <= c.untyped_storage().nbytes()):
+            (whole == K or c.storage_offset() + (rows - 1) * pitch + whole <=
+             c.untyped_storage().nbytes())):
         return c, pitch
-    copy, pitch = e4m3.new_codes((rows,), K, c.device)
+    copy, pitch = e4m3.new_codes(c, (rows,), K)
     copy.view(torch.uint8).copy_(c.view(torch.uint8))
     return copy, pitch
 
 
 def _scales(name, s, rows, K):
     """(scales, row stride, block stride, whether they are of tiles)."""
-    n = e4m3.blocks(K)
-    capi.require(s.dim() == 2 and s.size(1) == n and s.size(0) in (rows, e4m3.blocks(rows)),
-                 f"{name}_scales must be [rows, {n}] or, of tiles, [{e4m3.blocks(rows)}, {n}], "
-                 f"got {tuple(s.shape)}")
-    if s.stride(0) > LONGEST:
+    n, tiles = (K + 127) // 128, (rows + 127) // 128
+    shape = tuple(s.shape)
+    capi.require(shape == (rows, n) or shape == (tiles, n), name)
+    row, block = s.stride()
+    if row > LONGEST:
         s = s.contiguous()
-    return s, s.stride(0), s.stride(1), int(s.size(0) == e4m3.blocks(rows))
+        row, block = s.stride()
+    return s, row, block, int(shape[0] == tiles)
+
+
+def _product(a, a_scales, b, b_scales, out, M, N, K):
+    """out = a b^T for matrices of codes and their scales on one GPU."""
+    lib = _lib()
+    a, a_pitch = _codes(a, M, K)
+    b, b_pitch = _codes(b, N, K)
+    a_scales, a_row, a_block, a_tiles = _scales(
+        "a_scales must be [rows, blocks] of a or [tiles, blocks]", a_scales, M, K)
+    b_scales, b_row, b_block, b_tiles = _scales(
+        "b_scales must be [rows, blocks] of b or [tiles, blocks]", b_scales, N, K)
+    dtype = e4m3.DTYPES[out.dtype]
+    ws_bytes, ws_ptr = _workspace_bytes(M, N, K, dtype), 0
+    if ws_bytes:
+        ws = a.new_empty(ws_bytes // 4, dtype=torch.float32)
+        ws_ptr = ws.data_ptr()
+    st = capi.launch(lib.block_matmul, a.get_device(), a.data_ptr(), a_pitch, a_scales.data_ptr(),
+                     a_row, a_block, a_tiles, b.data_ptr(), b_pitch, b_scales.data_ptr(), b_row,
+                     b_block, b_tiles, e4m3.SCALES[a_scales.dtype], out.data_ptr(), dtype, M, N, K,
+                     ws_ptr, ws_bytes)
+    if st:
+        capi.check(st, lib.block_matmul_last_error, "block_matmul")
+    return out
 
 
 def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
@@ -80,42 +106,35 @@ def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
     rounded, which is what the 8-bit matrix instruction's additions cost; a
     float32 one takes the 16-bit instruction, half as fast, and has its 24 bits.
     """
-    tensors = (a, a_scales, b, b_scales)
-    capi.require(all(t.is_cuda for t in tensors), "codes and scales must be GPU tensors")
     device = a.get_device()
-    capi.require(all(t.get_device() == device for t in tensors[1:]),
+    capi.require(device >= 0 and a_scales.is_cuda and b.is_cuda and b_scales.is_cuda,
+                 "codes and scales must be GPU tensors")
+    capi.require(device == a_scales.get_device() == b.get_device() == b_scales.get_device(),
                  "codes and scales must be on one GPU")
     capi.require(a.dtype == b.dtype == e4m3.CODES, "a and b must be float8_e4m3fn")
     capi.require(a_scales.dtype == b_scales.dtype and a_scales.dtype in e4m3.SCALES,
                  "scales must both be float32 or both float8_e8m0fnu")
     capi.require(out_dtype in e4m3.DTYPES, "out_dtype must be float32, bfloat16 or float16")
-    capi.require(a.dim() >= 1 and b.dim() == 2 and a.size(-1) == b.size(1) >= 1,
+    shape = a.shape
+    capi.require(len(shape) >= 1 and b.dim() == 2 and shape[-1] == b.shape[1] >= 1,
                  "a must be [..., K] and b [N, K] with K >= 1")
-    capi.require(not differentiated(*tensors),
+    capi.require(not differentiated(a, a_scales, b, b_scales),
                  "block_matmul has no gradient: use block_linear, or torch.no_grad()")
-    lib = _lib()
-    lead, K, N = a.shape[:-1], a.size(-1), b.size(0)
-    out = torch.empty((*lead, N), dtype=out_dtype, device=a.device)
-    M = out.numel() // N if N else 0
-    if M == 0:
+    N, K = b.shape
+    if len(shape) == 2:
+        out = a.new_empty((shape[0], N), dtype=out_dtype)
+        M = shape[0]
+    else:
+        out = a.new_empty((*shape[:-1], N), dtype=out_dtype)
+        capi.require(a_scales.shape == (*shape[:-1], e4m3.blocks(K)),
+                     f"a_scales must be {(*shape[:-1], e4m3.blocks(K))}, got "
+                     f"{tuple(a_scales.shape)}")
+        M = out.numel() // N if N else 0
+        if M:
+            a, a_scales = a.reshape(M, K), a_scales.reshape(M, -1)
+    if M == 0 or N == 0:
         return out
-    if a.dim() != 2:
-        capi.require(a_scales.shape == (*lead, e4m3.blocks(K)),
-                     f"a_scales must be {(*lead, e4m3.blocks(K))}, got {tuple(a_scales.shape)}")
-        a, a_scales = a.reshape(M, K), a_scales.reshape(M, -1)
-    a, a_pitch = _codes(a, M, K)
-    b, b_pitch = _codes(b, N, K)
-    a_scales, *a_how = _scales("a", a_scales, M, K)
-    b_scales, *b_how = _scales("b", b_scales, N, K)
-    ws_bytes = _workspace_bytes(M, N, K, e4m3.DTYPES[out_dtype])
-    ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=a.device) if ws_bytes else None
-    st = capi.launch(lib.block_matmul, device, a.data_ptr(), a_pitch, a_scales.data_ptr(), *a_how,
-                     b.data_ptr(), b_pitch, b_scales.data_ptr(), *b_how,
-                     e4m3.SCALES[a_scales.dtype], out.data_ptr(), e4m3.DTYPES[out_dtype], M, N, K,
-                     ws.data_ptr() if ws_bytes else 0, ws_bytes)
-    if st:
-        capi.check(st, lib.block_matmul_last_error, "block_matmul")
-    return out
+    return _product(a, a_scales, b, b_scales, out, M, N, K)
 
 
 def quantize_weight(weight, scale_dtype=torch.float8_e8m0fnu):
@@ -128,40 +147,50 @@ class BlockLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, quantized, scale_dtype):
         want_x, want_w = ctx.needs_input_grad[:2]
-        rows = x.reshape(-1, x.size(-1))
+        N, K = weight.shape
+        rows = x if x.dim() == 2 else x.reshape(-1, K)
+        M = rows.shape[0]
         if want_w:
             codes, scales, codes_t, scales_t = quantize_rows(rows, scale_dtype, transposed=True)
         else:
             codes, scales, codes_t, scales_t = *quantize_rows(rows, scale_dtype), None, None
         if quantized is None:
             quantized = quantize_tiles(weight, scale_dtype, transposed=want_x)
-        y = block_matmul(codes, scales, quantized[0], quantized[1], x.dtype)
-        ctx.scale_dtype, ctx.dtypes, ctx.x_shape = scale_dtype, (x.dtype, weight.dtype), x.shape
-        ctx.w_shape = weight.shape
+        y = x.new_empty((*x.shape[:-1], N))
+        if M:
+            _product(codes, scales, quantized[0], quantized[1], y, M, N, K)
+        ctx.scale_dtype, ctx.dtypes = scale_dtype, (x.dtype, weight.dtype)
+        ctx.x_shape, ctx.w_shape = x.shape, weight.shape
         ctx.save_for_backward(codes_t, scales_t, *(quantized[2:] if want_x else (None, None)))
-        return y.view(*x.shape[:-1], weight.size(0))
+        return y
 
     @staticmethod
     def backward(ctx, dy):
         codes_t, scales_t, w_codes, w_scales = ctx.saved_tensors
         N, K = ctx.w_shape
-        dy = dy.reshape(-1, N)
-        M = dy.size(0)
-        if codes_t is not None:
-            capi.require(codes_t.shape == (K, M), "autograd gave back other tensors than were saved")
-        if w_codes is not None:
-            capi.require(w_codes.shape == (K, N), "autograd gave back other tensors than were saved")
+        if dy.dim() != 2:
+            dy = dy.reshape(-1, N)
+        M, device = dy.shape[0], dy.get_device()
+        # what autograd gives back of what was saved: every read lies within it
+        for codes, scales, n in ((codes_t, scales_t, M), (w_codes, w_scales, N)):
+            capi.require(codes is None or codes.shape == (K, n) and
+                         codes.dtype == e4m3.CODES and scales.dtype == ctx.scale_dtype and
+                         codes.get_device() == device == scales.get_device(),
+                         "autograd gave back other tensors than were saved")
         dx = dw = None
         if codes_t is None:
             codes, scales = quantize_rows(dy, ctx.scale_dtype)
         else:
             codes, scales, dy_t, dy_scales_t = quantize_rows(dy, ctx.scale_dtype, transposed=True)
             if M:
-                dw = block_matmul(dy_t, dy_scales_t, codes_t, scales_t, ctx.dtypes[1])
+                dw = dy.new_empty((N, K), dtype=ctx.dtypes[1])
+                _product(dy_t, dy_scales_t, codes_t, scales_t, dw, N, K, M)
             else:
-                dw = torch.zeros(N, K, dtype=ctx.dtypes[1], device=dy.device)
+                dw = dy.new_zeros((N, K), dtype=ctx.dtypes[1])
         if w_codes is not None:
-            dx = block_matmul(codes, scales, w_codes, w_scales, ctx.dtypes[0]).view(ctx.x_shape)
+            dx = dy.new_empty(ctx.x_shape, dtype=ctx.dtypes[0])
+            if M:
+                _product(codes, scales, w_codes, w_scales, dx, M, K, N)
         return *once("block_linear", dx, dw), None, None
 
 

@@ -54,15 +54,15 @@ def quantize_rows(x, scale_dtype=torch.float8_e8m0fnu, transposed=False):
     capi.require(not transposed or x.dim() == 2, "x must be [M, K] to be transposed")
     lib = _lib()
     x = x.detach()
-    lead, device = x.shape[:-1], x.device
+    lead = x.shape[:-1]
     x, M, K, stride = e4m3.rows_of(x)
-    codes, pitch = e4m3.new_codes(lead, K, device)
-    scales = e4m3.new_scales(lead, K, scale_dtype, device)
+    codes, pitch = e4m3.new_codes(x, lead, K)
+    scales = e4m3.new_scales(x, lead, K, scale_dtype)
     codes_t = scales_t = None
     pitch_t = 0
     if transposed:
-        codes_t, pitch_t = e4m3.new_codes((K,), M, device)
-        scales_t = e4m3.new_scales((K,), M, scale_dtype, device)
+        codes_t, pitch_t = e4m3.new_codes(x, (K,), M)
+        scales_t = e4m3.new_scales(x, (K,), M, scale_dtype)
     st = capi.launch(lib.block_quant_rows, x.get_device(), x.data_ptr(), e4m3.DTYPES[x.dtype],
                      stride, codes.data_ptr(), pitch, scales.data_ptr(),
                      codes_t.data_ptr() if transposed else 0, pitch_t,
@@ -84,9 +84,9 @@ def quantize_tiles(w, scale_dtype=torch.float8_e8m0fnu, transposed=False):
     capi.require(w.dim() == 2 and w.size(1) >= 1, "w must be [N, K] with K >= 1")
     lib = _lib()
     w, N, K, stride = e4m3.rows_of(w.detach())
-    codes, pitch = e4m3.new_codes((N,), K, w.device)
-    scales = torch.empty((e4m3.blocks(N), e4m3.blocks(K)), dtype=scale_dtype, device=w.device)
-    codes_t, pitch_t = e4m3.new_codes((K,), N, w.device) if transposed else (None, 0)
+    codes, pitch = e4m3.new_codes(w, (N,), K)
+    scales = w.new_empty((e4m3.blocks(N), e4m3.blocks(K)), dtype=scale_dtype)
+    codes_t, pitch_t = e4m3.new_codes(w, (K,), N) if transposed else (None, 0)
     st = capi.launch(lib.block_quant_tiles, w.get_device(), w.data_ptr(), e4m3.DTYPES[w.dtype],
                      stride, codes.data_ptr(), pitch, scales.data_ptr(),
                      codes_t.data_ptr() if transposed else 0, pitch_t, e4m3.SCALES[scale_dtype],

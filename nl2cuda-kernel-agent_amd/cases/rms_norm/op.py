@@ -44,26 +44,29 @@ def _workspace_bytes(rows, D):
 
 
 def _check(x, weight, residual):
-    capi.require(x.is_cuda and weight.is_cuda and (residual is None or residual.is_cuda),
-                 "x, weight and residual must be GPU tensors")
     device = x.get_device()
+    capi.require(device >= 0 and weight.is_cuda and (residual is None or residual.is_cuda),
+                 "x, weight and residual must be GPU tensors")
     capi.require(weight.get_device() == device and
                  (residual is None or residual.get_device() == device),
                  "weight and residual must be on the GPU of x")
     capi.require(x.dtype in e4m3.DTYPES and weight.dtype in e4m3.DTYPES,
                  "x and weight must be float32, bfloat16 or float16")
-    capi.require(x.dim() >= 1 and x.size(-1) >= 1 and weight.shape == x.shape[-1:],
+    shape = x.shape
+    capi.require(len(shape) >= 1 and shape[-1] >= 1 and weight.shape == shape[-1:],
                  "x must be [..., D] with D >= 1 and weight [D]")
-    capi.require(residual is None or residual.shape == x.shape and
+    capi.require(residual is None or residual.shape == shape and
                  residual.dtype in (x.dtype, torch.float32),
                  "residual must have x's shape, and its type or float32")
+    return device
 
 
 def _inputs(x, weight, residual):
     """What the C entries take of x, the residual and the weight, the tensors that they read, and
     the rows."""
     x, rows, D, stride = e4m3.rows_of(x)
-    weight = weight.contiguous()
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
     if residual is None:
         r, r_ptr, r_type, r_stride = None, 0, 0, 0
     else:
@@ -73,15 +76,22 @@ def _inputs(x, weight, residual):
              weight.data_ptr(), e4m3.DTYPES[weight.dtype]), (x, weight, r), rows, D)
 
 
+def _like(t, shape, dtype):
+    """A dense tensor beside t."""
+    if t.is_contiguous() and t.dtype == dtype and t.shape == shape:
+        return torch.empty_like(t)
+    return t.new_empty(shape, dtype=dtype)
+
+
 def _forward(x, weight, residual, eps, keep):
     """(y, h or None, rstd or None, weight as read)."""
-    _check(x, weight, residual)
+    device = _check(x, weight, residual)
     lib = _lib()
     args, held, rows, D = _inputs(x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
-    st = capi.launch(lib.rms_norm_forward, x.get_device(), *args, y.data_ptr(),
+    y = _like(x, x.shape, x.dtype)
+    h = None if residual is None else _like(residual, x.shape, residual.dtype)
+    rstd = x.new_empty(rows, dtype=torch.float32) if keep else None
+    st = capi.launch(lib.rms_norm_forward, device, *args, y.data_ptr(),
                      0 if h is None else h.data_ptr(), rstd.data_ptr() if keep else 0, rows, D,
                      eps)
     if st:
@@ -98,25 +108,29 @@ def _backward(dy, dh, h, weight, rstd, dtype, want_weight):
     capi.require(0 <= device == weight.get_device() == rstd.get_device() and
                  weight.numel() == D and rstd.numel() == rows,
                  "autograd gave back other tensors than were saved")
-    weight, rstd = weight.contiguous(), rstd.contiguous()
-    dx = torch.empty(shape, dtype=dtype, device=h.device)
-    dres = dx if h.dtype == dtype else torch.empty(shape, dtype=h.dtype, device=h.device)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    if not rstd.is_contiguous():
+        rstd = rstd.contiguous()
     dy, _, _, dy_stride = e4m3.rows_of(dy)
     dh_ptr = dh_stride = 0
     if dh is not None:
         dh, _, _, dh_stride = e4m3.rows_of(dh)
         dh_ptr = dh.data_ptr()
-    dw = ws = None
-    ws_bytes = 0
+    dx = _like(dy, shape, dtype)
+    dres = dx if h.dtype == dtype else _like(h, shape, h.dtype)
+    dw_ptr = ws_ptr = ws_bytes = 0
+    dw = None
     if want_weight:
-        dw = torch.empty(D, dtype=weight.dtype, device=h.device)
+        dw = torch.empty_like(weight)
         ws_bytes = _workspace_bytes(rows, D)
-        ws = torch.empty(max(ws_bytes, 16) // 4, dtype=torch.float32, device=h.device)
-    st = capi.launch(lib.rms_norm_backward, device, dy.data_ptr(), e4m3.DTYPES[dtype], dy_stride,
-                     h.data_ptr(), e4m3.DTYPES[h.dtype], h_stride, dh_ptr, dh_stride,
-                     weight.data_ptr(), e4m3.DTYPES[weight.dtype], rstd.data_ptr(), dx.data_ptr(),
-                     0 if dres is dx else dres.data_ptr(), dw.data_ptr() if want_weight else 0,
-                     rows, D, ws.data_ptr() if want_weight else 0, ws_bytes)
+        ws = rstd.new_empty(max(ws_bytes, 16) // 4)
+        dw_ptr, ws_ptr = dw.data_ptr(), ws.data_ptr()
+    types = e4m3.DTYPES
+    st = capi.launch(lib.rms_norm_backward, device, dy.data_ptr(), types[dtype], dy_stride,
+                     h.data_ptr(), types[h.dtype], h_stride, dh_ptr, dh_stride, weight.data_ptr(),
+                     types[weight.dtype], rstd.data_ptr(), dx.data_ptr(),
+                     0 if dres is dx else dres.data_ptr(), dw_ptr, rows, D, ws_ptr, ws_bytes)
     if st:
         capi.check(st, lib.rms_norm_last_error, "rms_norm backward")
     return dx, dres, dw
@@ -164,14 +178,16 @@ def rms_norm_quantized(x, weight, residual=None, eps=1e-6, scale_dtype=torch.flo
     inputs that need a gradient are refused."""
     capi.require(not differentiated(x, weight, residual),
                  "rms_norm_quantized has no gradient: use rms_norm, or torch.no_grad()")
-    _check(x, weight, residual)
+    device = _check(x, weight, residual)
     e4m3.require_scales(scale_dtype)
     lib = _lib()
     args, held, rows, D = _inputs(x, weight, residual)
-    codes, pitch = e4m3.new_codes(x.shape[:-1], D, x.device)
-    scales = e4m3.new_scales(x.shape[:-1], D, scale_dtype, x.device)
-    h = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    st = capi.launch(lib.rms_norm_quant, x.get_device(), *args, codes.data_ptr(), pitch,
+    shape = x.shape
+    lead = shape[:-1]
+    codes, pitch = e4m3.new_codes(x, lead, D)
+    scales = e4m3.new_scales(x, lead, D, scale_dtype)
+    h = None if residual is None else _like(residual, shape, residual.dtype)
+    st = capi.launch(lib.rms_norm_quant, device, *args, codes.data_ptr(), pitch,
                      scales.data_ptr(), e4m3.SCALES[scale_dtype], 0 if h is None else h.data_ptr(),
                      rows, D, eps)
     if st:

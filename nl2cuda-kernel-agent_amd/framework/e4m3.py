@@ -30,26 +30,24 @@ def pitch(n):
     return (n + 15) // 16 * 16
 
 
-def new_codes(lead, n, device):
-    """Codes [*lead, n] and the bytes between their rows."""
-    p = pitch(n)
-    codes = torch.empty((*lead, p), dtype=CODES, device=device)
+def new_codes(like, lead, n):
+    """Codes [*lead, n] on the GPU of ``like``, and the bytes between their rows."""
+    p = (n + 15) // 16 * 16
+    codes = like.new_empty((*lead, p), dtype=CODES)
     return (codes if p == n else codes[..., :n]), p
 
 
-def new_scales(lead, n, dtype, device):
+def new_scales(like, lead, n, dtype):
     """Scales of rows of n numbers, [*lead, blocks]."""
-    scales = torch.empty((blocks(n), *lead), dtype=dtype, device=device)
+    scales = like.new_empty(((n + 127) // 128, *lead), dtype=dtype)
     return scales.t() if len(lead) == 1 else scales.movedim(0, -1)
 
 
 def rows_of(x):
     """(x, rows, numbers a row, numbers between rows) with dense rows, copied only if it must be."""
-    D, d = x.size(-1), x.dim()
-    dense = D == 1 or x.stride(-1) == 1
-    if d == 2 and dense and x.stride(0) >= 0:
-        return x, x.size(0), D, x.stride(0)
-    if d == 1 and dense:
-        return x, 1, D, D
-    x = x.contiguous()
-    return x, x.numel() // D if D else 0, D, D
+    D = x.shape[-1]
+    if not x.is_contiguous():
+        if x.dim() == 2 and (D == 1 or x.stride(1) == 1):
+            return x, x.shape[0], D, x.stride(0)
+        x = x.contiguous()
+    return x, x.numel() // D, D, D

@@ -7,17 +7,19 @@ refused where somebody goes on to take it.
 """
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 
 def differentiated(*tensors):
     """Whether a call goes through its autograd function: where an input needs a
     gradient, and where one carries a tangent, which is refused there."""
-    for t in tensors:
-        if t is not None and (t.requires_grad and torch.is_grad_enabled() or
-                              unpack_dual(t).tangent is not None):
-            return True
-    return False
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", 0) < 0:    # no tangents anywhere
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Once(torch.autograd.Function):
