@@ -49,6 +49,41 @@ int block_matmul(const void* a, int64_t a_pitch, const void* a_scales, int64_t a
                  int scale_type, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
                  void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/*
+ * A layer of it: y = Q(x) Q(w)^T, dx = Q(dy) Q(w), dw = Q(dy^T) Q(x^T)^T, where
+ * Q quantises x, dy and their transposes by rows and w [N, K] by tiles, as
+ * block_quant.h describes.  x, dy, w, y, dx, dw: types 0, 1, 2 as above; rows of
+ * x, dy and w a stride in numbers apart, written arrays dense, y and dx of x's
+ * type.  w_codes, where not NULL, is w quantised already (w is not read then),
+ * with its pitch, and scales of tiles at w_row_stride, w_block_stride; the
+ * backward takes the transposed matrix's, [K, N].
+ *
+ * What a backward needs is kept by the forward in `kept`, 256-byte aligned, of
+ * block_linear_kept_bytes: for dx the transposed w (unless w_codes is given),
+ * for dw the transposed x.  M = 0 does nothing; dw is the caller's to clear.
+ */
+size_t block_linear_kept_bytes(int64_t M, int64_t N, int64_t K, int scale_type, int want_dx,
+                               int want_dw, int have_codes);
+
+/* Bytes of scratch, 256-byte aligned, of the forward (backward 0; x's type) or
+ * the backward (1; w's type); 0 for sizes that the call refuses. */
+size_t block_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype,
+                                    int w_dtype, int backward);
+
+int block_linear_forward(const void* x, int x_dtype, int64_t x_stride, const void* w, int w_dtype,
+                         int64_t w_stride, const void* w_codes, int64_t w_pitch,
+                         const void* w_scales, int64_t w_row_stride, int64_t w_block_stride,
+                         int scale_type, int want_dx, int want_dw, void* y, void* kept, int64_t M,
+                         int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                         hipStream_t stream);
+
+/* dx or dw NULL: not wanted (as the forward was told). */
+int block_linear_backward(const void* dy, int x_dtype, int64_t dy_stride, const void* w_codes_t,
+                          int64_t w_pitch_t, const void* w_scales_t, int64_t w_row_stride_t,
+                          int64_t w_block_stride_t, int scale_type, const void* kept, void* dx,
+                          void* dw, int w_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                          size_t workspace_bytes, hipStream_t stream);
+
 const char* block_matmul_last_error(void);
 
 #ifdef __cplusplus

@@ -23,6 +23,7 @@
 
 #include "e4m3.h"
 #include "lds_direct.h"
+#include "quantize.h"
 
 namespace {
 
@@ -894,6 +895,208 @@ extern "C" int block_matmul(const void* a, int64_t a_pitch, const void* a_scales
   if (b_tiles)
     return full ? launch<kTiles, true>(g, p, stream) : launch<kTiles, false>(g, p, stream);
   return full ? launch<kRows, true>(g, p, stream) : launch<kRows, false>(g, p, stream);
+}
+
+namespace {
+
+// Where a layer's matrices lie in scratch: codes, then scales, each from a multiple of 256 bytes on.
+struct Place {
+  size_t codes, scales;
+  int64_t pitch, row, block;  // of codes in bytes, of scales in numbers
+};
+
+struct Scratch {
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+  // of rows' blocks, scales blocks first
+  Place rows(int64_t m, int64_t k, int scale_type) {
+    Place p{};
+    p.pitch = nl2k::ceil_div(k, 16) * 16;
+    p.codes = take((size_t)m * p.pitch);
+    p.scales = take((size_t)nl2k::ceil_div(k, kBlock) * m * scale_bytes(scale_type));
+    p.row = 1, p.block = m;
+    return p;
+  }
+};
+
+// What the forward keeps: x^T [K, M] for dw, w^T [K, N] and w's scales for dx.
+struct Kept {
+  Place xt, wt;
+  size_t bytes;
+};
+Kept kept_layout(int64_t M, int64_t N, int64_t K, int scale_type, bool dx, bool dw) {
+  Scratch s;
+  Kept k{};
+  if (dw) k.xt = s.rows(K, M, scale_type);
+  if (dx) {
+    k.wt.pitch = nl2k::ceil_div(N, 16) * 16;
+    k.wt.codes = s.take((size_t)K * k.wt.pitch);
+    k.wt.scales = s.take((size_t)nl2k::ceil_div(N, kBlock) * nl2k::ceil_div(K, kBlock) *
+                         scale_bytes(scale_type));
+    k.wt.row = 1, k.wt.block = nl2k::ceil_div(K, kBlock);  // of the transposed matrix's tiles
+  }
+  k.bytes = s.bytes;
+  return k;
+}
+
+struct ForwardScratch {
+  Place x, w;
+  size_t product, bytes;
+};
+ForwardScratch forward_layout(int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype) {
+  Scratch s;
+  ForwardScratch f{};
+  f.x = s.rows(M, K, scale_type);
+  f.w.pitch = nl2k::ceil_div(K, 16) * 16;
+  f.w.codes = s.take((size_t)N * f.w.pitch);
+  f.w.scales = s.take((size_t)nl2k::ceil_div(N, kBlock) * nl2k::ceil_div(K, kBlock) *
+                      scale_bytes(scale_type));
+  f.w.row = nl2k::ceil_div(K, kBlock), f.w.block = 1;
+  f.product = s.take(workspace_of(plan(M, N, K, x_dtype == kF32), M, N));
+  f.bytes = s.bytes;
+  return f;
+}
+
+struct BackwardScratch {
+  Place dy, dyt;
+  size_t product, bytes;
+};
+BackwardScratch backward_layout(int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype,
+                                int w_dtype) {
+  Scratch s;
+  BackwardScratch b{};
+  b.dy = s.rows(M, N, scale_type);
+  b.dyt = s.rows(N, M, scale_type);
+  // one product after the other
+  b.product = s.take(std::max(workspace_of(plan(M, K, N, x_dtype == kF32), M, K),
+                              workspace_of(plan(N, K, M, w_dtype == kF32), N, K)));
+  b.bytes = s.bytes;
+  return b;
+}
+
+int check_layer(const char* who, int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype,
+                int w_dtype) {
+  if (M < 0 || N < 1 || K < 1)
+    return nl2k::fail(NL2K_ERR_SHAPE, "%s: need M >= 0, N, K >= 1 (got %lld, %lld, %lld)", who,
+                      (long long)M, (long long)N, (long long)K);
+  if (M > kLongest || N > kLongest || K > kLongest)
+    return nl2k::fail(NL2K_ERR_OVERFLOW, "%s: sizes too large (M=%lld N=%lld K=%lld)", who,
+                      (long long)M, (long long)N, (long long)K);
+  if (int st = check_sizes(M, N, K)) return st;
+  if (int st = check_sizes(M, K, N)) return st;
+  if (int st = M ? check_sizes(N, K, M) : 0) return st;
+  if (x_dtype < kF32 || x_dtype > kF16 || w_dtype < kF32 || w_dtype > kF16 ||
+      (scale_type != kScaleF32 && scale_type != kScaleE8M0))
+    return nl2k::fail(NL2K_ERR_VALUE, "%s: types must be 0, 1 or 2, scale_type 0 or 1 (got %d, %d, %d)",
+                      who, x_dtype, w_dtype, scale_type);
+  return NL2K_SUCCESS;
+}
+
+int check_scratch(const char* who, const char* name, const void* p, size_t have, size_t need) {
+  if (need && (!p || have < need))
+    return nl2k::fail(NL2K_ERR_WORKSPACE, "%s: %s of %zu bytes is needed (got %zu)", who, name, need,
+                      have);
+  if (reinterpret_cast<uintptr_t>(p) % 256)
+    return nl2k::fail(NL2K_ERR_ALIGN, "%s: %s must be aligned to 256 bytes", who, name);
+  return NL2K_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" size_t block_linear_kept_bytes(int64_t M, int64_t N, int64_t K, int scale_type,
+                                          int want_dx, int want_dw, int have_codes) {
+  if (check_layer("block_linear_kept_bytes", M, N, K, scale_type, 0, 0) || M == 0) return 0;
+  return kept_layout(M, N, K, scale_type, want_dx && !have_codes, want_dw).bytes;
+}
+
+extern "C" size_t block_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int scale_type,
+                                               int x_dtype, int w_dtype, int backward) {
+  if (check_layer("block_linear_workspace_bytes", M, N, K, scale_type, x_dtype, w_dtype) || M == 0)
+    return 0;
+  return backward ? backward_layout(M, N, K, scale_type, x_dtype, w_dtype).bytes
+                  : forward_layout(M, N, K, scale_type, x_dtype).bytes;
+}
+
+extern "C" int block_linear_forward(const void* x, int x_dtype, int64_t x_stride, const void* w,
+                                    int w_dtype, int64_t w_stride, const void* w_codes,
+                                    int64_t w_pitch, const void* w_scales, int64_t w_row_stride,
+                                    int64_t w_block_stride, int scale_type, int want_dx,
+                                    int want_dw, void* y, void* kept, int64_t M, int64_t N,
+                                    int64_t K, void* workspace, size_t workspace_bytes,
+                                    hipStream_t stream) {
+  const char* who = "block_linear_forward";
+  int st = check_layer(who, M, N, K, scale_type, x_dtype, w_dtype);
+  if (st) return st;
+  if (M == 0) return nl2k::succeed();
+  if (!x || !y || (!w && !w_codes) || !w_codes != !w_scales)
+    return nl2k::fail(NL2K_ERR_NULL, "%s: x, y and w, or its codes and scales, are required", who);
+  const ForwardScratch f = forward_layout(M, N, K, scale_type, x_dtype);
+  const bool keep_w = want_dx && !w_codes;
+  const Kept k = kept_layout(M, N, K, scale_type, keep_w, want_dw);
+  if ((st = check_scratch(who, "a workspace", workspace, workspace_bytes, f.bytes))) return st;
+  if ((st = check_scratch(who, "kept", kept, kept ? k.bytes : 0, k.bytes))) return st;
+  char* ws = static_cast<char*>(workspace);
+  char* to = static_cast<char*>(kept);
+  st = nl2k::quant::run(who, x, x_dtype, x_stride, ws + f.x.codes, f.x.pitch, ws + f.x.scales,
+                        want_dw ? to + k.xt.codes : nullptr, k.xt.pitch,
+                        want_dw ? to + k.xt.scales : nullptr, scale_type, M, K, false, stream);
+  if (st) return st;
+  if (!w_codes) {
+    void* scales = keep_w ? to + k.wt.scales : ws + f.w.scales;
+    st = nl2k::quant::run(who, w, w_dtype, w_stride, ws + f.w.codes, f.w.pitch, scales,
+                          keep_w ? to + k.wt.codes : nullptr, k.wt.pitch, nullptr, scale_type, N, K,
+                          true, stream);
+    if (st) return st;
+    w_codes = ws + f.w.codes, w_pitch = f.w.pitch;
+    w_scales = scales, w_row_stride = f.w.row, w_block_stride = f.w.block;
+  }
+  return block_matmul(ws + f.x.codes, f.x.pitch, ws + f.x.scales, f.x.row, f.x.block, 0, w_codes,
+                      w_pitch, w_scales, w_row_stride, w_block_stride, 1, scale_type, y, x_dtype, M,
+                      N, K, ws + f.product, f.bytes - f.product, stream);
+}
+
+extern "C" int block_linear_backward(const void* dy, int x_dtype, int64_t dy_stride,
+                                     const void* w_codes_t, int64_t w_pitch_t,
+                                     const void* w_scales_t, int64_t w_row_stride_t,
+                                     int64_t w_block_stride_t, int scale_type, const void* kept,
+                                     void* dx, void* dw, int w_dtype, int64_t M, int64_t N,
+                                     int64_t K, void* workspace, size_t workspace_bytes,
+                                     hipStream_t stream) {
+  const char* who = "block_linear_backward";
+  int st = check_layer(who, M, N, K, scale_type, x_dtype, w_dtype);
+  if (st) return st;
+  if (M == 0 || (!dx && !dw)) return nl2k::succeed();
+  const bool kept_w = dx && !w_codes_t;
+  if (!dy || !w_codes_t != !w_scales_t || ((kept_w || dw) && !kept))
+    return nl2k::fail(NL2K_ERR_NULL, "%s: dy, and what the forward kept, are required", who);
+  const BackwardScratch b = backward_layout(M, N, K, scale_type, x_dtype, w_dtype);
+  const Kept k = kept_layout(M, N, K, scale_type, kept_w, dw != nullptr);
+  if ((st = check_scratch(who, "a workspace", workspace, workspace_bytes, b.bytes))) return st;
+  if ((st = check_scratch(who, "kept", kept, k.bytes, k.bytes))) return st;
+  char* ws = static_cast<char*>(workspace);
+  const char* from = static_cast<const char*>(kept);
+  st = nl2k::quant::run(who, dy, x_dtype, dy_stride, ws + b.dy.codes, b.dy.pitch, ws + b.dy.scales,
+                        dw ? ws + b.dyt.codes : nullptr, b.dyt.pitch,
+                        dw ? ws + b.dyt.scales : nullptr, scale_type, M, N, false, stream);
+  if (st) return st;
+  if (dw) {
+    st = block_matmul(ws + b.dyt.codes, b.dyt.pitch, ws + b.dyt.scales, b.dyt.row, b.dyt.block, 0,
+                      from + k.xt.codes, k.xt.pitch, from + k.xt.scales, k.xt.row, k.xt.block, 0,
+                      scale_type, dw, w_dtype, N, K, M, ws + b.product, b.bytes - b.product, stream);
+    if (st) return st;
+  }
+  if (!dx) return NL2K_SUCCESS;
+  if (kept_w) {
+    w_codes_t = from + k.wt.codes, w_pitch_t = k.wt.pitch;
+    w_scales_t = from + k.wt.scales, w_row_stride_t = k.wt.row, w_block_stride_t = k.wt.block;
+  }
+  return block_matmul(ws + b.dy.codes, b.dy.pitch, ws + b.dy.scales, b.dy.row, b.dy.block, 0,
+                      w_codes_t, w_pitch_t, w_scales_t, w_row_stride_t, w_block_stride_t, 1,
+                      scale_type, dx, x_dtype, M, K, N, ws + b.product, b.bytes - b.product, stream);
 }
 
 extern "C" const char* block_matmul_last_error(void) { return nl2k::error_slot().text; }

@@ -14,7 +14,7 @@ import os
 
 import torch
 
-from cases.block_quant.op import quantize_rows, quantize_tiles
+from cases.block_quant.op import quantize_tiles
 from framework import capi, e4m3
 from framework.loader import load_kernel
 from framework.once import differentiated, once
@@ -31,6 +31,13 @@ def bind_library(lib):
     V, I64, I, S = capi.c_void_p, capi.c_int64, capi.c_int, capi.c_size_t
     capi.bind(lib, "block_matmul_workspace_bytes", [I64, I64, I64, I], S)
     capi.bind(lib, "block_matmul", [V, I64, V, I64, I64, I] * 2 + [I, V, I, I64, I64, I64, V, S, V])
+    capi.bind(lib, "block_linear_kept_bytes", [I64, I64, I64, I, I, I, I], S)
+    capi.bind(lib, "block_linear_workspace_bytes", [I64, I64, I64, I, I, I, I], S)
+    weight = [V, I64, V, I64, I64]
+    capi.bind(lib, "block_linear_forward",
+              [V, I, I64, V, I, I64] + weight + [I, I, I, V, V, I64, I64, I64, V, S, V])
+    capi.bind(lib, "block_linear_backward",
+              [V, I, I64] + weight + [I, V, V, V, I, I64, I64, I64, V, S, V])
     capi.bind_last_error(lib, "block_matmul_last_error")
     return lib
 
@@ -43,6 +50,16 @@ def _lib():
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(M, N, K, out_dtype):
     return _lib().block_matmul_workspace_bytes(M, N, K, out_dtype)
+
+
+@functools.lru_cache(maxsize=1024)
+def _layer_bytes(M, N, K, scale_type, x_type, w_type, want_x, want_w, have_codes):
+    """(workspace of the forward, of the backward, what is kept between them)."""
+    lib = _lib()
+    sizes = (M, N, K, scale_type)
+    return (lib.block_linear_workspace_bytes(*sizes, x_type, w_type, 0),
+            lib.block_linear_workspace_bytes(*sizes, x_type, w_type, 1),
+            lib.block_linear_kept_bytes(*sizes, want_x, want_w, have_codes))
 
 
 def _codes(c, rows, K):
@@ -143,54 +160,89 @@ def quantize_weight(weight, scale_dtype=torch.float8_e8m0fnu):
     return QuantizedWeight(*quantize_tiles(weight, scale_dtype, transposed=True))
 
 
+def _tiles(codes, scales, rows, n):
+    """A quantised weight, or its transpose, as the C entries take it."""
+    codes, pitch = _codes(codes, rows, n)
+    scales, row, block, _ = _scales("quantized must be quantize_weight's", scales, rows, n)
+    return (codes.data_ptr(), pitch, scales.data_ptr(), row, block), (codes, scales)
+
+
+def _layer_forward(x, weight, quantized, scale_dtype, want_x, want_w):
+    """(y, what the backward needs or None)."""
+    lib = _lib()
+    N, K = weight.shape
+    rows, M, _, x_stride = e4m3.rows_of(x)
+    types = e4m3.DTYPES
+    x_type, w_type, s_type = types[x.dtype], types[weight.dtype], e4m3.SCALES[scale_dtype]
+    y = x.new_empty((*x.shape[:-1], N))
+    if M == 0:
+        return y, None
+    if quantized is None:
+        weight, _, _, w_stride = e4m3.rows_of(weight)
+        w, held = (weight.data_ptr(), w_type, w_stride, 0, 0, 0, 0, 0), weight
+    else:
+        codes, held = _tiles(quantized[0], quantized[1], N, K)
+        w = (0, w_type, 0) + codes
+    ws_bytes, _, kept_bytes = _layer_bytes(M, N, K, s_type, x_type, w_type, want_x, want_w,
+                                           quantized is not None)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    kept = x.new_empty(kept_bytes, dtype=torch.uint8) if kept_bytes else None
+    st = capi.launch(lib.block_linear_forward, x.get_device(), rows.data_ptr(), x_type, x_stride,
+                     *w, s_type, want_x, want_w, y.data_ptr(),
+                     kept.data_ptr() if kept_bytes else 0, M, N, K, ws.data_ptr(), ws_bytes)
+    if st:
+        capi.check(st, lib.block_matmul_last_error, "block_linear")
+    return y, kept
+
+
 class BlockLinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, quantized, scale_dtype):
-        want_x, want_w = ctx.needs_input_grad[:2]
-        N, K = weight.shape
-        rows = x if x.dim() == 2 else x.reshape(-1, K)
-        M = rows.shape[0]
-        if want_w:
-            codes, scales, codes_t, scales_t = quantize_rows(rows, scale_dtype, transposed=True)
-        else:
-            codes, scales, codes_t, scales_t = *quantize_rows(rows, scale_dtype), None, None
-        if quantized is None:
-            quantized = quantize_tiles(weight, scale_dtype, transposed=want_x)
-        y = x.new_empty((*x.shape[:-1], N))
-        if M:
-            _product(codes, scales, quantized[0], quantized[1], y, M, N, K)
+        ctx.want = ctx.needs_input_grad[:2]
+        y, kept = _layer_forward(x, weight, quantized, scale_dtype, *ctx.want)
         ctx.scale_dtype, ctx.dtypes = scale_dtype, (x.dtype, weight.dtype)
         ctx.x_shape, ctx.w_shape = x.shape, weight.shape
-        ctx.save_for_backward(codes_t, scales_t, *(quantized[2:] if want_x else (None, None)))
+        ctx.quantized = quantized is not None
+        ctx.save_for_backward(kept, *(quantized[2:] if ctx.quantized and ctx.want[0] else ()))
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        codes_t, scales_t, w_codes, w_scales = ctx.saved_tensors
+        kept, *codes_t = ctx.saved_tensors
+        want_x, want_w = ctx.want
         N, K = ctx.w_shape
-        if dy.dim() != 2:
-            dy = dy.reshape(-1, N)
-        M, device = dy.shape[0], dy.get_device()
+        dy, M, _, dy_stride = e4m3.rows_of(dy)
+        dx = dy.new_empty(ctx.x_shape, dtype=ctx.dtypes[0]) if want_x else None
+        if M == 0:
+            dw = dy.new_zeros((N, K), dtype=ctx.dtypes[1]) if want_w else None
+            return *once("block_linear", dx, dw), None, None
+        lib, device = _lib(), dy.get_device()
+        types = e4m3.DTYPES
+        x_type, w_type = types[ctx.dtypes[0]], types[ctx.dtypes[1]]
+        s_type = e4m3.SCALES[ctx.scale_dtype]
+        _, ws_bytes, kept_bytes = _layer_bytes(M, N, K, s_type, x_type, w_type, want_x, want_w,
+                                               ctx.quantized)
         # what autograd gives back of what was saved: every read lies within it
-        for codes, scales, n in ((codes_t, scales_t, M), (w_codes, w_scales, N)):
-            capi.require(codes is None or codes.shape == (K, n) and
-                         codes.dtype == e4m3.CODES and scales.dtype == ctx.scale_dtype and
-                         codes.get_device() == device == scales.get_device(),
-                         "autograd gave back other tensors than were saved")
-        dx = dw = None
-        if codes_t is None:
-            codes, scales = quantize_rows(dy, ctx.scale_dtype)
-        else:
-            codes, scales, dy_t, dy_scales_t = quantize_rows(dy, ctx.scale_dtype, transposed=True)
-            if M:
-                dw = dy.new_empty((N, K), dtype=ctx.dtypes[1])
-                _product(dy_t, dy_scales_t, codes_t, scales_t, dw, N, K, M)
-            else:
-                dw = dy.new_zeros((N, K), dtype=ctx.dtypes[1])
-        if w_codes is not None:
-            dx = dy.new_empty(ctx.x_shape, dtype=ctx.dtypes[0])
-            if M:
-                _product(codes, scales, w_codes, w_scales, dx, M, K, N)
+        message = "autograd gave back other tensors than were saved"
+        if kept_bytes:
+            capi.require(kept.get_device() == device and kept.dtype == torch.uint8 and
+                         kept.numel() == kept_bytes, message)
+            kept = kept.contiguous()
+        w = (0, 0, 0, 0, 0)
+        if codes_t:
+            codes_t, scales_t = codes_t
+            capi.require(codes_t.shape == (K, N) and codes_t.dtype == e4m3.CODES and
+                         scales_t.dtype == ctx.scale_dtype and
+                         codes_t.get_device() == device == scales_t.get_device(), message)
+            w, held = _tiles(codes_t, scales_t, K, N)
+        dw = dy.new_empty((N, K), dtype=ctx.dtypes[1]) if want_w else None
+        ws = dy.new_empty(ws_bytes, dtype=torch.uint8)
+        st = capi.launch(lib.block_linear_backward, device, dy.data_ptr(), x_type, dy_stride, *w,
+                         s_type, kept.data_ptr() if kept_bytes else 0,
+                         dx.data_ptr() if want_x else 0, dw.data_ptr() if want_w else 0, w_type, M,
+                         N, K, ws.data_ptr(), ws_bytes)
+        if st:
+            capi.check(st, lib.block_matmul_last_error, "block_linear backward")
         return *once("block_linear", dx, dw), None, None
 
 
@@ -206,24 +258,25 @@ def block_linear(x, weight, quantized=None, scale_dtype=torch.float8_e8m0fnu):
     dweight come in x's and the weight's type.  Differentiable once and in
     reverse.  quantized: what ``quantize_weight`` gave for this weight.
     """
-    capi.require(x.is_cuda and weight.is_cuda and x.get_device() == weight.get_device(),
+    device = x.get_device()
+    capi.require(device >= 0 and device == weight.get_device(),
                  "x and weight must be GPU tensors on one GPU")
     capi.require(x.dtype in e4m3.DTYPES and weight.dtype in e4m3.DTYPES,
                  "x and weight must be float32, bfloat16 or float16")
-    capi.require(x.dim() >= 1 and weight.dim() == 2 and x.size(-1) == weight.size(1) >= 1 and
-                 weight.size(0) >= 1, "x must be [..., K] and weight [N, K] with N, K >= 1")
+    capi.require(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] >= 1 and
+                 weight.shape[0] >= 1, "x must be [..., K] and weight [N, K] with N, K >= 1")
     e4m3.require_scales(scale_dtype)
     if quantized is not None:
-        capi.require(quantized[0].shape == weight.shape and
-                     quantized[2].shape == weight.shape[::-1] and
-                     quantized[1].dtype == scale_dtype,
-                     "quantized must be quantize_weight's, of this weight and scale_dtype")
+        N, K = weight.shape
+        for codes, scales, shape in ((*quantized[:2], (N, K)), (*quantized[2:], (K, N))):
+            capi.require(codes.shape == shape and codes.dtype == e4m3.CODES and
+                         scales.shape == (e4m3.blocks(shape[0]), e4m3.blocks(shape[1])) and
+                         scales.dtype == scale_dtype and
+                         codes.get_device() == device == scales.get_device(),
+                         "quantized must be quantize_weight's, of this weight and scale_dtype")
     if differentiated(x, weight):
         return BlockLinearFunction.apply(x, weight, quantized, scale_dtype)
-    codes, scales = quantize_rows(x, scale_dtype)
-    if quantized is None:
-        quantized = quantize_tiles(weight, scale_dtype)
-    return block_matmul(codes, scales, quantized[0], quantized[1], x.dtype)
+    return _layer_forward(x.detach(), weight.detach(), quantized, scale_dtype, False, False)[0]
 
 
 def candidate(inputs, params):
