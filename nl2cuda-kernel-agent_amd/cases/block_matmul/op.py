@@ -232,6 +232,7 @@ class BlockLinearFunction(torch.autograd.Function):
         if codes_t:
             codes_t, scales_t = codes_t
             capi.require(codes_t.shape == (K, N) and codes_t.dtype == e4m3.CODES and
+                         scales_t.shape == (e4m3.blocks(K), e4m3.blocks(N)) and
                          scales_t.dtype == ctx.scale_dtype and
                          codes_t.get_device() == device == scales_t.get_device(), message)
             w, held = _tiles(codes_t, scales_t, K, N)
