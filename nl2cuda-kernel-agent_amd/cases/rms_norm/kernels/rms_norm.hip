@@ -4,6 +4,12 @@
 // A lane holds windows of eight numbers of a row, so that 16 lanes next to each
 // other hold a block of 128; a wave, a workgroup of 256 or one of 1024 takes a
 // row, which stays in registers from its sum of squares to its result.
+//
+// Bound by memory.  Measured with bfloat16 rows and a residual of the same type, where a large copy
+// reaches 5.1 TB/s: 8192 x 4096 forward 47.0 us (5.7 TB/s of what it has to read and write),
+// quantised 44.9 (5.2), backward 43.1 with dweight's second kernel (6.2); 4096 x 2048 11.7, 11.8 and
+// 15.7; 16 x 4096 2.7, 3.1 and 5.3, which is a launch's latency and a few loads' (the backward has two
+// launches).
 
 #include "rms_norm.h"
 
@@ -80,9 +86,9 @@ __device__ __forceinline__ void sum8(const Raw<T>& x, const Raw<R>& r, float (&h
   }
 }
 
-// y of a window at column k, from its h.
+// y of a window at column k, from its h, of which `count` lie in the row.
 template <class T, bool kCodes>
-__device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, float rstd,
+__device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, int count, float rstd,
                                         float (&v)[8], const float (&w)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = v[e] * rstd * w[e];
@@ -90,10 +96,10 @@ __device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, fl
     const float top = nl2k::row16_max_dpp(magnitude(v));
     const Scale s =
         f.scale_type == kScaleF32 ? scale_of<kScaleF32>(top) : scale_of<kScaleE8M0>(top);
-    if (k < (f.D + 15) / 16 * 16)
+    if (count > 0 || k < (f.D + 15) / 16 * 16)
       *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(f.y) + row * f.pitch + k) =
           pack8(v, s.inverse);
-    if ((threadIdx.x & 15) == 0 && k < f.D) {
+    if ((threadIdx.x & 15) == 0 && count > 0) {
       const int64_t at = (int64_t)(k / kBlock) * f.rows + row;
       if (f.scale_type == kScaleF32)
         keep<kScaleF32>(f.scales, at, s.kept);
@@ -101,11 +107,16 @@ __device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, fl
         keep<kScaleE8M0>(f.scales, at, s.kept);
     }
   } else {
-    store8<T>(static_cast<typename Elem<T>::type*>(f.y) + row * f.D + k, f.D - k, v);
+    store8<T>(static_cast<typename Elem<T>::type*>(f.y) + row * f.D + k, count, v);
   }
 }
 
-template <class T, class R, bool kRes, bool kCodes, int TPR, int U>
+// h = round(x + residual), y = h rstd weight with rstd = (mean(h^2) + eps)^(-1/2); all in 32 bits but
+// for h, whose rounding to the residual's type is part of the function: a next layer reads that h.
+//
+// kWhole: rows are all of the windows, and nothing needs to ask where one ends, which saves a branch
+// a load: 8192 x 4096 51.2 -> 47.8 us, 4096 x 2048 13.3 -> 11.7, its backward 16.6 -> 15.6.
+template <class T, class R, bool kRes, bool kCodes, int TPR, int U, bool kWhole>
 __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(Forward f) {
   __shared__ float red[TPR / 64];
   const int64_t row = row_in<TPR>(blockIdx.x);
@@ -113,19 +124,20 @@ __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(Forward f) {
   const int lane = lane_in<TPR>();
   const auto* x = static_cast<const typename Elem<T>::type*>(f.x) + row * f.x_stride;
   const auto* res = static_cast<const typename Elem<R>::type*>(f.residual) + row * f.r_stride;
+  auto count = [&](int k) { return kWhole ? 8 : f.D - k; };
   Raw<T> xr[U];
   Raw<R> rr[kRes ? U : 1];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int k = (u * TPR + lane) * 8;
-    xr[u] = load8<T>(x + k, f.D - k);
-    if constexpr (kRes) rr[u] = load8<R>(res + k, f.D - k);
+    xr[u] = load8<T>(x + k, count(k));
+    if constexpr (kRes) rr[u] = load8<R>(res + k, count(k));
   }
   float w[U][8];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int k = (u * TPR + lane) * 8;
-    weights8(f.weight, f.w_dtype, k, f.D - k, w[u]);
+    weights8(f.weight, f.w_dtype, k, count(k), w[u]);
   }
   float h[U][8], sum = 0.f;
 #pragma unroll
@@ -133,18 +145,20 @@ __global__ __launch_bounds__(block_of<TPR>()) void forward_kernel(Forward f) {
     const int k = (u * TPR + lane) * 8;
     sum8<T, R, kRes>(xr[u], rr[kRes ? u : 0], h[u]);
     if constexpr (kRes)
-      store8<R>(static_cast<typename Elem<R>::type*>(f.h) + row * f.D + k, f.D - k, h[u]);
+      store8<R>(static_cast<typename Elem<R>::type*>(f.h) + row * f.D + k, count(k), h[u]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = fmaf(h[u][e], h[u][e], sum);
   }
   const float rstd = 1.f / sqrtf(row_sum<TPR>(sum, red) / (float)f.D + f.eps);
   if (f.rstd && lane == 0) f.rstd[row] = rstd;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    finish8<T, kCodes>(f, row, (u * TPR + lane) * 8, rstd, h[u], w[u]);
+  for (int u = 0; u < U; ++u) {
+    const int k = (u * TPR + lane) * 8;
+    finish8<T, kCodes>(f, row, k, count(k), rstd, h[u], w[u]);
+  }
 }
 
-// Rows that registers do not hold: read again for the result.
+// Rows that registers do not hold, above 32768: read again for the result, mostly from the caches.
 template <class T, class R, bool kRes, bool kCodes>
 __global__ __launch_bounds__(1024) void forward_long_kernel(Forward f) {
   __shared__ float red[16];
@@ -175,7 +189,7 @@ __global__ __launch_bounds__(1024) void forward_long_kernel(Forward f) {
     load(k, h);
     weights8(f.weight, f.w_dtype, k, f.D - k, w);
     if constexpr (kRes) store8<R>(hs + k, f.D - k, h);
-    finish8<T, kCodes>(f, row, k, rstd, h, w);
+    finish8<T, kCodes>(f, row, k, f.D - k, rstd, h, w);
   }
 }
 
@@ -195,29 +209,36 @@ struct Backward {
 
 // dx of a window, stored; u = h r in place of h, d = dy.
 template <class T, class R>
-__device__ __forceinline__ void gradient8(const Backward& b, int64_t row, int k, float rstd,
-                                          float mean, const float (&u)[8], const float (&d)[8],
+__device__ __forceinline__ void gradient8(const Backward& b, int64_t row, int k, int count,
+                                          float rstd, float mean, const float (&u)[8], const float (&d)[8],
                                           const float (&w)[8], const Raw<R>& dh) {
   float v[8], add[8];
   values<R>(dh, add);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = fmaf(rstd, d[e] * w[e] - u[e] * mean, add[e]);
-  if (b.dx) store8<T>(static_cast<typename Elem<T>::type*>(b.dx) + row * b.D + k, b.D - k, v);
-  if (b.dres) store8<R>(static_cast<typename Elem<R>::type*>(b.dres) + row * b.D + k, b.D - k, v);
+  if (b.dx) store8<T>(static_cast<typename Elem<T>::type*>(b.dx) + row * b.D + k, count, v);
+  if (b.dres) store8<R>(static_cast<typename Elem<R>::type*>(b.dres) + row * b.D + k, count, v);
 }
 
-// A workgroup takes every gridDim.x-th row (or four), and adds up their share of dweight.
-template <class T, class R, int TPR, int U>
+// With d = dy, u = h rstd and c = mean(d weight u) over the row:
+//   dx = dresidual = rstd (d weight - u c) + dh,  dweight = sum over rows of d u.
+// A workgroup takes every gridDim.x-th row (or four), and adds up their share of dweight in registers;
+// columns_kernel adds the workgroups' shares, so that no atomics are needed and the order is fixed.
+// dh and rows' ends are asked for before they are loaded, not masked out of a load: without a
+// residual 16384 x 2048 56 -> 47 us, 65536 x 256 49 -> 34.  Loading the next row ahead gave nothing,
+// since the other workgroups of a CU cover the wait.
+template <class T, class R, int TPR, int U, bool kWhole>
 __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(Backward b) {
   constexpr int kRows = block_of<TPR>() / TPR;
   __shared__ float red[TPR / 64];
   __shared__ float shared_dw[kRows > 1 ? TPR * U * 8 : 1];
   const int lane = lane_in<TPR>();
+  auto count = [&](int k) { return kWhole ? 8 : b.D - k; };
   float w[U][8], dw[U][8];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int k = (u * TPR + lane) * 8;
-    weights8(b.weight, b.w_dtype, k, b.D - k, w[u]);
+    weights8(b.weight, b.w_dtype, k, count(k), w[u]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[u][e] = 0.f;
   }
@@ -230,9 +251,10 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(Backward b) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = (u * TPR + lane) * 8;
-      dr[u] = load8<T>(dy + k, b.D - k);
-      hr[u] = load8<R>(h + k, b.D - k);
-      ar[u] = load8<R>(dh + k, b.dh ? b.D - k : 0);
+      dr[u] = load8<T>(dy + k, count(k));
+      hr[u] = load8<R>(h + k, count(k));
+      ar[u] = Raw<R>{};
+      if (b.dh) ar[u] = load8<R>(dh + k, count(k));
     }
     const float rstd = b.rstd[row];
     float sum = 0.f;
@@ -256,7 +278,8 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(Backward b) {
       values<R>(hr[u], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= rstd;
-      gradient8<T, R>(b, row, (u * TPR + lane) * 8, rstd, mean, v, d, w[u], ar[u]);
+      const int k = (u * TPR + lane) * 8;
+      gradient8<T, R>(b, row, k, count(k), rstd, mean, v, d, w[u], ar[u]);
     }
   }
   if (!b.partial) return;
@@ -278,10 +301,12 @@ __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(Backward b) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int k = (u * TPR + lane) * 8;
-    store8<float>(b.partial + (int64_t)blockIdx.x * b.D + k, b.D - k, dw[u]);
+    store8<float>(b.partial + (int64_t)blockIdx.x * b.D + k, count(k), dw[u]);
   }
 }
 
+// Rows above 16384, whose share of dweight registers do not hold: in the workgroup's own row of the
+// workspace, added to at each of its rows; 1024 x 32768 103 us (2.6 TB/s of what the others move).
 template <class T, class R>
 __global__ __launch_bounds__(1024) void backward_long_kernel(Backward b) {
   __shared__ float red[16];
@@ -318,7 +343,9 @@ __global__ __launch_bounds__(1024) void backward_long_kernel(Backward b) {
         for (int e = 0; e < 8; ++e) p[e] = fmaf(d[e], v[e], p[e]);
         store8<float>(mine + k, b.D - k, p);
       }
-      gradient8<T, R>(b, row, k, rstd, mean, v, d, w, load8<R>(dh + k, b.dh ? b.D - k : 0));
+      Raw<R> add{};
+      if (b.dh) add = load8<R>(dh + k, b.D - k);
+      gradient8<T, R>(b, row, k, b.D - k, rstd, mean, v, d, w, add);
     }
     first = false;
   }
@@ -349,7 +376,14 @@ __global__ __launch_bounds__(256) void columns_kernel(const float* __restrict__ 
   }
 }
 
-// Threads a row and windows a thread for a row of D numbers.
+// Threads a row and windows a thread for a row of D numbers.  The fewest threads that hold a row lose
+// least to its sum, more of them have more loads in the air.  bfloat16 with a residual, forward and
+// backward in us, against the neighbour that also holds the row:
+//   1024: {64, 2} 47.2, 42.5 (32768 rows);   {256, 1} 52.4, 81.7
+//   2048: {256, 1} 11.7, 15.7 (4096 rows);   {64, 4} 12.8, 16.8
+//   4096: {256, 2} 47.0, 43.1 (8192 rows);   {1024, 1} 52.3, 56.2
+//   8192: {1024, 1} 21.8, 24.5 (2048 rows);  {256, 4} 23.0, 28.0
+//   16384: {1024, 2} 50.0, 51.2 (2048 rows); {256, 8} 52.7, 68.0
 struct Plan {
   int tpr, u;
 };
@@ -360,16 +394,18 @@ Plan plan(int64_t D) {
   if (n <= 128) return {64, 2};
   if (n <= 256) return {256, 1};
   if (n <= 512) return {256, 2};
-  if (n <= 1024) return {256, 4};
+  if (n <= 1024) return {1024, 1};
   if (n <= 2048) return {1024, 2};
   if (n <= 4096) return {1024, 4};
   return {0, 0};
 }
 
-// Workgroups of a backward.
+// Workgroups of a backward: each has a row of the workspace that the second kernel reads, and must be
+// enough of them to have the memory busy.  Rows of up to 256 numbers leave most of a wave's lanes idle:
+// 65536 x 256 33.6 us with 512 workgroups, 27.8 with 1024, where 32768 x 1024 has 43 either way.
 int64_t backward_blocks(int64_t rows, int64_t D) {
   const Plan p = plan(D);
-  const int64_t most = p.tpr == 1024 || p.tpr == 0 ? 256 : 512;
+  const int64_t most = p.tpr == 1024 || p.tpr == 0 ? 256 : D <= 256 ? 1024 : 512;
   return std::min(p.tpr == 64 ? nl2k::ceil_div(rows, 4) : rows, most);
 }
 
@@ -380,49 +416,65 @@ int with_types(int dtype, int r_dtype, F&& f) {
   return r_dtype == kF32 ? f(f16_t{}, float{}) : f(f16_t{}, f16_t{});
 }
 
+template <class T, class R, bool kRes, bool kCodes, bool kWhole>
+void pick_forward(const Plan& p, const Forward& f, dim3 grid, hipStream_t s) {
+  auto is = [&](int t, int u) { return p.tpr == t && p.u == u; };
+  if (is(64, 1))
+    forward_kernel<T, R, kRes, kCodes, 64, 1, kWhole><<<grid, 256, 0, s>>>(f);
+  else if (is(64, 2))
+    forward_kernel<T, R, kRes, kCodes, 64, 2, kWhole><<<grid, 256, 0, s>>>(f);
+  else if (is(256, 1))
+    forward_kernel<T, R, kRes, kCodes, 256, 1, kWhole><<<grid, 256, 0, s>>>(f);
+  else if (is(256, 2))
+    forward_kernel<T, R, kRes, kCodes, 256, 2, kWhole><<<grid, 256, 0, s>>>(f);
+  else if (is(1024, 1))
+    forward_kernel<T, R, kRes, kCodes, 1024, 1, kWhole><<<grid, 1024, 0, s>>>(f);
+  else if (is(1024, 2))
+    forward_kernel<T, R, kRes, kCodes, 1024, 2, kWhole><<<grid, 1024, 0, s>>>(f);
+  else
+    forward_kernel<T, R, kRes, kCodes, 1024, 4, kWhole><<<grid, 1024, 0, s>>>(f);
+}
+
 template <class T, class R, bool kRes, bool kCodes>
 int launch_forward(const Forward& f, hipStream_t s) {
   const Plan p = plan(f.D);
   const dim3 grid(p.tpr == 64 ? (uint32_t)nl2k::ceil_div(f.rows, 4) : (uint32_t)f.rows);
+  if (p.tpr == 0)
+    forward_long_kernel<T, R, kRes, kCodes><<<grid, 1024, 0, s>>>(f);
+  else if (f.D == p.tpr * p.u * 8)
+    pick_forward<T, R, kRes, kCodes, true>(p, f, grid, s);
+  else
+    pick_forward<T, R, kRes, kCodes, false>(p, f, grid, s);
+  return nl2k::check_launch("rms_norm");
+}
+
+template <class T, class R, bool kWhole>
+void pick_backward(const Plan& p, const Backward& b, dim3 grid, hipStream_t s) {
   auto is = [&](int t, int u) { return p.tpr == t && p.u == u; };
   if (is(64, 1))
-    forward_kernel<T, R, kRes, kCodes, 64, 1><<<grid, 256, 0, s>>>(f);
+    backward_kernel<T, R, 64, 1, kWhole><<<grid, 256, 0, s>>>(b);
   else if (is(64, 2))
-    forward_kernel<T, R, kRes, kCodes, 64, 2><<<grid, 256, 0, s>>>(f);
+    backward_kernel<T, R, 64, 2, kWhole><<<grid, 256, 0, s>>>(b);
   else if (is(256, 1))
-    forward_kernel<T, R, kRes, kCodes, 256, 1><<<grid, 256, 0, s>>>(f);
+    backward_kernel<T, R, 256, 1, kWhole><<<grid, 256, 0, s>>>(b);
   else if (is(256, 2))
-    forward_kernel<T, R, kRes, kCodes, 256, 2><<<grid, 256, 0, s>>>(f);
-  else if (is(256, 4))
-    forward_kernel<T, R, kRes, kCodes, 256, 4><<<grid, 256, 0, s>>>(f);
-  else if (is(1024, 2))
-    forward_kernel<T, R, kRes, kCodes, 1024, 2><<<grid, 1024, 0, s>>>(f);
-  else if (is(1024, 4))
-    forward_kernel<T, R, kRes, kCodes, 1024, 4><<<grid, 1024, 0, s>>>(f);
+    backward_kernel<T, R, 256, 2, kWhole><<<grid, 256, 0, s>>>(b);
+  else if (is(1024, 1))
+    backward_kernel<T, R, 1024, 1, kWhole><<<grid, 1024, 0, s>>>(b);
   else
-    forward_long_kernel<T, R, kRes, kCodes><<<grid, 1024, 0, s>>>(f);
-  return nl2k::check_launch("rms_norm");
+    backward_kernel<T, R, 1024, 2, kWhole><<<grid, 1024, 0, s>>>(b);
 }
 
 template <class T, class R>
 int launch_backward(const Backward& b, hipStream_t s) {
   const Plan p = plan(b.D);
   const dim3 grid((uint32_t)backward_blocks(b.rows, b.D));
-  auto is = [&](int t, int u) { return p.tpr == t && p.u == u; };
-  if (is(64, 1))
-    backward_kernel<T, R, 64, 1><<<grid, 256, 0, s>>>(b);
-  else if (is(64, 2))
-    backward_kernel<T, R, 64, 2><<<grid, 256, 0, s>>>(b);
-  else if (is(256, 1))
-    backward_kernel<T, R, 256, 1><<<grid, 256, 0, s>>>(b);
-  else if (is(256, 2))
-    backward_kernel<T, R, 256, 2><<<grid, 256, 0, s>>>(b);
-  else if (is(256, 4))
-    backward_kernel<T, R, 256, 4><<<grid, 256, 0, s>>>(b);
-  else if (is(1024, 2))
-    backward_kernel<T, R, 1024, 2><<<grid, 1024, 0, s>>>(b);
-  else
+  if (p.tpr == 0 || p.tpr * p.u > 2048)
     backward_long_kernel<T, R><<<grid, 1024, 0, s>>>(b);
+  else if (b.D == p.tpr * p.u * 8)
+    pick_backward<T, R, true>(p, b, grid, s);
+  else
+    pick_backward<T, R, false>(p, b, grid, s);
   return nl2k::check_launch("rms_norm_backward");
 }
 

@@ -83,18 +83,24 @@ __device__ __forceinline__ Raw<T> load8(const typename Elem<T>::type* p, int cou
       r.a = *reinterpret_cast<const f32x4_u*>(p);
       r.b = *reinterpret_cast<const f32x4_u*>(p + 4);
     } else {
+      r.a = r.b = zero4();
+      if (count > 0) {  // a branch that waves whose rows are whole do not enter
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        r.a[e] = e < count ? p[e] : 0.f;
-        r.b[e] = e + 4 < count ? p[e + 4] : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          r.a[e] = e < count ? p[e] : 0.f;
+          r.b[e] = e + 4 < count ? p[e + 4] : 0.f;
+        }
       }
     }
   } else {
     if (count >= 8) {
       r.h = __builtin_bit_cast(u16x8, (u32x4)*reinterpret_cast<const u32x4_u*>(p));
     } else {
+      r.h = u16x8{};
+      if (count > 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r.h[e] = e < count ? p[e] : (unsigned short)0;
+        for (int e = 0; e < 8; ++e) r.h[e] = e < count ? p[e] : (unsigned short)0;
+      }
     }
   }
   return r;
@@ -117,7 +123,7 @@ __device__ __forceinline__ void store8(typename Elem<T>::type* p, int count, con
     if (count >= 8) {
       *reinterpret_cast<f32x4_u*>(p) = f32x4{v[0], v[1], v[2], v[3]};
       *reinterpret_cast<f32x4_u*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-    } else {
+    } else if (count > 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (e < count) p[e] = v[e];
@@ -128,7 +134,7 @@ __device__ __forceinline__ void store8(typename Elem<T>::type* p, int count, con
     for (int e = 0; e < 8; ++e) h[e] = narrow<T>(v[e]);
     if (count >= 8) {
       *reinterpret_cast<u32x4_u*>(p) = __builtin_bit_cast(u32x4, h);
-    } else {
+    } else if (count > 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (e < count) p[e] = h[e];

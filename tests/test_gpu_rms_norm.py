@@ -12,7 +12,8 @@ from oracle import layers as ol
 pytestmark = pytest.mark.gpu
 
 # the kernels change at 512, 1024, 2048, 4096, 8192, 16384 and 32768
-WIDTHS = [1, 2, 7, 8, 9, 64, 127, 513, 1000, 1024, 1025, 2049, 4100, 8192, 8193, 16385, 32769, 40003]
+WIDTHS = [1, 2, 7, 8, 9, 64, 127, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4100, 8192, 8193,
+          16384, 16385, 32768, 32769, 40003]
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # x, residual (None: without), weight
 KINDS = [(torch.float32, None, torch.float32), (torch.float32, torch.float32, torch.bfloat16),
