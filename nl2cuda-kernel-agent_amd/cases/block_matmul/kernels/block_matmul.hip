@@ -204,21 +204,24 @@ __device__ __forceinline__ void arrive() {
   workgroup_barrier();
 }
 
-// BM x BN tiles of WM x WN waves, two stages of 128 bytes a row in LDS.
+// BM x BN tiles of WM x WN waves, S stages of 128 bytes a row in LDS.
 //
 // A wave goes through its rows of a with all its rows of b in registers.  The last kLast rows of a
 // it keeps back: once every wave has read the stage for the last time, these are multiplied column
 // by column, and between them the next stage's rows of b come into the registers that become free.
-// So the barrier, and the reads after it, lie under products; a stage's loads have a stage's time.
+// So the barrier, and the reads after it, lie under products; a stage's loads have S - 1 stages' time.
 // The loop has no branch, without which the compiler keeps everything in registers: the last block
 // of k, inside which rows may end, is taken first and its zeros are put in before the loop, and past
 // the last stage the last one is loaded again, to where nobody reads.
 //
-// Bound by power: 8192 x 8192 x 8192 takes 425 us, 2590 TFLOP/s, at a clock that falls to 1.8 GHz,
-// the matrix cores busy 68 in 100 clocks; with 32-bit scales for tiles 456 us, for rows 512.  Scales
+// Bound by power: 8192 x 8192 x 8192 takes 410 us, 2680 TFLOP/s, at a clock that falls to 1.8 GHz,
+// the matrix cores busy 68 in 100 clocks; with 32-bit scales for tiles 454 us, for rows 510.  Scales
 // that are applied afterwards are two products behind, which hides them: 495 and 575 us at once
 // after each product.  Four waves of 128 x 128 took 445 us, b straight to registers 764.
-template <int BM, int BN, int WM, int WN, int kLast, Mode kMode, bool kFull>
+// 128 x 128 tiles, for smaller products, wait for LDS: eight waves and four stages take 19 us for
+// 512 x 4096 x 4096 and 35 for 3000 x 1000 x 8192, with two stages 24 and 44, four waves with two or
+// four stages 26 and 47.  256 x 128 with three stages 36 us for 2048 x 4096 x 4096, with two 37.
+template <int BM, int BN, int WM, int WN, int kLast, int S, Mode kMode, bool kFull>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   constexpr int kWaves = WM * WN;
   constexpr int kRowsAll = BM + BN;
@@ -232,7 +235,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
                     BM % 64 == 0 && BN % 64 == 0 && kLast > 1 && kLast <= MT,
                 "tile shape");
   constexpr int kBytes = kMode == kHardware ? 1 : 4;  // of a scale
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
   const int lane = threadIdx.x & 63, group = lane >> 4, piece = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -294,8 +297,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   }
   const int64_t a_step = g.a.s_block, b_step = g.b.s_block;
   const uint32_t lds0 = offset_of(lds);
-  auto load_some = [&](int s, int q0, int q1) {
-    const uint32_t to = lds0 + (s & 1) * kStage;
+  auto load_some = [&](uint32_t stage, int q0, int q1) {
+    const uint32_t to = lds0 + stage;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q)
       if (q >= q0 && q < q1)
@@ -303,8 +306,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
                    __builtin_amdgcn_readfirstlane(to + (q * kWaves + wave) * 1024));
   };
   // the scales, and on to the next block: after the last the first
-  auto load_rest = [&](int s) {
-    const uint32_t to = lds0 + (s & 1) * kStage;
+  auto load_rest = [&](uint32_t stage, int s) {
+    const uint32_t to = lds0 + stage;
     const int64_t by = s == 0 ? 1 - steps : s + 1 < steps ? 1 : 0;
 #pragma unroll
     for (int q = 0; q < kScaleLoads; ++q) {
@@ -334,8 +337,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
   constexpr int kB = scales_of_b<kMode, kFull>();
   Operand<kFull> fb[NT], fa[kLast];  // row m of a in fa[m % kLast]
   uint32_t sb[NT][kB], sa[kLast];
-  auto get_b = [&](int s, int n) {
-    const int stage = (s & 1) * kStage;
+  auto get_b = [&](int stage, int n) {
     const uint32_t* scales = reinterpret_cast<const uint32_t*>(lds + stage + kCodes) + BM;
     fb[n] = operand<kFull>(
         read_row(fb0 + stage + ((n >> 2) * 64 + 4 * (n & 3)) * 128, group, kb));
@@ -345,8 +347,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
           scales[kMode == kTiles ? wj + (n >> 2) * 64
                                  : (kB == 1 ? row_of_b(n, piece) : row_of_b(n, 4 * group) + r)]);
   };
-  auto get_a = [&](int s, int m) {
-    const int stage = (s & 1) * kStage;
+  auto get_a = [&](int stage, int m) {
     fa[m % kLast] = operand<kFull>(read_row(fa0 + stage + m * 2048, group, ka));
     sa[m % kLast] = ready<kMode, kFull>(
         reinterpret_cast<const uint32_t*>(lds + stage + kCodes)[wi + m * 16 + piece]);
@@ -387,10 +388,13 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) off[q] += past_end(q);
   }
-  load_rest(0);
-  arrive<0>();
-  load_some(1, 0, kLoads);
-  load_rest(1);
+  load_rest(0, 0);
+#pragma unroll
+  for (int s = 1; s < S; ++s) {
+    load_some(s * kStage, 0, kLoads);
+    load_rest(s * kStage, s);
+  }
+  arrive<(S - 1) * (kLoads + kScaleLoads)>();
   if (left < 128) {  // zeros where rows have ended
     for (int i = threadIdx.x; i < kRowsAll * 8; i += 64 * kWaves) {
       const int row = i >> 3;
@@ -404,28 +408,29 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) get_b(0, n);
   for (int s = 0; s < steps; ++s) {
+    const int at = s % S * kStage, next = (s + 1) % S * kStage;
 #pragma unroll
     for (int m = 0; m < MT - kLast; ++m) {
-      get_a(s, m + 1);
+      get_a(at, m + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < NT; ++n) multiply(m * NT + n);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int m = MT - kLast + 1; m < MT; ++m) get_a(s, m);
-    arrive<0>();
+    for (int m = MT - kLast + 1; m < MT; ++m) get_a(at, m);
+    arrive<(S - 2) * (kLoads + kScaleLoads)>();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      load_some(s + 2, n * kLoads / NT, (n + 1) * kLoads / NT);
+      load_some(at, n * kLoads / NT, (n + 1) * kLoads / NT);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int m = 0; m < kLast; ++m) multiply(kFirst + n * kLast + m);
       __builtin_amdgcn_sched_barrier(0);
-      get_b(s + 1, n);
-      if (n == NT - 1) get_a(s + 1, 0);
+      get_b(next, n);
+      if (n == NT - 1) get_a(next, 0);
     }
-    load_rest(s + 2);
+    load_rest(at, s + S);
     if constexpr (kLater) {
 #pragma unroll
       for (int j = MT * NT - kBehind; j < MT * NT; ++j) retire(j);
@@ -725,16 +730,19 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool full) {
     return divide(kThin, 64, 16, std::min(256 / n16, steps / 32));
   }
   // Microseconds of a stage on an idle chip, and on one whose every CU has a tile, or two of the
-  // 128-wide ones; with scales in 8 bits.  Products in full precision leave registers for those alone.
+  // precise ones, whose products leave registers for 128 x 128 alone; what a tile begins and ends
+  // with; all with scales in 8 bits.  Measured against the others in us, 256 x 256, 256 x 128 and
+  // 128 x 128: 4096 x 4096 x 4096 58, 71, 85; 2048 x 4096 x 4096 47, 38, 43; 1024 x 4096 x 4096 45,
+  // 29, 23; 256 x 8192 x 8192 with k in two parts 55, 38, 31, whole 80, 48, 32.
   struct Tile {
     Kernel kernel;
     int bm, bn, a_round;
-    double idle, busy;
+    double idle, busy, once;
   };
-  static const Tile kFast[] = {{kTile256, 256, 256, 256, 1.2, 1.6},
-                               {kTile256x128, 256, 128, 256, 0.72, 1.0},
-                               {kTile128, 128, 128, 512, 0.65, 1.15}};
-  static const Tile kPrecise[] = {{kTile128, 128, 128, 512, 1.35, 2.4}};
+  static const Tile kFast[] = {{kTile256, 256, 256, 256, 1.2, 1.7, 5.5},
+                               {kTile256x128, 256, 128, 256, 0.72, 1.1, 4.0},
+                               {kTile128, 128, 128, 256, 0.47, 0.65, 2.5}};
+  static const Tile kPrecise[] = {{kTile128, 128, 128, 512, 1.35, 2.4, 2.5}};
   Plan best{};
   double least = 1e30;
   for (int i = 0; i < (full ? 1 : 3); ++i) {
@@ -743,7 +751,7 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool full) {
       const Plan p = divide(t.kernel, t.bm, t.bn, wanted);
       const int64_t n = p.blocks * p.parts, rounds = nl2k::ceil_div(n, t.a_round);
       const double share = t.a_round == 256 ? std::min(n / 256.0, 1.0) : (n > 256 ? 1.0 : 0.0);
-      double us = (double)(rounds * p.per) * (t.idle + (t.busy - t.idle) * share);
+      double us = (double)rounds * (p.per * (t.idle + (t.busy - t.idle) * share * share) + t.once);
       // the parts' sums: a launch, and their bytes
       if (p.parts > 1) us += 3.0 + 2e-6 * (double)p.parts * (double)(M * N);
       if (us < least) least = us, best = p;
@@ -778,13 +786,14 @@ int launch(const Args& g, const Plan& p, hipStream_t s) {
       slim_kernel<3, 4, kMode, kFull><<<grid, 256, 0, s>>>(g);
     else
       slim_kernel<4, 4, kMode, kFull><<<grid, 256, 0, s>>>(g);
+  } else if constexpr (kFull) {  // 16 bits an operand do not leave registers for more
+    tile_kernel<128, 128, 2, 2, 2, 2, kMode, kFull><<<tiles, 256, 0, s>>>(g);
   } else if (p.kernel == kTile128) {
-    tile_kernel<128, 128, 2, 2, 2, kMode, kFull><<<tiles, 256, 0, s>>>(g);
-  } else if constexpr (!kFull) {  // 16 bits an operand do not leave registers for more
-    if (p.kernel == kTile256x128)
-      tile_kernel<256, 128, 4, 2, 2, kMode, kFull><<<tiles, 512, 0, s>>>(g);
-    else
-      tile_kernel<256, 256, 2, 4, 3, kMode, kFull><<<tiles, 512, 0, s>>>(g);
+    tile_kernel<128, 128, 4, 2, 2, 4, kMode, kFull><<<tiles, 512, 0, s>>>(g);
+  } else if (p.kernel == kTile256x128) {
+    tile_kernel<256, 128, 4, 2, 2, 3, kMode, kFull><<<tiles, 512, 0, s>>>(g);
+  } else {
+    tile_kernel<256, 256, 2, 4, 3, 2, kMode, kFull><<<tiles, 512, 0, s>>>(g);
   }
   int st = nl2k::check_launch("block_matmul");
   if (st || p.parts == 1) return st;

@@ -83,9 +83,14 @@ def test_many_tiles(tiles, scale_dtype):
     (17, 16390, 1030),        # few rows, many numbers of b: stages, one part
     (40, 4099, 4111),         # and parts of k
     (64, 1200, 14345),
-    (1300, 3100, 515),        # tiles of 128
-    (2100, 4000, 300),        # of 256 x 128
+    (520, 2100, 515),         # tiles of 128, with fewer blocks than stages and more
+    (300, 1100, 1111),
+    (65, 130, 384),
+    (1300, 3100, 515),        # of 256 x 128
+    (2100, 3000, 900),
+    (2100, 4000, 300),
     (4100, 4000, 130),        # of 256
+    (3500, 4000, 600),
 ])
 def test_every_kernel(m, n, k, tiles, scale_dtype):
     """Sizes that take each kernel, ragged at every end: all against 64 bits, 16-bit results also
