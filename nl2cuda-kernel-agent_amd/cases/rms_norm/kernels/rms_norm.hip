@@ -483,7 +483,10 @@ int check_sizes(const char* who, int64_t rows, int64_t D, int dtype, int r_dtype
   if (rows < 0 || D < 1)
     return nl2k::fail(NL2K_ERR_SHAPE, "%s: need rows >= 0 and D >= 1 (got %lld, %lld)", who,
                       (long long)rows, (long long)D);
-  if (D > INT32_MAX - 16384 || rows > nl2k::max_blocks(1024) || (rows && D > INT64_MAX / 8 / rows))
+  const Plan p = plan(D);
+  const int64_t blocks = p.tpr == 64 ? nl2k::ceil_div(rows, 4) : rows;
+  if (D > INT32_MAX - 16384 || rows > INT32_MAX ||
+      blocks > nl2k::max_blocks(p.tpr == 64 || p.tpr == 256 ? 256 : 1024))
     return nl2k::fail(NL2K_ERR_OVERFLOW, "%s: sizes too large (rows=%lld D=%lld)", who,
                       (long long)rows, (long long)D);
   if (dtype < kF32 || dtype > kF16 || w_dtype < kF32 || w_dtype > kF16 ||

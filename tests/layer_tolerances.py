@@ -4,7 +4,7 @@ u = 2^-24.  Norm of D numbers: a lane adds 8 ceil(D / 8192) to 16 squares one af
 the other, then 6 lanes' steps and at most 16 waves: `adds` covers each kernel's.
 A mean's relative error is (adds + 2) u, 1 / sqrt adds two units and halves what is
 under the root.  Sums over rows: at most rows / 256 + 1 a workgroup, four waves,
-512 / 16 and 16 sums after that.
+1024 / 16 and 16 sums after that.
 
 The product: a block's 128 products and the sum of blocks in 32 bits, each
 addition off by at most a unit in the last place (2 u) of a number that the sum of
@@ -48,7 +48,7 @@ def dx_error(dy, h, weight, r, dh, dx, dtype):
 def dw_error(dy, h, r, dw, dtype):
     rows, D = h.shape
     size = (dy.double() * h * r).abs().sum(0)
-    return rounded(size * U * (rows / 256 + 60 + (adds(D) + 2) / 2 + 8), dw, dtype)
+    return rounded(size * U * (rows / 256 + 92 + (adds(D) + 2) / 2 + 8), dw, dtype)
 
 
 def largest_of_eight(a, b):

@@ -230,6 +230,43 @@ def test_special_numbers(m, scale_dtype):
     _check(out, ol.values(*(t.cpu() for t in tiny)), ol.values(*(t.cpu() for t in b)), torch.float32)
 
 
+@pytest.mark.parametrize("scale_dtype", SCALES, ids=str)
+@pytest.mark.parametrize("m", [3, 260])
+def test_rows_far_apart(m, scale_dtype):
+    """Rows the longest pitch apart: offsets within a tile of almost 32 bits."""
+    from cases.block_matmul.op import LONGEST, block_matmul
+    announce(f"block_matmul rows far apart {m} {scale_dtype}")
+    n, k, far = 300, 200, 2 * LONGEST
+    ((a, av), (b, bv)) = _operands(m, n, k, (False, True), scale_dtype)
+
+    def apart(c):
+        buf = torch.empty(len(c) * far, dtype=torch.uint8, device="cuda")
+        view = buf.as_strided(c.shape, (far, 1))
+        view.copy_(c.view(torch.uint8))
+        return view.view(torch.float8_e4m3fn)
+    ac, bc = apart(a[0]), apart(b[0])
+    assert ac.stride(0) == bc.stride(0) == far
+    _check(block_matmul(ac, a[1], bc, b[1]), av, bv, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m", [2, 66])
+def test_longest_rows(m):
+    from cases.block_matmul.op import LONGEST, block_matmul
+    announce(f"block_matmul {m} x 5 x {LONGEST}")
+    ((a, av), (b, bv)) = _operands(2, 5, LONGEST, (False, False), torch.float8_e8m0fnu)
+    pick = torch.arange(m) % 2
+    ac = a[0].view(torch.uint8)[pick.cuda()].view(torch.float8_e4m3fn)
+    asc = a[1].view(torch.uint8)[pick.cuda()].view(torch.float8_e8m0fnu)
+    out = block_matmul(ac, asc, *b, out_dtype=torch.float32)
+    assert torch.equal(out, out[:2][pick.cuda()])
+    _check(out[:2], av, bv, torch.float32)
+    with pytest.raises(RuntimeError, match="too large"):
+        block_matmul(torch.zeros(1, LONGEST + 1, device="cuda").to(torch.float8_e4m3fn),
+                     torch.ones(1, LONGEST // 128 + 1, device="cuda"),
+                     torch.zeros(1, LONGEST + 1, device="cuda").to(torch.float8_e4m3fn),
+                     torch.ones(1, LONGEST // 128 + 1, device="cuda"))
+
+
 def test_empty():
     from cases.block_matmul.op import block_linear, block_matmul
     from cases.block_quant.op import quantize_rows

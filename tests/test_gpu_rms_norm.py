@@ -319,6 +319,31 @@ def test_offsets_past_32_bits():
     _check_forward(x, None, w, y, None)
 
 
+def test_many_rows():
+    """More rows than a launch has workgroups of 1024 threads: a head's numbers each."""
+    from cases.rms_norm.op import rms_norm, rms_norm_quantized
+    rows, d, few = (1 << 22) + 4099, 64, 3
+    announce(f"rms_norm {rows} x {d}")
+    x, _, w, dy, _ = _inputs(few, d, (torch.bfloat16, None, torch.float32))
+    big = torch.zeros(rows, d, dtype=torch.bfloat16, device="cuda")
+    big[-few:] = x.cuda()
+    big.requires_grad_(True)
+    wd = w.cuda().requires_grad_(True)
+    dyd = torch.zeros_like(big)
+    dyd[-few:] = dy.cuda()
+    y = rms_norm(big, wd, eps=EPS)
+    dx, dw = torch.autograd.grad(y, (big, wd), dyd)
+    assert torch.all(y[:-few] == 0) and torch.all(dx[:-few] == 0)
+    _, wh, r = _check_forward(x, None, w, y[-few:].detach(), None)
+    _check_backward(x, None, w, dy, None, wh, r, dx[-few:], None, dw)
+    with torch.no_grad():
+        codes, scales = rms_norm_quantized(big, wd, eps=EPS)
+        last = rms_norm_quantized(big[-few:], wd, eps=EPS)
+    assert torch.equal(codes[-few:].view(torch.uint8), last[0].view(torch.uint8))
+    assert torch.equal(scales[-few:].view(torch.uint8), last[1].view(torch.uint8))
+    assert torch.all(codes[:-few].view(torch.uint8) == 0)
+
+
 def test_refusals():
     from cases.rms_norm.op import rms_norm, rms_norm_quantized
     announce("rms_norm refusals")
