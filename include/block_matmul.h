@@ -18,7 +18,8 @@
  * the 8-bit matrix instruction, which drops what lies 13 bits below the largest
  * of each eight (1.5e-5 of a result's size where rounding costs 1.7e-3); for
  * float32 results by the 16-bit one, at half its rate, which drops nothing.
- * Products of two float32 scales are formed in float32.
+ * Products of two scales are formed in float32, where they can overflow or
+ * lose bits below 2^-126; for 16-bit results powers of two are exact.
  *
  * Device arrays owned by the caller; the library allocates nothing, keeps no
  * state, never synchronises and launches on `stream`.  The workspace is

@@ -52,15 +52,18 @@ def dw_error(dy, h, r, dw, dtype):
 
 
 def largest_of_eight(a, b):
-    """sum over each eight products of a row of a and one of b of the largest."""
+    """sum over each eight products of a row of a and one of b of the largest.  In float32, of
+    rows' numbers over a power of two that brings the operand's largest to 1 to 2: exact, and
+    (x / p)(y / q) p q = x y, so that operands beyond float32's range have a bound too."""
     pad = (0, -a.shape[1] % 8)
-    a, b = (torch.nn.functional.pad(t.abs().float(), pad) for t in (a, b))
+    tops = [2.0 ** torch.floor(torch.log2(t.abs().max().clamp_min(1e-300))) for t in (a, b)]
+    a, b = (torch.nn.functional.pad((t.abs() / top).float(), pad) for t, top in zip((a, b), tops))
     out = torch.empty(a.shape[0], b.shape[0], dtype=torch.float64)
     step = max(1, (1 << 24) // (b.numel() + 1))
     for i in range(0, a.shape[0], step):
         p = a[i:i + step, None] * b
         out[i:i + step] = p.view(*p.shape[:2], -1, 8).amax(-1).double().sum(-1)
-    return out * (1 + 2.0 ** -22)
+    return out * (1 + 2.0 ** -22) * (tops[0] * tops[1])
 
 
 def matmul_error(a, b, size, want, dtype):

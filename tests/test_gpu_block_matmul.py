@@ -230,6 +230,30 @@ def test_special_numbers(m, scale_dtype):
     _check(out, ol.values(*(t.cpu() for t in tiny)), ol.values(*(t.cpu() for t in b)), torch.float32)
 
 
+@pytest.mark.parametrize("m", [3, 40, 150])
+def test_scales_that_no_quantiser_gives(m):
+    """The ends of the exponents' range: 2^-127 and 2^127."""
+    from cases.block_matmul.op import block_matmul
+    announce(f"block_matmul e8m0 ends {m}")
+    n, k = 70, 400
+    ((a, _), (b, _)) = _operands(m, n, k, (False, False), torch.float8_e8m0fnu)
+    u8 = torch.uint8
+    asc, bsc = a[1].clone().view(u8), b[1].clone().view(u8)
+    bsc.copy_(torch.tensor([127, 120], dtype=u8, device="cuda")[torch.arange(n) % 2, None])
+    bsc += 100
+    asc[0] = 0
+    kinds = [(asc, bsc, 0)]
+    asc2, bsc2 = asc.clone(), bsc - 200
+    asc2[0] = 254
+    kinds.append((asc2, bsc2, 0))
+    for sa, sb, row in kinds:
+        sa, sb = sa.view(torch.float8_e8m0fnu), sb.view(torch.float8_e8m0fnu)
+        av, bv = ol.values(a[0].cpu(), sa.cpu()), ol.values(b[0].cpu(), sb.cpu())
+        for dtype in (torch.float32, torch.bfloat16):
+            out = block_matmul(a[0], sa, b[0], sb, out_dtype=dtype)
+            _check(out[row:row + 1], av[row:row + 1], bv, dtype)
+
+
 @pytest.mark.parametrize("scale_dtype", SCALES, ids=str)
 @pytest.mark.parametrize("m", [3, 260])
 def test_rows_far_apart(m, scale_dtype):
