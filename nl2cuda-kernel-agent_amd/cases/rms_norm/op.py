@@ -44,7 +44,13 @@ def _workspace_bytes(rows, D):
 
 
 def _check(x, weight, residual):
-    device = x.get_device()
+    device, shape = x.get_device(), x.shape
+    # the common case in one expression; what is wrong with another is said below
+    if (device >= 0 and weight.get_device() == device and shape and shape[-1] >= 1 and
+            weight.shape == shape[-1:] and x.dtype in e4m3.DTYPES and weight.dtype in e4m3.DTYPES and
+            (residual is None or residual.get_device() == device and residual.shape == shape and
+             (residual.dtype == x.dtype or residual.dtype == torch.float32))):
+        return device
     capi.require(device >= 0 and weight.is_cuda and (residual is None or residual.is_cuda),
                  "x, weight and residual must be GPU tensors")
     capi.require(weight.get_device() == device and
@@ -52,13 +58,9 @@ def _check(x, weight, residual):
                  "weight and residual must be on the GPU of x")
     capi.require(x.dtype in e4m3.DTYPES and weight.dtype in e4m3.DTYPES,
                  "x and weight must be float32, bfloat16 or float16")
-    shape = x.shape
     capi.require(len(shape) >= 1 and shape[-1] >= 1 and weight.shape == shape[-1:],
                  "x must be [..., D] with D >= 1 and weight [D]")
-    capi.require(residual is None or residual.shape == shape and
-                 residual.dtype in (x.dtype, torch.float32),
-                 "residual must have x's shape, and its type or float32")
-    return device
+    raise RuntimeError("residual must have x's shape, and its type or float32")
 
 
 def _inputs(x, weight, residual):

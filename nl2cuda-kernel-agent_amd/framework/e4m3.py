@@ -33,14 +33,17 @@ def pitch(n):
 def new_codes(like, lead, n):
     """Codes [*lead, n] on the GPU of ``like``, and the bytes between their rows."""
     p = (n + 15) // 16 * 16
-    codes = like.new_empty((*lead, p), dtype=CODES)
+    codes = like.new_empty(*lead, p, dtype=CODES)
     return (codes if p == n else codes[..., :n]), p
 
 
 def new_scales(like, lead, n, dtype):
     """Scales of rows of n numbers, [*lead, blocks]."""
-    scales = like.new_empty(((n + 127) // 128, *lead), dtype=dtype)
-    return scales.t() if len(lead) == 1 else scales.movedim(0, -1)
+    n = (n + 127) // 128
+    if len(lead) == 1:
+        rows = lead[0]
+        return like.new_empty_strided((rows, n), (1, rows), dtype=dtype)
+    return like.new_empty(n, *lead, dtype=dtype).movedim(0, -1)
 
 
 def rows_of(x):
