@@ -119,14 +119,17 @@ constexpr int scales_of_b() {
   return kMode == kTiles || !applied_later<kMode, kFull>() ? 1 : 4;
 }
 
+__device__ __forceinline__ float as_float(uint32_t bits) {
+  return __builtin_bit_cast(float, bits);
+}
+
 // A scale as it is read, for the instruction or as the bits of what sums are multiplied by.
 template <Mode kMode, bool kFull>
 __device__ __forceinline__ uint32_t ready(uint32_t kept) {
   if constexpr (kMode != kHardware || !kFull) return kept;
-  return kept == 255 ? 0x7fc00000u : (kept ? kept << 23 : 0x00400000u);
-}
-__device__ __forceinline__ float as_float(uint32_t bits) {
-  return __builtin_bit_cast(float, bits);
+  // 2^-127 is half of what `kept` << 23 begins with, and infinity times 0 makes 255 a NaN
+  const float f = as_float(max(kept << 23, 0x00400000u));
+  return __builtin_bit_cast(uint32_t, fmaf(f, 0.f, f));
 }
 
 // A block's products, without scales.
@@ -221,8 +224,12 @@ __device__ __forceinline__ void arrive() {
 // 128 x 128 tiles, for smaller products, wait for LDS: eight waves and four stages take 19 us for
 // 512 x 4096 x 4096 and 35 for 3000 x 1000 x 8192, with two stages 24 and 44, four waves with two or
 // four stages 26 and 47.  256 x 128 with three stages 36 us for 2048 x 4096 x 4096, with two 37.
+// Precise products are bound by vector instructions, 128 conversions, 64 additions and 16 or 64
+// multiplications of scales for 64 matrix instructions: 8192 x 8192 x 8192 1015 us, with 32-bit
+// scales for tiles 960.  The second number of __launch_bounds__ leaves a wave no registers but those
+// that vector instructions read, without which each sum is moved there: 1072 us for 1144, and 962 for 1029.
 template <int BM, int BN, int WM, int WN, int kLast, int S, Mode kMode, bool kFull>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Args g) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Args g) {
   constexpr int kWaves = WM * WN;
   constexpr int kRowsAll = BM + BN;
   constexpr int kCodes = kRowsAll * 128;
@@ -742,7 +749,7 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool full) {
   static const Tile kFast[] = {{kTile256, 256, 256, 256, 1.2, 1.7, 5.5},
                                {kTile256x128, 256, 128, 256, 0.72, 1.1, 4.0},
                                {kTile128, 128, 128, 256, 0.47, 0.65, 2.5}};
-  static const Tile kPrecise[] = {{kTile128, 128, 128, 512, 1.35, 2.4, 2.5}};
+  static const Tile kPrecise[] = {{kTile128, 128, 128, 512, 1.25, 2.1, 2.5}};
   Plan best{};
   double least = 1e30;
   for (int i = 0; i < (full ? 1 : 3); ++i) {

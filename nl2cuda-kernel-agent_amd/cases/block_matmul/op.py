@@ -121,7 +121,7 @@ def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
     both.  Codes in another layout than the quantisers' are copied.  Sums are
     held in float32.  A 16-bit result is off by 1.5e-5 of its size before it is
     rounded, which is what the 8-bit matrix instruction's additions cost; a
-    float32 one takes the 16-bit instruction, half as fast, and has its 24 bits.
+    float32 one takes the 16-bit instruction, 2.5 times as long, and has its 24 bits.
     """
     device = a.get_device()
     capi.require(device >= 0 and a_scales.is_cuda and b.is_cuda and b_scales.is_cuda,
