@@ -17,7 +17,8 @@
 // the 16-bit one).  That is a hundredth of what rounding to 16 bits costs, so
 // 16-bit results are computed with it.  For 32-bit results the codes become
 // bfloat16, which holds them exactly, and the 16-bit instruction, at half the
-// rate, keeps every product whole.
+// rate, keeps every product whole; with the conversions it takes 2.5 times as
+// long.
 
 #include "block_matmul.h"
 
@@ -731,10 +732,18 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool full) {
   };
   if (M <= 64) {
     const int64_t n64 = nl2k::ceil_div(N, 64), n16 = nl2k::ceil_div(N, 16);
-    // below 2^24 numbers of b a workgroup for every 16 rows of it is faster: 5.6 us for 7.7 at 37
-    // rows times 2048 x 2048
-    if (M > 16 && N * K > (int64_t)1 << 24) return divide(kSlim, 64, 64, 256 / n64);
-    return divide(kThin, 64, 16, std::min(256 / n16, steps / 32));
+    // A workgroup for every 16 rows of b has more of them in the air, one for every 64 reads a less
+    // often; us, the first against the second: 37 rows times 2048 x 2048 5.5, 7.2, 4096 x 14336 24.7,
+    // 15.6; 16 rows times 8192 x 8192 17.3, 14.4, 28672 x 8192 58, 45, 6000 x 6000 11.2, 11.9.  Where
+    // the second are one round of the CUs, fewer rows too: 8 times 14336 x 4096 14.5, 10.9, one 12.2,
+    // 11.1; but one times 11008 x 4096 (two thirds of a round, 32-bit scales) 10.2, 11.2, times 28672 x
+    // 4096 22.1, 24.6.
+    const bool one_round = n64 > 200 && n64 <= 256 && N * K >= (int64_t)1 << 25;
+    if (one_round || (M > 8 && N * K > (int64_t)(M > 16 ? 2 : 5) << 23))
+      return divide(kSlim, 64, 64, 256 / n64);
+    // parts of k as CUs are idle, but no shorter than pays for the second launch: 64 rows times 512 x
+    // 16384 in 8 parts 12.0, in 4 15.1; 17 times 2048 x 4096 in one part 6.4, in two 7.0
+    return divide(kThin, 64, 16, std::min(256 / n16, steps / (M > 32 ? 16 : 30)));
   }
   // Microseconds of a stage on an idle chip, and on one whose every CU has a tile, or two of the
   // precise ones, whose products leave registers for 128 x 128 alone; what a tile begins and ends

@@ -402,7 +402,9 @@ Plan plan(int64_t D) {
 
 // Workgroups of a backward: each has a row of the workspace that the second kernel reads, and must be
 // enough of them to have the memory busy.  Rows of up to 256 numbers leave most of a wave's lanes idle:
-// 65536 x 256 33.6 us with 512 workgroups, 27.8 with 1024, where 32768 x 1024 has 43 either way.
+// 65536 x 256 33.6 us with 512 workgroups, 27.8 with 1024, where 8192 x 4096 has 43.4 and 48.9.
+// Workgroups of 1024 threads are one a CU: 999 x 5121 float32 18.8 with 256, 21.9 with 512, 2048 x
+// 16384 51.8 and 60.1.
 int64_t backward_blocks(int64_t rows, int64_t D) {
   const Plan p = plan(D);
   const int64_t most = p.tpr == 1024 || p.tpr == 0 ? 256 : D <= 256 ? 1024 : 512;

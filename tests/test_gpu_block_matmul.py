@@ -80,7 +80,11 @@ def test_many_tiles(tiles, scale_dtype):
 @pytest.mark.parametrize("m,n,k", [
     (16, 16390, 1030),        # a token or a few: two blocks at a time, and one
     (1, 700, 16500),
+    (50, 500, 9000),
     (17, 16390, 1030),        # few rows, many numbers of b: stages, one part
+    (1, 14000, 2500),
+    (13, 5000, 10300),
+    (9, 13000, 2700),
     (40, 4099, 4111),         # and parts of k
     (64, 1200, 14345),
     (520, 2100, 515),         # tiles of 128, with fewer blocks than stages and more
