@@ -930,8 +930,14 @@ struct Place {
   int64_t pitch, row, block;  // of codes in bytes, of scales in numbers
 };
 
+// For M rows of x.  Tiles read 128 bytes of a row at a time: rows from multiples of 128 on are a line
+// each, 4096 x 4096 x 2050 with 32-bit scales 40.3 us for 46.0, 1000 x 1111 x 2050 14.9 for 16.1; few
+// rows are read as they come, 3 x 5000 x 5000 9.0 us for 10.7 (5120 bytes apart).
 struct Scratch {
+  const int64_t unit;
   size_t bytes = 0;
+  explicit Scratch(int64_t M) : unit(M > 64 ? 128 : 16) {}
+  int64_t pitch(int64_t n) const { return nl2k::ceil_div(n, unit) * unit; }
   size_t take(size_t n) {
     const size_t at = bytes;
     bytes += (n + 255) / 256 * 256;
@@ -940,7 +946,7 @@ struct Scratch {
   // of rows' blocks, scales blocks first
   Place rows(int64_t m, int64_t k, int scale_type) {
     Place p{};
-    p.pitch = nl2k::ceil_div(k, 16) * 16;
+    p.pitch = pitch(k);
     p.codes = take((size_t)m * p.pitch);
     p.scales = take((size_t)nl2k::ceil_div(k, kBlock) * m * scale_bytes(scale_type));
     p.row = 1, p.block = m;
@@ -954,11 +960,11 @@ struct Kept {
   size_t bytes;
 };
 Kept kept_layout(int64_t M, int64_t N, int64_t K, int scale_type, bool dx, bool dw) {
-  Scratch s;
+  Scratch s(M);
   Kept k{};
   if (dw) k.xt = s.rows(K, M, scale_type);
   if (dx) {
-    k.wt.pitch = nl2k::ceil_div(N, 16) * 16;
+    k.wt.pitch = s.pitch(N);
     k.wt.codes = s.take((size_t)K * k.wt.pitch);
     k.wt.scales = s.take((size_t)nl2k::ceil_div(N, kBlock) * nl2k::ceil_div(K, kBlock) *
                          scale_bytes(scale_type));
@@ -973,10 +979,10 @@ struct ForwardScratch {
   size_t product, bytes;
 };
 ForwardScratch forward_layout(int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype) {
-  Scratch s;
+  Scratch s(M);
   ForwardScratch f{};
   f.x = s.rows(M, K, scale_type);
-  f.w.pitch = nl2k::ceil_div(K, 16) * 16;
+  f.w.pitch = s.pitch(K);
   f.w.codes = s.take((size_t)N * f.w.pitch);
   f.w.scales = s.take((size_t)nl2k::ceil_div(N, kBlock) * nl2k::ceil_div(K, kBlock) *
                       scale_bytes(scale_type));
@@ -992,7 +998,7 @@ struct BackwardScratch {
 };
 BackwardScratch backward_layout(int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype,
                                 int w_dtype) {
-  Scratch s;
+  Scratch s(M);
   BackwardScratch b{};
   b.dy = s.rows(M, N, scale_type);
   b.dyt = s.rows(N, M, scale_type);
