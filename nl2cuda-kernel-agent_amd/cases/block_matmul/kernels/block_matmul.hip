@@ -576,69 +576,93 @@ __global__ __launch_bounds__(256) void slim_kernel(Args g) {
   }
 }
 
-// Few rows of a: 16 rows of b a workgroup, straight to registers, its eight waves taking U blocks of
-// k in turn, the next ones on their way, and their sums added at the end in a fixed order.  Bound by
-// the reading of b: one row times 8192 x 4096 7.6 us (4.4 TB/s), times 4096 x 14336 12.2 (4.8).
+// Few rows, or small products: MT times 16 rows of a and NT times 16 of b a workgroup, straight to
+// registers, its eight waves taking U blocks of k in turn, the next ones on their way, and their sums
+// added at the end in a fixed order.  Few rows are bound by the reading of b: one row times 8192 x
+// 4096 7.7 us (4.4 TB/s), times 4096 x 14336 10.8 (5.4).  Small products are bound by the loads'
+// latency, eight blocks' at a time where tile_kernel's is each block's, who starts with 4 us of first
+// loads and barriers: 384 x 256 x 1423 5.0 us for 10.1.  64 x 64 did not fit in registers, 31 us for
+// 225 x 1125 x 3320 where 64 x 32 takes 12.
 constexpr int kThinWaves = 8;
 
-template <int MT, int U, Mode kMode, bool kFull>
+template <int MT, int NT, int U, Mode kMode, bool kFull>
 __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
-  __shared__ __attribute__((aligned(16))) float red[kThinWaves][MT * 256];
+  constexpr int kChunks = NT * 4;  // of four sums, in a row
+  __shared__ f32x4 red[kThinWaves][MT * 16 * kChunks];
   const int lane = threadIdx.x & 63, group = lane >> 4, piece = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16, part = blockIdx.y;
+  const int ta = NT > 1 ? (int)blockIdx.x / g.tiles_b : 0, part = blockIdx.y;
+  const int m0 = ta * MT * 16, n0 = ((int)blockIdx.x - ta * g.tiles_b) * NT * 16;
   const int from = part * g.per, upto = min(from + g.per, g.steps);
   const int left = g.K - (g.steps - 1) * 128;  // numbers of the last block
   const uint32_t end = (uint32_t)((g.K + 15) & ~15) - 16;
   constexpr int kB = scales_of_b<kMode, kFull>();
-  const uint8_t *pa[MT], *qa[MT], *qb[kB];
-  const uint8_t* pb = g.b.codes + (int64_t)min(n0 + piece, g.b.rows - 1) * g.b.pitch;
-#pragma unroll
-  for (int r = 0; r < kB; ++r) {
-    const int row = n0 + (kB == 4 ? 4 * group + r : (kMode == kTiles ? 0 : piece));
-    qb[r] = g.b.scales + (int64_t)(min(row, g.b.rows - 1) >> g.b.shift) * g.b.s_row;
-  }
+  const uint8_t* abase = scalar_base(g.a.codes + (int64_t)m0 * g.a.pitch);
+  const uint8_t* bbase = scalar_base(g.b.codes + (int64_t)n0 * g.b.pitch);
+  const uint8_t* sabase = scalar_base(g.a.scales + (int64_t)(m0 >> g.a.shift) * g.a.s_row);
+  const uint8_t* sbbase = scalar_base(g.b.scales + (int64_t)(n0 >> g.b.shift) * g.b.s_row);
+  // of the rows that a lane reads, and of their scales; rows past the last are copies of it
+  uint32_t offa[MT], offb[NT], sca[MT], scb[NT][kB];
+  auto scale_at = [](const Side& s, int first, int row) {
+    return (uint32_t)((row >> s.shift) - (first >> s.shift)) * (uint32_t)s.s_row;
+  };
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int row = min(m * 16 + piece, g.a.rows - 1);
-    pa[m] = g.a.codes + (int64_t)row * g.a.pitch;
-    qa[m] = g.a.scales + (int64_t)(row >> g.a.shift) * g.a.s_row;
+    const int row = min(m0 + m * 16 + piece, g.a.rows - 1);
+    offa[m] = (uint32_t)(row - m0) * (uint32_t)g.a.pitch;
+    sca[m] = scale_at(g.a, m0, row);
   }
-  auto fragment = [&](const uint8_t* p, int s) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = min(n0 + n * 16 + piece, g.b.rows - 1);
+    offb[n] = (uint32_t)(row - n0) * (uint32_t)g.b.pitch;
+#pragma unroll
+    for (int r = 0; r < kB; ++r) {
+      const int of = n0 + n * 16 + (kB == 4 ? 4 * group + r : (kMode == kTiles ? 0 : piece));
+      scb[n][r] = scale_at(g.b, n0, min(of, g.b.rows - 1));
+    }
+  }
+  auto fragment = [&](const uint8_t* base, uint32_t off, int s) {
     const uint32_t k = s * 128 + group * 16;
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(p + min(k, end));
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(p + min(k + 64, end));
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(base + (off + min(k, end)));
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(base + (off + min(k + 64, end)));
     i32x8 f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = (int)lo[i], f[4 + i] = (int)hi[i];
     return f;
   };
-  auto scale = [&](const uint8_t* p, int64_t step, int s) {
-    p += s * step;
-    return ready<kMode, kFull>(kMode == kHardware ? (uint32_t)*p
-                                                  : *reinterpret_cast<const uint32_t*>(p));
+  auto scale = [&](const uint8_t* base, uint32_t off, int64_t step, int s) {
+    const uint8_t* p = base + s * step;
+    return ready<kMode, kFull>(kMode == kHardware
+                                   ? (uint32_t)p[off]
+                                   : *reinterpret_cast<const uint32_t*>(p + off));
   };
   struct Batch {
-    i32x8 fb[U], fa[U][MT];
-    uint32_t sb[U][kB], sa[U][MT];
+    i32x8 fb[U][NT], fa[U][MT];
+    uint32_t sb[U][NT][kB], sa[U][MT];
   };
   auto fetch = [&](int s0, Batch& t) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = min(s0 + u * kThinWaves, upto - 1);
-      t.fb[u] = fragment(pb, s);
 #pragma unroll
-      for (int r = 0; r < kB; ++r) t.sb[u][r] = scale(qb[r], g.b.s_block, s);
+      for (int n = 0; n < NT; ++n) {
+        t.fb[u][n] = fragment(bbase, offb[n], s);
+#pragma unroll
+        for (int r = 0; r < kB; ++r) t.sb[u][n][r] = scale(sbbase, scb[n][r], g.b.s_block, s);
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        t.fa[u][m] = fragment(pa[m], s);
-        t.sa[u][m] = scale(qa[m], g.a.s_block, s);
+        t.fa[u][m] = fragment(abase, offa[m], s);
+        t.sa[u][m] = scale(sabase, sca[m], g.a.s_block, s);
       }
     }
   };
-  f32x4 acc[MT];
+  f32x4 acc[MT][NT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m] = nl2k::zero4();
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = nl2k::zero4();
   auto use = [&](int s0, Batch& t) {
     // All that depends on where k ends comes before the products, and a block past the end is
     // taken as zeros: no branch lies between a product and what reads it.  (Across one, hipcc of
@@ -649,7 +673,8 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
       const int s = s0 + u * kThinWaves;
       const int valid = s >= upto ? 0 : (s == g.steps - 1 ? left : 128);
       if (valid < 128) {
-        cut(t.fb[u], valid, group);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) cut(t.fb[u][n], valid, group);
 #pragma unroll
         for (int m = 0; m < MT; ++m) cut(t.fa[u][m], valid, group);
       }
@@ -657,11 +682,16 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Operand<kFull> ob = operand<kFull>(t.fb[u]);
+      Operand<kFull> ob[NT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        acc[m] =
-            block<kMode, kFull>(ob, operand<kFull>(t.fa[u][m]), acc[m], t.sb[u], t.sa[u][m]);
+      for (int n = 0; n < NT; ++n) ob[n] = operand<kFull>(t.fb[u][n]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const Operand<kFull> oa = operand<kFull>(t.fa[u][m]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          acc[m][n] = block<kMode, kFull>(ob[n], oa, acc[m][n], t.sb[u][n], t.sa[u][m]);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -677,15 +707,21 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
     use(s0, t1);
     s0 += kThinWaves * U;
   }
+  // chunks permuted by their row, so that 16 rows' lie in all banks
 #pragma unroll
   for (int m = 0; m < MT; ++m)
-    *reinterpret_cast<f32x4*>(&red[wave][m * 256 + piece * 16 + group * 4]) = acc[m];
-  __syncthreads();
-  for (int i = threadIdx.x; i < MT * 256; i += 64 * kThinWaves) {
-    float v = red[0][i];
 #pragma unroll
-    for (int w = 1; w < kThinWaves; ++w) v += red[w][i];
-    const int m = i >> 4, n = n0 + (i & 15);
+    for (int n = 0; n < NT; ++n)
+      red[wave][(m * 16 + piece) * kChunks + ((n * 4 + group) ^ (piece & (kChunks - 1)))] =
+          acc[m][n];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * 16 * kChunks * 4; i += 64 * kThinWaves) {
+    const int row = i / (kChunks * 4), col = i - row * (kChunks * 4);
+    const int at = row * kChunks + ((col >> 2) ^ (row & (kChunks - 1)));
+    float v = red[0][at][col & 3];
+#pragma unroll
+    for (int w = 1; w < kThinWaves; ++w) v += red[w][at][col & 3];
+    const int m = m0 + row, n = n0 + col;
     if (m < g.a.rows && n < g.b.rows) put1(g, part, m, n, v);
   }
 }
@@ -708,7 +744,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args g, int parts) {
 }
 
 // The kernel and the parts of k for a product's sizes.
-enum Kernel { kThin, kSlim, kTile128, kTile256x128, kTile256 };
+enum Kernel { kThin, kSmall, kSlim, kTile128, kTile256x128, kTile256 };
 
 constexpr int64_t kMostParts = 16;
 
@@ -749,25 +785,30 @@ Plan plan(int64_t M, int64_t N, int64_t K, bool full) {
   // precise ones, whose products leave registers for 128 x 128 alone; what a tile begins and ends
   // with; all with scales in 8 bits.  Measured against the others in us, 256 x 256, 256 x 128 and
   // 128 x 128: 4096 x 4096 x 4096 58, 71, 85; 2048 x 4096 x 4096 47, 38, 43; 1024 x 4096 x 4096 45,
-  // 29, 23; 256 x 8192 x 8192 with k in two parts 55, 38, 31, whole 80, 48, 32.
+  // 29, 23; 256 x 8192 x 8192 with k in two parts 55, 38, 31, whole 80, 48, 32.  64 x 32, whose stage
+  // is eight blocks of k, one for each wave, against 128 x 128: 386 x 1128 x 1581 6.0, 10.7, with
+  // float32 results 9.1, 17.5; 147 x 3085 x 5632 28, 18.
   struct Tile {
     Kernel kernel;
-    int bm, bn, a_round;
+    int bm, bn, blocks, a_round;
     double idle, busy, once;
   };
-  static const Tile kFast[] = {{kTile256, 256, 256, 256, 1.2, 1.7, 5.5},
-                               {kTile256x128, 256, 128, 256, 0.72, 1.1, 4.0},
-                               {kTile128, 128, 128, 256, 0.47, 0.65, 2.5}};
-  static const Tile kPrecise[] = {{kTile128, 128, 128, 512, 1.25, 2.1, 2.5}};
+  static const Tile kFast[] = {{kTile256, 256, 256, 1, 256, 1.2, 1.7, 7.0},
+                               {kTile256x128, 256, 128, 1, 256, 0.72, 1.1, 5.5},
+                               {kTile128, 128, 128, 1, 256, 0.47, 0.65, 4.0},
+                               {kSmall, 64, 32, 8, 256, 2.4, 2.5, 1.0}};
+  static const Tile kPrecise[] = {{kTile128, 128, 128, 1, 512, 1.25, 2.1, 4.0},
+                                  {kSmall, 64, 32, 8, 256, 3.2, 3.3, 1.0}};
   Plan best{};
   double least = 1e30;
-  for (int i = 0; i < (full ? 1 : 3); ++i) {
+  for (int i = 0; i < (full ? 2 : 4); ++i) {
     const Tile& t = full ? kPrecise[i] : kFast[i];
     for (int64_t wanted = 1; wanted <= kMostParts; ++wanted) {
       const Plan p = divide(t.kernel, t.bm, t.bn, wanted);
       const int64_t n = p.blocks * p.parts, rounds = nl2k::ceil_div(n, t.a_round);
       const double share = t.a_round == 256 ? std::min(n / 256.0, 1.0) : (n > 256 ? 1.0 : 0.0);
-      double us = (double)rounds * (p.per * (t.idle + (t.busy - t.idle) * share * share) + t.once);
+      const double stages = (double)nl2k::ceil_div(p.per, t.blocks);
+      double us = (double)rounds * (stages * (t.idle + (t.busy - t.idle) * share * share) + t.once);
       // the parts' sums: a launch, and their bytes
       if (p.parts > 1) us += 3.0 + 2e-6 * (double)p.parts * (double)(M * N);
       if (us < least) least = us, best = p;
@@ -783,18 +824,21 @@ int launch(const Args& g, const Plan& p, hipStream_t s) {
   if (p.kernel == kThin) {
     const int threads = 64 * kThinWaves;
     // two blocks at a time where a wave has three to eight: 7.6 us for 8.3 at 32 blocks of 8192 rows,
-    // but 8.3 for 7.5 at 16 of 16384 rows and 12.9 for 12.2 at 112 of 4096
-    const bool two = g.per > 2 * kThinWaves && g.per <= 8 * kThinWaves;
+    // but 8.3 for 7.5 at 16 of 16384 rows and 12.9 for 12.2 at 112 of 4096; precise ones would have
+    // registers for one workgroup a CU alone, 11.4 for 9.4 at 32 of 8192
+    const bool two = !kFull && g.per > 2 * kThinWaves && g.per <= 8 * kThinWaves;
     if (mt == 1 && two)
-      thin_kernel<1, 2, kMode, kFull><<<grid, threads, 0, s>>>(g);
+      thin_kernel<1, 1, 2, kMode, kFull><<<grid, threads, 0, s>>>(g);
     else if (mt == 1)
-      thin_kernel<1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+      thin_kernel<1, 1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
     else if (mt == 2)
-      thin_kernel<2, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+      thin_kernel<2, 1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
     else if (mt == 3)
-      thin_kernel<3, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+      thin_kernel<3, 1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
     else
-      thin_kernel<4, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+      thin_kernel<4, 1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
+  } else if (p.kernel == kSmall) {
+    thin_kernel<4, 2, 1, kMode, kFull><<<grid, 64 * kThinWaves, 0, s>>>(g);
   } else if (p.kernel == kSlim) {
     if (mt <= 2)
       slim_kernel<2, 4, kMode, kFull><<<grid, 256, 0, s>>>(g);

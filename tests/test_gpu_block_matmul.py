@@ -87,9 +87,13 @@ def test_many_tiles(tiles, scale_dtype):
     (9, 13000, 2700),
     (40, 4099, 4111),         # and parts of k
     (64, 1200, 14345),
-    (520, 2100, 515),         # tiles of 128, with fewer blocks than stages and more
-    (300, 1100, 1111),
+    (300, 1100, 1111),        # small products, with parts of k and without
     (65, 130, 384),
+    (230, 128, 6016),
+    (66, 33, 64),
+    (700, 2500, 200),         # tiles of 128, with fewer blocks than stages and more
+    (520, 2100, 515),
+    (900, 1500, 890),
     (1300, 3100, 515),        # of 256 x 128
     (2100, 3000, 900),
     (2100, 4000, 300),
