@@ -262,13 +262,16 @@ def test_scales_that_no_quantiser_gives(m):
             _check(out[row:row + 1], av[row:row + 1], bv, dtype)
 
 
-@pytest.mark.parametrize("scale_dtype", SCALES, ids=str)
-@pytest.mark.parametrize("m", [3, 260])
-def test_rows_far_apart(m, scale_dtype):
+@pytest.mark.parametrize("m,n,scale_dtype", [(3, 300, torch.float32),
+                                             (3, 300, torch.float8_e8m0fnu),
+                                             (260, 300, torch.float32),
+                                             (260, 300, torch.float8_e8m0fnu),
+                                             (700, 2100, torch.float8_e8m0fnu)])
+def test_rows_far_apart(m, n, scale_dtype):
     """Rows the longest pitch apart: offsets within a tile of almost 32 bits."""
     from cases.block_matmul.op import LONGEST, block_matmul
-    announce(f"block_matmul rows far apart {m} {scale_dtype}")
-    n, k, far = 300, 200, 2 * LONGEST
+    announce(f"block_matmul rows far apart {m} x {n} {scale_dtype}")
+    k, far = 200, 2 * LONGEST
     ((a, av), (b, bv)) = _operands(m, n, k, (False, True), scale_dtype)
 
     def apart(c):
@@ -279,6 +282,8 @@ def test_rows_far_apart(m, scale_dtype):
     ac, bc = apart(a[0]), apart(b[0])
     assert ac.stride(0) == bc.stride(0) == far
     _check(block_matmul(ac, a[1], bc, b[1]), av, bv, torch.bfloat16)
+    del ac, bc
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("m", [2, 66])
