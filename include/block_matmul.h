@@ -13,8 +13,8 @@
  * 1: exponent + 127 in a byte (e8m0, 255 NaN), for both operands.
  *
  * out: M rows of N numbers of out_dtype (0 float32, 1 bfloat16, 2 float16),
- * dense; like all that is written it overlaps nothing else.  A block's sum and the sum over blocks are held in float32; the
- * result is rounded once.  For 16-bit results a block's products are added by
+ * dense; like all that is written it overlaps nothing else.  A block's sum and
+ * the sum over blocks are held in float32; the result is rounded once.  For 16-bit results a block's products are added by
  * the 8-bit matrix instruction, which drops what lies 13 bits below the largest
  * of each eight (1.5e-5 of a result's size where rounding costs 1.7e-3); for
  * float32 results by the 16-bit one, which takes 2.5 times as long and drops

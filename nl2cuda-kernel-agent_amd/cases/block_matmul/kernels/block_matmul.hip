@@ -213,10 +213,10 @@ __device__ __forceinline__ void arrive() {
 // A wave goes through its rows of a with all its rows of b in registers.  The last kLast rows of a
 // it keeps back: once every wave has read the stage for the last time, these are multiplied column
 // by column, and between them the next stage's rows of b come into the registers that become free.
-// So the barrier, and the reads after it, lie under products; a stage's loads have S - 1 stages' time.
-// The loop has no branch, without which the compiler keeps everything in registers: the last block
-// of k, inside which rows may end, is taken first and its zeros are put in before the loop, and past
-// the last stage the last one is loaded again, to where nobody reads.
+// So the barrier, and the reads after it, lie under products; a stage's loads have S - 1 stages'
+// time.  The loop has no branch, since with one the compiler no longer keeps everything in registers:
+// the last block of k, inside which rows may end, is taken first and its zeros are put in before the
+// loop, and past the last stage the last one is loaded again, to where nobody reads.
 //
 // Bound by power: 8192 x 8192 x 8192 takes 410 us, 2680 TFLOP/s, at a clock that falls to 1.8 GHz,
 // the matrix cores busy 68 in 100 clocks; with 32-bit scales for tiles 454 us, for rows 510.  Scales
@@ -228,7 +228,8 @@ __device__ __forceinline__ void arrive() {
 // Precise products are bound by vector instructions, 128 conversions, 64 additions and 16 or 64
 // multiplications of scales for 64 matrix instructions: 8192 x 8192 x 8192 1015 us, with 32-bit
 // scales for tiles 960.  The second number of __launch_bounds__ leaves a wave no registers but those
-// that vector instructions read, without which each sum is moved there: 1072 us for 1144, and 962 for 1029.
+// that vector instructions read, without which each sum is moved there: 1072 us for 1144, and 962
+// for 1029.
 template <int BM, int BN, int WM, int WN, int kLast, int S, Mode kMode, bool kFull>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Args g) {
   constexpr int kWaves = WM * WN;
@@ -883,7 +884,7 @@ size_t workspace_of(const Plan& p, int64_t M, int64_t N) {
 }
 
 int check_side(const char* name, const void* codes, int64_t pitch, const void* scales,
-               int64_t row_stride, int64_t block_stride, int scale_type, int64_t rows, int64_t K) {
+               int64_t row_stride, int64_t block_stride, int scale_type, int64_t K) {
   if (!codes || !scales)
     return nl2k::fail(NL2K_ERR_NULL, "block_matmul: codes and scales of %s are required", name);
   if (!nl2k::aligned16(codes) ||
@@ -899,7 +900,6 @@ int check_side(const char* name, const void* codes, int64_t pitch, const void* s
       block_stride > INT64_MAX / 16 / kLongest)
     return nl2k::fail(NL2K_ERR_SHAPE, "block_matmul: strides of the scales of %s out of range (%lld, "
                       "%lld)", name, (long long)row_stride, (long long)block_stride);
-  (void)rows;
   return NL2K_SUCCESS;
 }
 
@@ -926,9 +926,9 @@ extern "C" int block_matmul(const void* a, int64_t a_pitch, const void* a_scales
     return nl2k::fail(NL2K_ERR_VALUE, "block_matmul: out_dtype must be 0, 1 or 2 (got %d)",
                       out_dtype);
   if (M == 0 || N == 0) return nl2k::succeed();
-  if ((st = check_side("a", a, a_pitch, a_scales, a_row_stride, a_block_stride, scale_type, M, K)))
+  if ((st = check_side("a", a, a_pitch, a_scales, a_row_stride, a_block_stride, scale_type, K)))
     return st;
-  if ((st = check_side("b", b, b_pitch, b_scales, b_row_stride, b_block_stride, scale_type, N, K)))
+  if ((st = check_side("b", b, b_pitch, b_scales, b_row_stride, b_block_stride, scale_type, K)))
     return st;
   if (!out) return nl2k::fail(NL2K_ERR_NULL, "block_matmul: out is required");
   if (reinterpret_cast<uintptr_t>(out) % bytes_of(out_dtype))

@@ -210,8 +210,9 @@ struct Backward {
 // dx of a window, stored; u = h r in place of h, d = dy.
 template <class T, class R>
 __device__ __forceinline__ void gradient8(const Backward& b, int64_t row, int k, int count,
-                                          float rstd, float mean, const float (&u)[8], const float (&d)[8],
-                                          const float (&w)[8], const Raw<R>& dh) {
+                                          float rstd, float mean, const float (&u)[8],
+                                          const float (&d)[8], const float (&w)[8],
+                                          const Raw<R>& dh) {
   float v[8], add[8];
   values<R>(dh, add);
 #pragma unroll
