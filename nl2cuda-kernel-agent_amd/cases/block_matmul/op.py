@@ -66,8 +66,10 @@ def _codes(c, rows, K):
     """(codes, bytes between rows) as the kernels read them: rows a multiple of 16 bytes apart, the
     last one's memory up to the next 16; copied only if they lie otherwise."""
     whole = (K + 15) // 16 * 16
-    pitch = c.stride(0) if rows > 1 else whole
-    if ((K == 1 or c.stride(1) == 1) and pitch >= K and pitch % 16 == 0 and
+    pitch, step = c.stride()
+    if rows == 1:
+        pitch = whole
+    if ((step == 1 or K == 1) and pitch >= K and pitch % 16 == 0 and
             pitch <= 2 * LONGEST and c.data_ptr() % 16 == 0 and
             (whole == K or c.storage_offset() + (rows - 1) * pitch + whole <=
              c.untyped_storage().nbytes())):
@@ -79,14 +81,15 @@ def _codes(c, rows, K):
 
 def _scales(name, s, rows, K):
     """(scales, row stride, block stride, whether they are of tiles)."""
-    n, tiles = (K + 127) // 128, (rows + 127) // 128
-    shape = tuple(s.shape)
-    capi.require(shape == (rows, n) or shape == (tiles, n), name)
+    n, tiles, shape = (K + 127) // 128, (rows + 127) // 128, s.shape
+    of_tiles = shape == (tiles, n)
+    if not of_tiles and shape != (rows, n):
+        raise RuntimeError(name)
     row, block = s.stride()
     if row > LONGEST:
         s = s.contiguous()
         row, block = s.stride()
-    return s, row, block, int(shape[0] == tiles)
+    return s, row, block, of_tiles
 
 
 def _product(a, a_scales, b, b_scales, out, M, N, K):
@@ -123,24 +126,28 @@ def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
     rounded, which is what the 8-bit matrix instruction's additions cost; a
     float32 one takes the 16-bit instruction, 2.5 times as long, and has its 24 bits.
     """
-    device = a.get_device()
-    capi.require(device >= 0 and a_scales.is_cuda and b.is_cuda and b_scales.is_cuda,
-                 "codes and scales must be GPU tensors")
-    capi.require(device == a_scales.get_device() == b.get_device() == b_scales.get_device(),
-                 "codes and scales must be on one GPU")
-    capi.require(a.dtype == b.dtype == e4m3.CODES, "a and b must be float8_e4m3fn")
-    capi.require(a_scales.dtype == b_scales.dtype and a_scales.dtype in e4m3.SCALES,
-                 "scales must both be float32 or both float8_e8m0fnu")
-    capi.require(out_dtype in e4m3.DTYPES, "out_dtype must be float32, bfloat16 or float16")
-    shape = a.shape
-    capi.require(len(shape) >= 1 and b.dim() == 2 and shape[-1] == b.shape[1] >= 1,
-                 "a must be [..., K] and b [N, K] with K >= 1")
+    device, shape, scale_dtype = a.get_device(), a.shape, a_scales.dtype
+    # the common case in one expression; what is wrong with another is said below
+    if not (device >= 0 and
+            device == a_scales.get_device() == b.get_device() == b_scales.get_device() and
+            a.dtype == b.dtype == e4m3.CODES and scale_dtype == b_scales.dtype and
+            scale_dtype in e4m3.SCALES and out_dtype in e4m3.DTYPES and len(shape) >= 1 and
+            b.dim() == 2 and shape[-1] == b.shape[1] >= 1):
+        capi.require(device >= 0 and a_scales.is_cuda and b.is_cuda and b_scales.is_cuda,
+                     "codes and scales must be GPU tensors")
+        capi.require(device == a_scales.get_device() == b.get_device() == b_scales.get_device(),
+                     "codes and scales must be on one GPU")
+        capi.require(a.dtype == b.dtype == e4m3.CODES, "a and b must be float8_e4m3fn")
+        capi.require(scale_dtype == b_scales.dtype and scale_dtype in e4m3.SCALES,
+                     "scales must both be float32 or both float8_e8m0fnu")
+        capi.require(out_dtype in e4m3.DTYPES, "out_dtype must be float32, bfloat16 or float16")
+        raise RuntimeError("a must be [..., K] and b [N, K] with K >= 1")
     capi.require(not differentiated(a, a_scales, b, b_scales),
                  "block_matmul has no gradient: use block_linear, or torch.no_grad()")
     N, K = b.shape
     if len(shape) == 2:
-        out = a.new_empty((shape[0], N), dtype=out_dtype)
         M = shape[0]
+        out = a.new_empty(M, N, dtype=out_dtype)
     else:
         out = a.new_empty((*shape[:-1], N), dtype=out_dtype)
         capi.require(a_scales.shape == (*shape[:-1], e4m3.blocks(K)),
