@@ -78,11 +78,9 @@ def _inputs(x, weight, residual):
              weight.data_ptr(), e4m3.DTYPES[weight.dtype]), (x, weight, r), rows, D)
 
 
-def _like(t, shape, dtype):
-    """A dense tensor beside t."""
-    if t.is_contiguous() and t.dtype == dtype and t.shape == shape:
-        return torch.empty_like(t)
-    return t.new_empty(shape, dtype=dtype)
+def _dense(t):
+    """A dense tensor of t's shape and type beside it."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _forward(x, weight, residual, eps, keep):
@@ -90,8 +88,8 @@ def _forward(x, weight, residual, eps, keep):
     device = _check(x, weight, residual)
     lib = _lib()
     args, held, rows, D = _inputs(x, weight, residual)
-    y = _like(x, x.shape, x.dtype)
-    h = None if residual is None else _like(residual, x.shape, residual.dtype)
+    y = _dense(x)
+    h = None if residual is None else _dense(residual)
     rstd = x.new_empty(rows, dtype=torch.float32) if keep else None
     st = capi.launch(lib.rms_norm_forward, device, *args, y.data_ptr(),
                      0 if h is None else h.data_ptr(), rstd.data_ptr() if keep else 0, rows, D,
@@ -108,7 +106,8 @@ def _backward(dy, dh, h, weight, rstd, dtype, want_weight):
     h, rows, D, h_stride = e4m3.rows_of(h)
     # what autograd gives back of what was saved: every read lies within it
     capi.require(0 <= device == weight.get_device() == rstd.get_device() and
-                 weight.numel() == D and rstd.numel() == rows,
+                 weight.numel() == D and rstd.numel() == rows and rstd.dtype == torch.float32 and
+                 dy.dtype == dtype and (dh is None or dh.dtype == h.dtype),
                  "autograd gave back other tensors than were saved")
     if not weight.is_contiguous():
         weight = weight.contiguous()
@@ -119,8 +118,8 @@ def _backward(dy, dh, h, weight, rstd, dtype, want_weight):
     if dh is not None:
         dh, _, _, dh_stride = e4m3.rows_of(dh)
         dh_ptr = dh.data_ptr()
-    dx = _like(dy, shape, dtype)
-    dres = dx if h.dtype == dtype else _like(h, shape, h.dtype)
+    dx = _dense(dy)
+    dres = dx if h.dtype == dtype else h.new_empty(shape)
     dw_ptr = ws_ptr = ws_bytes = 0
     dw = None
     if want_weight:
@@ -188,7 +187,7 @@ def rms_norm_quantized(x, weight, residual=None, eps=1e-6, scale_dtype=torch.flo
     lead = shape[:-1]
     codes, pitch = e4m3.new_codes(x, lead, D)
     scales = e4m3.new_scales(x, lead, D, scale_dtype)
-    h = None if residual is None else _like(residual, shape, residual.dtype)
+    h = None if residual is None else _dense(residual)
     st = capi.launch(lib.rms_norm_quant, device, *args, codes.data_ptr(), pitch,
                      scales.data_ptr(), e4m3.SCALES[scale_dtype], 0 if h is None else h.data_ptr(),
                      rows, D, eps)

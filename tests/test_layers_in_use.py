@@ -124,6 +124,29 @@ def test_other_tensors_than_were_saved_are_refused(name, recorded):
         assert not [c for c in recorded if "backward" in c[0]]
 
 
+@pytest.mark.parametrize("name,which", [("rms_norm", 2), ("with_residual", 0), ("with_residual", 2),
+                                        ("linear", 0), ("prepared", 2)])
+def test_other_types_than_were_saved_are_refused(name, which, recorded):
+    """A hook that gives back fewer bytes: what would be read past them is refused."""
+    x, w = torch.randn(6, 16, requires_grad=True), torch.randn(16, requires_grad=True)
+    packed = []
+
+    def pack(t):
+        packed.append(t.detach())
+        return len(packed) - 1
+
+    def unpack(i):
+        t = packed[i]
+        return t if i != which else t.to(torch.bfloat16 if t.dtype == torch.float32 else torch.bool)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        out = CALLS[name](x, w)
+    assert which < len(packed)
+    del recorded[:]
+    with pytest.raises(RuntimeError, match="saved"):
+        out.backward(torch.ones_like(out))
+    assert not [c for c in recorded if "backward" in c[0]]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("layout", LAYOUTS)
 @pytest.mark.parametrize("name", CALLS)
