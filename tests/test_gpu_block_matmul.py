@@ -304,6 +304,31 @@ def test_longest_rows(m):
                      torch.ones(1, LONGEST // 128 + 1, device="cuda"))
 
 
+@pytest.mark.parametrize("m,n", [(70000, 32800), (3, 5000000)])
+def test_large_results(m, n):
+    """More than 2^31 numbers; more rows of b than 2^16 times 64."""
+    from cases.block_matmul.op import block_matmul
+    announce(f"block_matmul {m} x {n}")
+    ((a, av), (b, bv)) = _operands(300, 300, 16, (False, False), torch.float8_e8m0fnu)
+    u8 = torch.uint8
+
+    def spread(q, rows):
+        """Zeros, then the last of q's rows."""
+        few = min(rows, 300)
+        codes = torch.zeros(rows, 16, dtype=u8, device="cuda")
+        codes[-few:] = q[0].view(u8)[-few:]
+        scales = torch.full((rows, 1), 127, dtype=u8, device="cuda")
+        scales[-few:] = q[1].view(u8)[-few:]
+        return codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), few
+    ac, asc, rows = spread(a, m)
+    bc, bsc, cols = spread(b, n)
+    out = block_matmul(ac, asc, bc, bsc)
+    _check(out[-rows:, -cols:], av[-rows:], bv[-cols:], torch.bfloat16)
+    assert torch.all(out[:-rows] == 0) and torch.all(out[:, :-cols] == 0)
+    del out
+    torch.cuda.empty_cache()
+
+
 def test_empty():
     from cases.block_matmul.op import block_linear, block_matmul
     from cases.block_quant.op import quantize_rows

@@ -151,6 +151,25 @@ def test_offsets_past_32_bits():
     _same(*quantize_rows(buf.as_strided((2, k), (far, 1))), x, False, torch.float8_e8m0fnu)
 
 
+@pytest.mark.parametrize("what", ["rows", "tiles"])
+def test_more_than_2_to_the_31_numbers(what):
+    from cases.block_quant.op import quantize_rows, quantize_tiles
+    announce(f"quantize {what} of 140032 x 16384")
+    m, k = 1094 * 128, 16384
+    quantize = quantize_rows if what == "rows" else quantize_tiles
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    last = torch.randn(128, k, device="cuda").bfloat16()
+    x[-128:] = last
+    u8 = torch.uint8
+    codes, s, codes_t, s_t = (t.view(u8) for t in quantize(x, transposed=True))
+    want, ws, want_t, ws_t = (t.view(u8) for t in quantize(last, transposed=True))
+    assert torch.equal(codes[-128:], want) and torch.equal(codes_t[:, -128:], want_t)
+    assert torch.equal(s[-len(ws):], ws) and torch.equal(s_t[:, -1:], ws_t)
+    assert torch.all(codes[:-128] == 0) and torch.all(codes_t[:, :-128] == 0)
+    del x, codes, codes_t
+    torch.cuda.empty_cache()
+
+
 def test_another_stream():
     from cases.block_quant.op import quantize_rows
     announce("quantize on a side stream")
