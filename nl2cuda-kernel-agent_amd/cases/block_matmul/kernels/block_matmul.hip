@@ -219,15 +219,16 @@ __device__ __forceinline__ void arrive() {
 // loop, and past the last stage the last one is loaded again, to where nobody reads.
 //
 // Bound by power: 8192 x 8192 x 8192 takes 410 us, 2680 TFLOP/s, at a clock that falls to 1.8 GHz,
-// the matrix cores busy 68 in 100 clocks; with 32-bit scales for tiles 454 us, for rows 510.  Scales
+// the matrix cores busy 68 in 100 clocks; with 32-bit scales for tiles 447 us, for rows 510.  Scales
 // that are applied afterwards are two products behind, which hides them: 495 and 575 us at once
-// after each product.  Four waves of 128 x 128 took 445 us, b straight to registers 764.
+// after each product; for tiles one scale is read and one factor formed for four products, 453 us for
+// 461 then.  Four waves of 128 x 128 took 445 us, b straight to registers 764.
 // 128 x 128 tiles, for smaller products, wait for LDS: eight waves and four stages take 19 us for
 // 512 x 4096 x 4096 and 35 for 3000 x 1000 x 8192, with two stages 24 and 44, four waves with two or
 // four stages 26 and 47.  256 x 128 with three stages 36 us for 2048 x 4096 x 4096, with two 37.
-// Precise products are bound by vector instructions, 128 conversions, 64 additions and 16 or 64
+// Precise products are bound by vector instructions, 128 conversions, 64 additions and 4 or 64
 // multiplications of scales for 64 matrix instructions: 8192 x 8192 x 8192 1015 us, with 32-bit
-// scales for tiles 960.  The second number of __launch_bounds__ leaves a wave no registers but those
+// scales for tiles 937.  The second number of __launch_bounds__ leaves a wave no registers but those
 // that vector instructions read, without which each sum is moved there: 1072 us for 1144, and 962
 // for 1029.
 template <int BM, int BN, int WM, int WN, int kLast, int S, Mode kMode, bool kFull>
@@ -350,11 +351,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Args g) {
     const uint32_t* scales = reinterpret_cast<const uint32_t*>(lds + stage + kCodes) + BM;
     fb[n] = operand<kFull>(
         read_row(fb0 + stage + ((n >> 2) * 64 + 4 * (n & 3)) * 128, group, kb));
+    if constexpr (kMode == kTiles) {  // four products' rows lie in one tile
+      if (n % 4 == 0) sb[n][0] = scales[wj + n * 16];
+    } else {
 #pragma unroll
-    for (int r = 0; r < kB; ++r)
-      sb[n][r] = ready<kMode, kFull>(
-          scales[kMode == kTiles ? wj + (n >> 2) * 64
-                                 : (kB == 1 ? row_of_b(n, piece) : row_of_b(n, 4 * group) + r)]);
+      for (int r = 0; r < kB; ++r)
+        sb[n][r] = ready<kMode, kFull>(
+            scales[kB == 1 ? row_of_b(n, piece) : row_of_b(n, 4 * group) + r]);
+    }
   };
   auto get_a = [&](int stage, int m) {
     fa[m % kLast] = operand<kFull>(read_row(fa0 + stage + m * 2048, group, ka));
@@ -370,13 +374,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Args g) {
   constexpr bool kLater = applied_later<kMode, kFull>();
   constexpr int kBehind = 2;
   f32x4 ring[kBehind];
-  float factors[kBehind][kB];
+  float factors[kMode == kTiles ? MT * NT / 4 : kBehind][kB];
+  auto factor_of = [&](int j) {
+    return kMode == kTiles ? row_of(j) * (NT / 4) + col_of(j) / 4 : j % kBehind;
+  };
   auto retire = [&](int j) {
     const int m = row_of(j), n = col_of(j);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       acc[m][n][r] =
-          fmaf(factors[j % kBehind][kB == 1 ? 0 : r], ring[j % kBehind][r], acc[m][n][r]);
+          fmaf(factors[factor_of(j)][kB == 1 ? 0 : r], ring[j % kBehind][r], acc[m][n][r]);
   };
   auto multiply = [&](int j) {
     const int m = row_of(j), n = col_of(j);
@@ -384,9 +391,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Args g) {
       acc[m][n] = block<kMode, kFull>(fb[n], fa[m % kLast], acc[m][n], sb[n], sa[m % kLast]);
     } else {
       if (j >= kBehind) retire(j - kBehind);
+      if (kMode != kTiles || n % 4 == 0) {
 #pragma unroll
-      for (int r = 0; r < kB; ++r)
-        factors[j % kBehind][r] = as_float(sa[m % kLast]) * as_float(sb[n][r]);
+        for (int r = 0; r < kB; ++r)
+          factors[factor_of(j)][r] = as_float(sa[m % kLast]) * as_float(sb[n][r]);
+      }
       ring[j % kBehind] = sums<kFull>(fb[n], fa[m % kLast]);
       __builtin_amdgcn_sched_barrier(0);
     }
