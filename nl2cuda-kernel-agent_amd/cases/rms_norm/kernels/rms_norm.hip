@@ -96,9 +96,14 @@ __device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, in
     const float top = nl2k::row16_max_dpp(magnitude(v));
     const Scale s =
         f.scale_type == kScaleF32 ? scale_of<kScaleF32>(top) : scale_of<kScaleE8M0>(top);
+    u32x2 codes = pack8(v, s.inverse);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // zeros behind the row, where 0 rstd = NaN too
+      const int bits = 4 * max(min(count - 4 * i, 4), 0);  // half of them: no shift by 32
+      codes[i] &= (1u << bits << bits) - 1;
+    }
     if (count > 0 || k < (f.D + 15) / 16 * 16)
-      *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(f.y) + row * f.pitch + k) =
-          pack8(v, s.inverse);
+      *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(f.y) + row * f.pitch + k) = codes;
     if ((threadIdx.x & 15) == 0 && count > 0) {
       const int64_t at = (int64_t)(k / kBlock) * f.rows + row;
       if (f.scale_type == kScaleF32)

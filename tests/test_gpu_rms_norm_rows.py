@@ -1,0 +1,29 @@
+"""Root-mean-square norm on the GPU: what lies behind a row's codes."""
+
+import pytest
+import torch
+
+from conftest import announce
+from test_gpu_rms_norm import _gpu, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float8_e8m0fnu], ids=str)
+@pytest.mark.parametrize("d", [1, 8, 13, 40, 300, 700, 1500, 2056, 3001, 5000, 9001, 20003, 40003])
+def test_codes_behind_a_row_are_zeros(d, scale_dtype):
+    """Also behind a row whose numbers are all NaN."""
+    from cases.rms_norm.op import rms_norm_quantized
+    announce(f"rms_norm_quantized padding {d} {scale_dtype}")
+    x, res, w, _, _ = _inputs(6, d, (torch.bfloat16, torch.bfloat16, torch.float32))
+    x[1, d // 2], x[2, 0], x[4] = float("nan"), float("inf"), float("nan")
+    xd, rd, wd = _gpu(x, res, w)
+    p = -(-d // 16) * 16
+    for r in (None, rd):
+        codes, scales = rms_norm_quantized(xd, wd, r, scale_dtype=scale_dtype)[:2]
+        whole = codes.as_strided((6, p), (p, 1)).view(torch.uint8)
+        assert torch.all(whole[:, d:] == 0)
+        assert torch.isnan(codes.float()[[1, 4]]).all()
+        assert torch.isfinite(codes.float()[[0, 3, 5]]).all()
+        # blocks without a number have the least scale
+        assert torch.all(scales.float()[[1, 4]] == 2.0 ** -126)
