@@ -1,12 +1,25 @@
-"""Root-mean-square norm on the GPU: what lies behind a row's codes."""
+"""Root-mean-square norm on the GPU: backwards whose workgroups take several rows, and
+what lies behind a row's codes.  Bounds: layer_tolerances.py."""
 
 import pytest
 import torch
 
 from conftest import announce
-from test_gpu_rms_norm import _gpu, _inputs
+from test_gpu_rms_norm import _check_backward, _check_forward, _gpu, _inputs, _run
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows,d", [(1, 300), (2, 5000), (3000, 72), (2100, 700), (1500, 1500),
+                                    (600, 9000), (300, 17000)])
+def test_rows_on_both_sides_of_the_workgroups(rows, d):
+    """On both sides of where a workgroup of the backward takes more than one."""
+    announce(f"rms_norm {rows} x {d}")
+    kind = (torch.bfloat16, torch.bfloat16, torch.float32)
+    x, res, w, dy, dh = _inputs(rows, d, kind)
+    y, h, dx, dres, dw = _run(x, res, w, dy, dh)
+    _, wh, r = _check_forward(x, res, w, y, h)
+    _check_backward(x, res, w, dy, dh, wh, r, dx, dres, dw)
 
 
 @pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float8_e8m0fnu], ids=str)
