@@ -1,9 +1,11 @@
-"""Root-mean-square norm on the GPU: backwards whose workgroups take several rows, and
-what lies behind a row's codes.  Bounds: layer_tolerances.py."""
+"""Root-mean-square norm on the GPU: backwards whose workgroups take several rows,
+gradients against differences, and what lies behind a row's codes.  Bounds:
+layer_tolerances.py and layer_differences.py."""
 
 import pytest
 import torch
 
+import layer_differences as ld
 from conftest import announce
 from test_gpu_rms_norm import _check_backward, _check_forward, _gpu, _inputs, _run
 
@@ -20,6 +22,26 @@ def test_rows_on_both_sides_of_the_workgroups(rows, d):
     y, h, dx, dres, dw = _run(x, res, w, dy, dh)
     _, wh, r = _check_forward(x, res, w, y, h)
     _check_backward(x, res, w, dy, dh, wh, r, dx, dres, dw)
+
+
+@pytest.mark.parametrize("d", [4, 7])
+def test_every_gradient_against_differences(d):
+    from cases.rms_norm.op import rms_norm
+    announce(f"rms_norm differences, rows of {d}")
+    x, res, w, dy, dh = ld.inputs(2, d, d)
+    xd, rd, wd = (t.cuda().requires_grad_(True) for t in (x, res, w))
+    y, h = rms_norm(xd, wd, rd, eps=ld.EPS)
+    dx, dres, dw = torch.autograd.grad((y, h), (xd, rd, wd), (dy.cuda(), dh.cuda()))
+    assert torch.equal(dx, dres)
+    got = {"x": dx.cpu().double(), "weight": dw.cpu().double()}
+
+    def value(x, w):
+        with torch.no_grad():
+            y, h = rms_norm(x.cuda(), w.cuda(), rd.detach(), eps=ld.EPS)
+        return (y.cpu().double() * dy).sum() + (h.cpu().double() * dh).sum()
+    for (which, at), (_, bound) in ld.bounds(x, res, w, dy, dh).items():
+        up, down = (value(*ld.moved(x, w, which, at, by)) for by in (ld.STEP, -ld.STEP))
+        assert abs((up - down) / (2 * ld.STEP) - got[which][at]) <= bound
 
 
 @pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float8_e8m0fnu], ids=str)
