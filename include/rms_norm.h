@@ -17,6 +17,7 @@
  * between rows; weight [D].  Types 0 float32, 1 bfloat16, 2 float16; the
  * residual (h, dh) of x's type or float32, the weight of any.  Written arrays
  * are dense and overlap nothing else.  Pointers are aligned to their type.
+ * Up to 67108860 rows, and up to 2^31 - 16385 numbers in one.
  *
  * In 8 bits (rms_norm_quant) the output is laid out as block_quant.h's rows:
  * codes of `pitch` bytes a row, zeros up to the next multiple of 16, scales

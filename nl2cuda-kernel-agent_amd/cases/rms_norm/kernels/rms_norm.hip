@@ -443,17 +443,31 @@ void pick_forward(const Plan& p, const Forward& f, dim3 grid, hipStream_t s) {
     forward_kernel<T, R, kRes, kCodes, 1024, 4, kWhole><<<grid, 1024, 0, s>>>(f);
 }
 
+// More rows than a launch has workgroups go in several.
 template <class T, class R, bool kRes, bool kCodes>
-int launch_forward(const Forward& f, hipStream_t s) {
+int launch_forward(Forward f, hipStream_t s) {
   const Plan p = plan(f.D);
-  const dim3 grid(p.tpr == 64 ? (uint32_t)nl2k::ceil_div(f.rows, 4) : (uint32_t)f.rows);
-  if (p.tpr == 0)
-    forward_long_kernel<T, R, kRes, kCodes><<<grid, 1024, 0, s>>>(f);
-  else if (f.D == p.tpr * p.u * 8)
-    pick_forward<T, R, kRes, kCodes, true>(p, f, grid, s);
-  else
-    pick_forward<T, R, kRes, kCodes, false>(p, f, grid, s);
-  return nl2k::check_launch("rms_norm");
+  const int64_t most = p.tpr == 64 ? f.rows : nl2k::max_blocks(p.tpr == 256 ? 256 : 1024);
+  for (int64_t left = f.rows;;) {
+    const int64_t n = std::min(left, most);
+    const dim3 grid((uint32_t)(p.tpr == 64 ? nl2k::ceil_div(n, 4) : n));
+    if (p.tpr == 0)
+      forward_long_kernel<T, R, kRes, kCodes><<<grid, 1024, 0, s>>>(f);
+    else if (f.D == p.tpr * p.u * 8)
+      pick_forward<T, R, kRes, kCodes, true>(p, f, grid, s);
+    else
+      pick_forward<T, R, kRes, kCodes, false>(p, f, grid, s);
+    if (int st = nl2k::check_launch("rms_norm")) return st;
+    if ((left -= n) == 0) return NL2K_SUCCESS;
+    // scales lie blocks first: f.rows stays the number of all rows
+    auto on = [](const void* p, int64_t bytes) { return static_cast<const char*>(p) + bytes; };
+    f.x = on(f.x, n * f.x_stride * Elem<T>::bytes);
+    if (kRes) f.residual = on(f.residual, n * f.r_stride * Elem<R>::bytes);
+    if (kRes) f.h = const_cast<char*>(on(f.h, n * f.D * Elem<R>::bytes));
+    f.y = const_cast<char*>(on(f.y, kCodes ? n * f.pitch : n * f.D * Elem<T>::bytes));
+    if (kCodes) f.scales = const_cast<char*>(on(f.scales, n * scale_bytes(f.scale_type)));
+    if (f.rstd) f.rstd += n;
+  }
 }
 
 template <class T, class R, bool kWhole>
@@ -491,10 +505,8 @@ int check_sizes(const char* who, int64_t rows, int64_t D, int dtype, int r_dtype
   if (rows < 0 || D < 1)
     return nl2k::fail(NL2K_ERR_SHAPE, "%s: need rows >= 0 and D >= 1 (got %lld, %lld)", who,
                       (long long)rows, (long long)D);
-  const Plan p = plan(D);
-  const int64_t blocks = p.tpr == 64 ? nl2k::ceil_div(rows, 4) : rows;
-  if (D > INT32_MAX - 16384 || rows > INT32_MAX ||
-      blocks > nl2k::max_blocks(p.tpr == 64 || p.tpr == 256 ? 256 : 1024))
+  // four rows a workgroup of 256 threads in one launch
+  if (D > INT32_MAX - 16384 || rows > 4 * nl2k::max_blocks(256))
     return nl2k::fail(NL2K_ERR_OVERFLOW, "%s: sizes too large (rows=%lld D=%lld)", who,
                       (long long)rows, (long long)D);
   if (dtype < kF32 || dtype > kF16 || w_dtype < kF32 || w_dtype > kF16 ||

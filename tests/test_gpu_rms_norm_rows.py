@@ -1,13 +1,15 @@
 """Root-mean-square norm on the GPU: backwards whose workgroups take several rows,
-gradients against differences, and what lies behind a row's codes.  Bounds:
-layer_tolerances.py and layer_differences.py."""
+gradients against differences, what lies behind a row's codes, and sizes past a
+launch's.  Bounds: layer_tolerances.py and layer_differences.py."""
 
 import pytest
 import torch
 
 import layer_differences as ld
+import layer_tolerances as tol
 from conftest import announce
-from test_gpu_rms_norm import _check_backward, _check_forward, _gpu, _inputs, _run
+from oracle import layers as ol
+from test_gpu_rms_norm import EPS, _check_backward, _check_forward, _gpu, _inputs, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +64,51 @@ def test_codes_behind_a_row_are_zeros(d, scale_dtype):
         assert torch.isfinite(codes.float()[[0, 3, 5]]).all()
         # blocks without a number have the least scale
         assert torch.all(scales.float()[[1, 4]] == 2.0 ** -126)
+
+
+# a launch has 4.19 million workgroups of 1024 threads, 16.7 million of 256
+@pytest.mark.parametrize("rows,d", [((1 << 22) + 777, 4104), ((1 << 24) + 555, 1030)])
+def test_more_rows_than_a_launch_has_workgroups(rows, d):
+    """Rows one number apart, so that all differ in little memory; the two halves alone give the same
+    bits."""
+    from cases.rms_norm.op import rms_norm, rms_norm_quantized
+    announce(f"rms_norm {rows} x {d}")
+    g = torch.Generator().manual_seed(d)
+    buf = torch.randn(rows + d, generator=g).bfloat16().cuda()
+    w = (1 + 0.2 * torch.randn(d, generator=g)).cuda().requires_grad_(True)
+    x = buf.as_strided((rows, d), (1, 1))
+    y = rms_norm(x, w, eps=EPS)
+    pick = torch.cat([torch.arange(0, 3), torch.arange(1 << 22, (1 << 22) + 5) - 3,
+                      torch.arange(rows - 5, rows)])
+    few = torch.stack([buf[i:i + d] for i in pick.tolist()]).cpu()
+    _check_forward(few, None, w.detach().cpu(), y.detach()[pick.cuda()], None)
+    with torch.no_grad():
+        codes, scales = rms_norm_quantized(x, w, eps=EPS)
+        for a, b in ((0, rows // 2), (rows // 2, rows)):
+            assert torch.equal(rms_norm(x[a:b], w, eps=EPS), y[a:b])
+            c, s = rms_norm_quantized(x[a:b], w, eps=EPS)
+            assert torch.equal(c.view(torch.uint8), codes[a:b].view(torch.uint8))
+            assert torch.equal(s.view(torch.uint8), scales[a:b].view(torch.uint8))
+            del c, s
+    del codes, scales
+    with torch.no_grad():           # with a residual, in 32 bits
+        res = buf.float().flip(0).as_strided((rows, d), (1, 1))
+        last = slice(rows - 5000, rows)
+        for call in (rms_norm, rms_norm_quantized):
+            got, want = call(x, w, res, eps=EPS), call(x[last], w, res[last], eps=EPS)
+            for a, b in zip(got, want):
+                assert torch.equal(a[last].view(torch.uint8) if "float8" in str(a.dtype) else a[last],
+                                   b.view(torch.uint8) if "float8" in str(b.dtype) else b)
+            del got, want
+    # ones for the last rows' gradients: the others' are zeros
+    dy = torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda")
+    dy[-5:] = 1
+    (dw,) = torch.autograd.grad(y, w, dy.expand(rows, d))
+    last = few[-5:]
+    _, wh, r = ol.norm(last, w.detach().cpu(), None, EPS)
+    ones = torch.ones(5, d)
+    _, want = ol.norm_backward(ones, wh, w.detach().cpu(), r)
+    # the same additions as of all the rows, of which all but five are zeros
+    assert torch.all((dw.cpu().double() - want).abs() <= tol.dw_error(ones, wh, r, want, torch.float32))
+    del y, dy
+    torch.cuda.empty_cache()
