@@ -357,12 +357,12 @@ __global__ __launch_bounds__(1024) void backward_long_kernel(Backward b) {
   }
 }
 
-// dweight: the workgroups' sums, 16 columns a workgroup, 16 threads a column.
+// dweight: the workgroups' sums, 16 columns a workgroup, from column `first` on, 16 threads a column.
 __global__ __launch_bounds__(256) void columns_kernel(const float* __restrict__ partial, int count,
-                                                      int D, void* dw, int w_dtype) {
+                                                      int D, int first, void* dw, int w_dtype) {
   __shared__ float part[16][17];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  const int64_t col = first + (int64_t)blockIdx.x * 16 + c;
   float sum = 0.f;
   if (col < D) {
 #pragma unroll 8
@@ -630,9 +630,16 @@ extern "C" int rms_norm_backward(const void* dy, int dtype, int64_t dy_stride, c
     if (st) return st;
   }
   if (dweight) {
-    columns_kernel<<<dim3((uint32_t)nl2k::ceil_div(D, 16)), 256, 0, stream>>>(
-        b.partial, rows ? (int)backward_blocks(rows, D) : 0, (int)D, dweight, weight_dtype);
-    return nl2k::check_launch(who);
+    const int count = rows ? (int)backward_blocks(rows, D) : 0;
+    // 2^28 columns and more have more workgroups than a launch
+    const int64_t most = 16 * nl2k::max_blocks(256);
+    for (int64_t first = 0; first < D; first += most) {
+      const int64_t n = nl2k::ceil_div(std::min(D - first, most), 16);
+      columns_kernel<<<dim3((uint32_t)n), 256, 0, stream>>>(b.partial, count, (int)D, (int)first,
+                                                            dweight, weight_dtype);
+      if ((st = nl2k::check_launch(who))) return st;
+    }
+    return st;
   }
   return nl2k::succeed();
 }

@@ -112,3 +112,22 @@ def test_more_rows_than_a_launch_has_workgroups(rows, d):
     assert torch.all((dw.cpu().double() - want).abs() <= tol.dw_error(ones, wh, r, want, torch.float32))
     del y, dy
     torch.cuda.empty_cache()
+
+
+def test_a_weight_gradient_of_more_columns_than_a_launch_has():
+    """More than 2^28 numbers a row, 16 a workgroup."""
+    from cases.rms_norm.op import rms_norm
+    d = (1 << 28) + 37
+    announce(f"rms_norm 1 x {d}")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(1, d, generator=g, device="cuda").bfloat16()
+    dy = torch.randn(1, d, generator=g, device="cuda").bfloat16()
+    w = torch.ones(d, device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(rms_norm(x, w, eps=EPS), w, dy)
+    r = 1 / torch.sqrt(x.double().square().mean() + EPS)
+    want = (dy.double() * x.double() * r)[0]
+    # one row: a product of three numbers, of which rstd's error is its sum's, (adds + 2) / 2
+    err = want.abs() * tol.U * ((tol.adds(d) + 2) / 2 + 8)
+    assert torch.all((dw.double() - want).abs() <= tol.rounded(err, want, torch.float32))
+    del x, dy, w, dw, want, err
+    torch.cuda.empty_cache()
