@@ -10,6 +10,7 @@ GPU the library refuses to load.
 
 import collections
 import functools
+import math
 import os
 
 import torch
@@ -120,7 +121,7 @@ def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
     [..., N] of out_dtype (float32, bfloat16 or float16); without a gradient.
 
     Scales are of rows, [..., ceil(K / 128)], or of tiles of 128 x 128,
-    [ceil(rows / 128), ceil(K / 128)]; float32 or float8_e8m0fnu, the same for
+    [ceil(M / 128), ceil(K / 128)] for M rows in all; float32 or float8_e8m0fnu, the same for
     both.  Codes in another layout than the quantisers' are copied.  Sums are
     held in float32.  A 16-bit result is off by 1.5e-5 of its size before it is
     rounded, which is what the 8-bit matrix instruction's additions cost; a
@@ -150,12 +151,14 @@ def block_matmul(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
         out = a.new_empty(M, N, dtype=out_dtype)
     else:
         out = a.new_empty((*shape[:-1], N), dtype=out_dtype)
-        capi.require(a_scales.shape == (*shape[:-1], e4m3.blocks(K)),
-                     f"a_scales must be {(*shape[:-1], e4m3.blocks(K))}, got "
-                     f"{tuple(a_scales.shape)}")
-        M = out.numel() // N if N else 0
+        M, blocks = math.prod(shape[:-1]), e4m3.blocks(K)
+        rows, tiles = (*shape[:-1], blocks), (e4m3.blocks(M), blocks)
+        capi.require(a_scales.shape == rows or a_scales.shape == tiles,
+                     f"a_scales must be {rows} or {tiles}, got {tuple(a_scales.shape)}")
         if M:
-            a, a_scales = a.reshape(M, K), a_scales.reshape(M, -1)
+            a = a.reshape(M, K)
+            if a_scales.shape == rows:
+                a_scales = a_scales.reshape(M, -1)
     if M == 0 or N == 0:
         return out
     return _product(a, a_scales, b, b_scales, out, M, N, K)
