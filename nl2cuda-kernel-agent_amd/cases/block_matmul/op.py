@@ -24,6 +24,7 @@ KERNEL_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kernels")
 LIB_NAME = "block_matmul_hip"
 SOURCES = ["block_matmul.hip"]
 LONGEST = 1 << 22     # of the kernels' offsets within a tile
+FARTHEST = 1 << 36    # scales of one row may lie apart
 
 QuantizedWeight = collections.namedtuple("QuantizedWeight", "codes scales codes_t scales_t")
 
@@ -87,9 +88,12 @@ def _scales(name, s, rows, K):
     if not of_tiles and shape != (rows, n):
         raise RuntimeError(name)
     row, block = s.stride()
-    if row > LONGEST:
-        s = s.contiguous()
-        row, block = s.stride()
+    if row > LONGEST or block > FARTHEST:
+        # strides of a dimension of one are never taken, and may be anything
+        row, block = row if shape[0] > 1 else 0, block if n > 1 else 0
+        if row > LONGEST or block > FARTHEST:
+            s = s.contiguous()
+            row, block = n, 1
     return s, row, block, of_tiles
 
 

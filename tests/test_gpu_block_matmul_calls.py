@@ -1,4 +1,5 @@
-"""Block-scaled products on the GPU: tile scales for vectors and batches."""
+"""Block-scaled products on the GPU: tile scales for vectors and batches, and a row of
+scales cut from a wide matrix."""
 
 import pytest
 import torch
@@ -22,3 +23,15 @@ def test_tile_scales_of_vectors_and_batches(lead, scale_dtype):
     assert out.shape == (*lead, 70)
     _check(out.view(m, 70), av, bv, torch.bfloat16)
     assert torch.equal(out.view(m, 70), block_matmul(*a, *b))
+
+
+def test_a_row_of_scales_of_a_wide_matrix():
+    from cases.block_matmul.op import LONGEST, block_matmul
+    announce("block_matmul scales of one row")
+    ((a, av), (b, bv)) = _operands(1, 40, 300, (False, True), torch.float32)
+    wide = [torch.zeros(2 * LONGEST + 3, device="cuda").as_strided((1, 3), (2 * LONGEST, 1))
+            for _ in range(2)]
+    for to, s in zip(wide, (a[1], b[1])):
+        to.copy_(s)
+    assert wide[0].stride(0) > LONGEST
+    _check(block_matmul(a[0], wide[0], b[0], wide[1]), av, bv, torch.bfloat16)

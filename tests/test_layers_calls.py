@@ -37,3 +37,23 @@ def test_scales_of_other_shapes_are_refused(scales, recorded):  # noqa: F811
     with pytest.raises(RuntimeError, match="a_scales must be"):
         block_matmul(_codes(2, 75, 384), torch.ones(scales), _codes(7, 384), torch.ones(7, 3))
     assert not recorded
+
+
+@pytest.mark.parametrize("m,k,shape,strides", [
+    (1, 384, (1, 3), (1 << 23, 1)),               # a row of a wide matrix
+    (100, 384, (1, 3), (1 << 40, 1)),             # a row of tiles of one
+    (5, 100, (5, 1), (1, 1 << 61)),               # one block: its stride is never taken
+    (300, 384, (3, 3), (1 << 23, 1)),             # too far apart: copied
+])
+def test_strides_of_scales_that_are_taken_are_in_range(m, k, shape, strides, recorded):  # noqa: F811
+    """A dimension of one may come with any stride; no offset is made of it."""
+    from cases.block_matmul.op import LONGEST, block_matmul
+    real = tuple(s if n > 1 else 0 for n, s in zip(shape, strides))
+    last = sum((n - 1) * s for n, s in zip(shape, real))
+    scales = torch.ones(last + 1).as_strided(shape, real)
+    scales = scales.as_strided(shape, strides)
+    block_matmul(_codes(m, k), scales, _codes(7, k), torch.ones(7, -(-k // 128)))
+    (entry, args), = recorded
+    row, block = args[3:5]
+    assert 0 <= row <= LONGEST and 0 <= block <= LONGEST
+    assert args[2] == scales.data_ptr() or shape == (3, 3)
