@@ -13,9 +13,10 @@
  * 1: exponent + 127 in a byte (e8m0, 255 NaN), for both operands.
  *
  * out: M rows of N numbers of out_dtype (0 float32, 1 bfloat16, 2 float16),
- * dense; like all that is written it overlaps nothing else.  A block's sum and
- * the sum over blocks are held in float32; the result is rounded once.  For 16-bit results a block's products are added by
- * the 8-bit matrix instruction, which drops what lies 13 bits below the largest
+ * dense; like all that is written it overlaps nothing else.  K is at most 2^22.
+ * A block's sum and the sum over blocks are held in float32; the result is
+ * rounded once.  For 16-bit results a block's products are added by the 8-bit
+ * matrix instruction, which drops what lies 13 bits below the largest
  * of each eight (1.5e-5 of a result's size where rounding costs 1.7e-3); for
  * float32 results by the 16-bit one, which takes 2.5 times as long and drops
  * nothing.
@@ -63,6 +64,8 @@ int block_matmul(const void* a, int64_t a_pitch, const void* a_scales, int64_t a
  * What a backward needs is kept by the forward in `kept`, 256-byte aligned, of
  * block_linear_kept_bytes: for dx the transposed w (unless w_codes is given),
  * for dw the transposed x.  M = 0 does nothing; dw is the caller's to clear.
+ * The numbers that a product adds are at most 2^22: K for y, N where dx is
+ * wanted, M where dw is.
  */
 size_t block_linear_kept_bytes(int64_t M, int64_t N, int64_t K, int scale_type, int want_dx,
                                int want_dw, int have_codes);

@@ -1051,28 +1051,29 @@ struct BackwardScratch {
 };
 BackwardScratch backward_layout(int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype,
                                 int w_dtype) {
+  // of what the sizes allow
+  const bool dx = !check_sizes(M, K, N), dw = !check_sizes(N, K, M);
   Scratch s(M);
   BackwardScratch b{};
   b.dy = s.rows(M, N, scale_type);
-  b.dyt = s.rows(N, M, scale_type);
+  if (dw) b.dyt = s.rows(N, M, scale_type);
   // one product after the other
-  b.product = s.take(std::max(workspace_of(plan(M, K, N, x_dtype == kF32), M, K),
-                              workspace_of(plan(N, K, M, w_dtype == kF32), N, K)));
+  b.product =
+      s.take(std::max(dx ? workspace_of(plan(M, K, N, x_dtype == kF32), M, K) : 0,
+                      dw ? workspace_of(plan(N, K, M, w_dtype == kF32), N, K) : 0));
   b.bytes = s.bytes;
   return b;
 }
 
+// Sizes that the products take which are wanted: each has its own sum, of K, of N or of M numbers.
 int check_layer(const char* who, int64_t M, int64_t N, int64_t K, int scale_type, int x_dtype,
-                int w_dtype) {
+                int w_dtype, bool dx, bool dw) {
   if (M < 0 || N < 1 || K < 1)
     return nl2k::fail(NL2K_ERR_SHAPE, "%s: need M >= 0, N, K >= 1 (got %lld, %lld, %lld)", who,
                       (long long)M, (long long)N, (long long)K);
-  if (M > kLongest || N > kLongest || K > kLongest)
+  if (check_sizes(M, N, K) || (dx && check_sizes(M, K, N)) || (dw && M && check_sizes(N, K, M)))
     return nl2k::fail(NL2K_ERR_OVERFLOW, "%s: sizes too large (M=%lld N=%lld K=%lld)", who,
                       (long long)M, (long long)N, (long long)K);
-  if (int st = check_sizes(M, N, K)) return st;
-  if (int st = check_sizes(M, K, N)) return st;
-  if (int st = M ? check_sizes(N, K, M) : 0) return st;
   if (x_dtype < kF32 || x_dtype > kF16 || w_dtype < kF32 || w_dtype > kF16 ||
       (scale_type != kScaleF32 && scale_type != kScaleE8M0))
     return nl2k::fail(NL2K_ERR_VALUE, "%s: types must be 0, 1 or 2, scale_type 0 or 1 (got %d, %d, %d)",
@@ -1093,13 +1094,15 @@ int check_scratch(const char* who, const char* name, const void* p, size_t have,
 
 extern "C" size_t block_linear_kept_bytes(int64_t M, int64_t N, int64_t K, int scale_type,
                                           int want_dx, int want_dw, int have_codes) {
-  if (check_layer("block_linear_kept_bytes", M, N, K, scale_type, 0, 0) || M == 0) return 0;
+  if (check_layer("block_linear_kept_bytes", M, N, K, scale_type, 0, 0, want_dx, want_dw) || M == 0)
+    return 0;
   return kept_layout(M, N, K, scale_type, want_dx && !have_codes, want_dw).bytes;
 }
 
 extern "C" size_t block_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int scale_type,
                                                int x_dtype, int w_dtype, int backward) {
-  if (check_layer("block_linear_workspace_bytes", M, N, K, scale_type, x_dtype, w_dtype) || M == 0)
+  if (check_layer("block_linear_workspace_bytes", M, N, K, scale_type, x_dtype, w_dtype, false, false) ||
+      M == 0)
     return 0;
   return backward ? backward_layout(M, N, K, scale_type, x_dtype, w_dtype).bytes
                   : forward_layout(M, N, K, scale_type, x_dtype).bytes;
@@ -1113,7 +1116,7 @@ extern "C" int block_linear_forward(const void* x, int x_dtype, int64_t x_stride
                                     int64_t K, void* workspace, size_t workspace_bytes,
                                     hipStream_t stream) {
   const char* who = "block_linear_forward";
-  int st = check_layer(who, M, N, K, scale_type, x_dtype, w_dtype);
+  int st = check_layer(who, M, N, K, scale_type, x_dtype, w_dtype, want_dx, want_dw);
   if (st) return st;
   if (M == 0) return nl2k::succeed();
   if (!x || !y || (!w && !w_codes) || !w_codes != !w_scales)
@@ -1151,7 +1154,7 @@ extern "C" int block_linear_backward(const void* dy, int x_dtype, int64_t dy_str
                                      int64_t K, void* workspace, size_t workspace_bytes,
                                      hipStream_t stream) {
   const char* who = "block_linear_backward";
-  int st = check_layer(who, M, N, K, scale_type, x_dtype, w_dtype);
+  int st = check_layer(who, M, N, K, scale_type, x_dtype, w_dtype, dx, dw);
   if (st) return st;
   if (M == 0 || (!dx && !dw)) return nl2k::succeed();
   const bool kept_w = dx && !w_codes_t;

@@ -1,5 +1,5 @@
-"""Block-scaled products on the GPU: tile scales for vectors and batches, and a row of
-scales cut from a wide matrix."""
+"""Block-scaled products on the GPU: tile scales for vectors and batches, a row of
+scales cut from a wide matrix, and layers of millions of tokens."""
 
 import pytest
 import torch
@@ -35,3 +35,29 @@ def test_a_row_of_scales_of_a_wide_matrix():
         to.copy_(s)
     assert wide[0].stride(0) > LONGEST
     _check(block_matmul(a[0], wide[0], b[0], wide[1]), av, bv, torch.bfloat16)
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+def test_a_layer_of_more_tokens_than_a_row_has_numbers(frozen):
+    """4.19 million is where dweight's sums end; without it the tokens are rows like any others."""
+    from cases.block_matmul.op import LONGEST, block_linear
+    m, n, k = LONGEST + 77, 24, 40
+    announce(f"block_linear {m} x {n} x {k}")
+    g = torch.Generator().manual_seed(2)
+    few = torch.randn(300, k, generator=g).bfloat16()
+    x = few.cuda().repeat(-(-m // 300), 1)[:m]
+    w = torch.randn(n, k, generator=g).cuda()
+    dy = torch.randn(300, n, generator=g).bfloat16()
+    if frozen:
+        x.requires_grad_(True)
+    y = block_linear(x, w)
+    part = x[:300].detach().requires_grad_(frozen)
+    z = block_linear(part, w)
+    assert torch.equal(y.detach(), z.detach().repeat(-(-m // 300), 1)[:m])
+    if frozen:
+        (dx,) = torch.autograd.grad(y, x, dy.cuda().repeat(-(-m // 300), 1)[:m])
+        (dp,) = torch.autograd.grad(z, part, dy.cuda())
+        assert torch.equal(dx, dp.repeat(-(-m // 300), 1)[:m])
+    with pytest.raises(RuntimeError, match="too large"):
+        block_linear(x, w.requires_grad_(True))
+    torch.cuda.empty_cache()
