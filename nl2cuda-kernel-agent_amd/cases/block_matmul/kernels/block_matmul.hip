@@ -838,7 +838,7 @@ int launch(const Args& g, const Plan& p, hipStream_t s) {
     // registers for one workgroup a CU alone, 11.4 for 9.4 at 32 of 8192
     const bool two = !kFull && g.per > 2 * kThinWaves && g.per <= 8 * kThinWaves;
     if (mt == 1 && two)
-      thin_kernel<1, 1, 2, kMode, kFull><<<grid, threads, 0, s>>>(g);
+      thin_kernel<1, 1, kFull ? 1 : 2, kMode, kFull><<<grid, threads, 0, s>>>(g);
     else if (mt == 1)
       thin_kernel<1, 1, 1, kMode, kFull><<<grid, threads, 0, s>>>(g);
     else if (mt == 2)
