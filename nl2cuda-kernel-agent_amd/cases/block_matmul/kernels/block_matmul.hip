@@ -675,9 +675,11 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(Args g) {
     for (int n = 0; n < NT; ++n) acc[m][n] = nl2k::zero4();
   auto use = [&](int s0, Batch& t) {
     // All that depends on where k ends comes before the products, and a block past the end is
-    // taken as zeros: no branch lies between a product and what reads it.  (Across one, hipcc of
-    // ROCm 7.2 left a sum's first reader two instructions behind the matrix instruction, which
-    // needs eight: sums were read before they were there.)
+    // taken as zeros, so that the products of all blocks and the scaling of their sums follow each
+    // other without a branch: in an earlier form, with one among them, sums were read before they
+    // were there.  Where the instruction applies scales, what reads its sums first lies behind the
+    // loop's exit; the compiler counts its waits across that branch, and a test reads the built
+    // kernels for them.
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u * kThinWaves;
