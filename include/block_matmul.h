@@ -16,10 +16,12 @@
  * dense; like all that is written it overlaps nothing else.  K is at most 2^22.
  * A block's sum and the sum over blocks are held in float32; the result is
  * rounded once.  For 16-bit results a block's products are added by the 8-bit
- * matrix instruction, which drops what lies 13 bits below the largest
- * of each eight (1.5e-5 of a result's size where rounding costs 1.7e-3); for
- * float32 results by the 16-bit one, which takes 2.5 times as long and drops
- * nothing.
+ * matrix instruction, which drops what lies 13 bits below the largest of each
+ * eight: a result is off by at most 7 * 2^-13 of the sum of those largest ones
+ * before it is rounded, however small it is itself.  Of random numbers that is
+ * 1.5e-5 of the results' root mean square (measured; rounding costs 1.7e-3 in
+ * bfloat16, 2.1e-4 in float16).  For float32 results they are added by the
+ * 16-bit instruction, which takes 2.5 times as long and drops nothing.
  * Products of two scales are formed in float32, where they can overflow or
  * lose bits below 2^-126; for 16-bit results powers of two are exact.
  *

@@ -1,5 +1,6 @@
 """Block-scaled products on the GPU: tile scales for vectors and batches, a row of
-scales cut from a wide matrix, and layers of millions of tokens."""
+scales cut from a wide matrix, layers of millions of tokens, and what 16-bit results
+lose beside their rounding."""
 
 import pytest
 import torch
@@ -61,3 +62,59 @@ def test_a_layer_of_more_tokens_than_a_row_has_numbers(frozen):
     with pytest.raises(RuntimeError, match="too large"):
         block_linear(x, w.requires_grad_(True))
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(64, 8192, 4096), (256, 4096, 4096), (1024, 2048, 2048),
+                                   (2048, 2048, 1024)])
+def test_what_16_bit_results_lose_as_a_whole(m, n, k, scale_dtype):
+    """Of random numbers 16-bit results are off by their rounding, and before it by what the 8-bit
+    instruction drops: e, a root mean square of 1.5e-5 of the results', here held to 2^-15, twice that.
+
+    e is seen through the rounding: it changes a result only where it carries it over a border between
+    two numbers, with a chance of |e| / step, and then moves the square of its error by 2 step a, a evenly
+    in [0, |e|]: by e^2 in the mean.  So the squares of the errors exceed those of the rounded 64-bit
+    results by the sum of e^2, give or take sqrt(4/3 step / |e| / N) of it over N results: 5 % for bfloat16
+    (step up to 2^-7) and 2 % for float16 with 2^19 of them.  Losing two bits more is four times the
+    bound."""
+    from cases.block_matmul.op import block_matmul
+    announce(f"block_matmul losses {m} x {n} x {k} {scale_dtype}")
+    ((a, av), (b, bv)) = _operands(m, n, k, (False, True), scale_dtype)
+    want = av.cuda() @ bv.cuda().t().contiguous()
+    assert want.abs().max() < 65504
+    for dtype in (torch.float16, torch.bfloat16):
+        out = block_matmul(*a, *b, out_dtype=dtype).double()
+        lost = (out - want).square().sum() - (want.to(dtype).double() - want).square().sum()
+        share = (lost / want.square().sum()).item()
+        print(f"{dtype}: {abs(share) ** 0.5:.2e}")
+        assert share <= 2.0 ** -30
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(3, 300, 1000), (12, 13000, 2700), (40, 4099, 1030), (200, 300, 1500),
+                                   (1300, 3100, 300), (3500, 4000, 200)])
+def test_what_outliers_take_from_their_eight(m, n, k, scale_dtype):
+    """In one eight of eight a product is 2^17 times the others and more, every second time beside one
+    that cancels it: only what shares its eight loses bits, and no more than the bound."""
+    from cases.block_matmul.op import block_matmul
+    announce(f"block_matmul outliers {m} x {n} x {k} {scale_dtype}")
+    g = torch.Generator().manual_seed(m + k)
+
+    def codes(rows, flip):
+        x = (0.25 + torch.rand(rows, k, generator=g)) * torch.sign(torch.randn(rows, k, generator=g))
+        at = torch.arange(3, k - 8, 64)                  # one eight of eight, at any of its places
+        at = at + torch.randint(-3, 4, at.shape, generator=torch.Generator().manual_seed(k))
+        x[:, at] = 448.0
+        pairs = at[::2]                                  # and one that cancels it, in the same eight
+        x[:, pairs // 8 * 8 + (pairs + 1) % 8] = 448.0 * flip
+        return x.to(torch.float8_e4m3fn)
+    a, b = codes(m, 1.0), codes(n, -1.0)
+    one = [torch.ones(r, -(-k // 128)).to(scale_dtype).cuda() for r in (m, -(-n // 128))]
+    av, bv = a.double(), b.double()
+    pick = [torch.unique(torch.cat([torch.arange(0, min(r, 60)), torch.arange(max(r - 60, 0), r)]))
+            for r in (m, n)]
+    for dtype in (torch.float16, torch.bfloat16):
+        # 448 * 448 a block would leave float16's range: a's scales take it back
+        out = block_matmul(a.cuda(), (one[0].float() * 2.0 ** -8).to(scale_dtype), b.cuda(), one[1],
+                           out_dtype=dtype)
+        _check(out[pick[0].cuda()][:, pick[1].cuda()], av[pick[0]] * 2.0 ** -8, bv[pick[1]], dtype)
