@@ -98,7 +98,7 @@ __device__ __forceinline__ void finish8(const Forward& f, int64_t row, int k, in
         f.scale_type == kScaleF32 ? scale_of<kScaleF32>(top) : scale_of<kScaleE8M0>(top);
     u32x2 codes = pack8(v, s.inverse);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // zeros behind the row, where 0 rstd = NaN too
+    for (int i = 0; i < 2; ++i) {  // zeros behind the row, where 0 rstd = NaN too; 8192 x 4100 48.4 -> 49.1
       const int bits = 4 * max(min(count - 4 * i, 4), 0);  // half of them: no shift by 32
       codes[i] &= (1u << bits << bits) - 1;
     }
@@ -231,8 +231,9 @@ __device__ __forceinline__ void gradient8(const Backward& b, int64_t row, int k,
 // A workgroup takes every gridDim.x-th row (or four), and adds up their share of dweight in registers;
 // columns_kernel adds the workgroups' shares, so that no atomics are needed and the order is fixed.
 // dh and rows' ends are asked for before they are loaded, not masked out of a load: without a
-// residual 16384 x 2048 56 -> 47 us, 65536 x 256 49 -> 34.  Loading the next row ahead gave nothing,
-// since the other workgroups of a CU cover the wait.
+// residual 16384 x 2048 56 -> 47 us, 65536 x 256 49 -> 34.  Loading the next row ahead gave nothing
+// where the other workgroups of a CU cover the wait; one of 1024 threads has its CU to itself, and its
+// rows' loads and sums follow one another: 999 x 5121 float32 14.3 us, its bytes 12.
 template <class T, class R, int TPR, int U, bool kWhole>
 __global__ __launch_bounds__(block_of<TPR>()) void backward_kernel(Backward b) {
   constexpr int kRows = block_of<TPR>() / TPR;
